@@ -153,6 +153,8 @@ def lib() -> C.CDLL:
         "rmsnorm_forward": (i32, [vp, vp, vp, i32, i32, f32, i32, vp, C.c_char_p, i32]),
         "rmsnorm_scratch_bytes": (C.c_int64, [i32, i32]),
         "rmsnorm_backward": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, f32, i32, vp, C.c_char_p, i32]),
+        "logprobs_forward": (i32, [vp, C.c_int64, vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, C.c_char_p, i32]),
+        "logprobs_backward": (i32, [vp, C.c_int64, vp, vp, vp, vp, vp, i32, i32, i32, vp, C.c_int64, vp, C.c_char_p, i32]),
         "moe_debug_tc_gemm": (i32, [i32, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp, vp]),
         "moe_debug_launch_count": (C.c_int64, []),
         "moe_debug_set_tc_pair": (i32, [i32]),
@@ -176,5 +178,5 @@ def exported_symbols():
     for h in sorted(os.listdir(inc)):
         if h.endswith(".h"):
             text = open(os.path.join(inc, h)).read()
-            names += re.findall(r"\b((?:moe|kv|rmsnorm|lm)_[a-z0-9_]+)\s*\(", text)
+            names += re.findall(r"\b((?:moe|kv|rmsnorm|lm|logprobs|q4_linear)_[a-z0-9_]+)\s*\(", text)
     return sorted(set(n for n in names if n not in ("moe_status", "moe_precision", "moe_weight", "lm_param", "lm_config", "lm_model", "lm_decoder")))

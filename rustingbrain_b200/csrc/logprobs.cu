@@ -1,0 +1,494 @@
+// Token log probabilities, entropy and the most likely tokens of rows of logits, and their gradient (the ABI of
+// include/logprobs_b200.h).
+//
+// Forward is one pass over the logits, bound by HBM: every thread keeps a running maximum m, s = sum 2^y and
+// t = sum y 2^y with y = (x - m) log2(e), rescaled when the maximum moves.  The entropy is then log s - t / s: both
+// terms are >= 0, so nothing cancels.  The alternatives cost no second pass: a thread remembers which of its 16-byte
+// vectors first reached its maximum, the top_n-th best of those (value, vector) pairs is a lower bound for the top_n-th best
+// logit, and only the threads above the bound (top_n of them) have their share of the row read again, by a whole
+// warp and out of L2.  What passes the bound is a few dozen values, sorted by one warp.
+//
+// One CTA takes a row.  When there are fewer rows than would fill the machine, a cluster of 2, 4 or 8 CTAs takes one and
+// joins its sums and candidate lists through distributed shared memory: still one launch and no workspace.
+
+#include <cooperative_groups.h>
+#include <cfloat>
+#include <cstdio>
+#include <cstring>
+
+#include "../../include/logprobs_b200.h"
+#include "../../include/moe_b200.h"
+#include "common.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace moe {
+namespace {
+
+constexpr int LP_THREADS = 256;
+constexpr int LP_WARPS = LP_THREADS / 32;
+constexpr int LP_UNROLL = 4;                  // 16-byte loads in flight per thread
+constexpr int LP_CAND = 768;                  // candidates kept; more of them take the slow way
+constexpr int LP_MAX_CLUSTER = 8;
+constexpr float LP_LOG2E = 1.4426950408889634f;
+constexpr float LP_LN2 = 0.6931471805599453f;
+constexpr float LP_BIG = 1024.f;              // |m| above this: x - m is taken first, see LpSums
+constexpr float LP_FLOOR = -1000.f;           // 2^-1000 is 0 in f32; keeps y finite, so that 0 * y is 0
+
+template <typename T> struct LpVec;
+template <> struct LpVec<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void widen(const uint4& a, float* o) {
+    o[0] = __uint_as_float(a.x); o[1] = __uint_as_float(a.y); o[2] = __uint_as_float(a.z); o[3] = __uint_as_float(a.w);
+  }
+  static __device__ __forceinline__ uint4 narrow(const float* o) {
+    return make_uint4(__float_as_uint(o[0]), __float_as_uint(o[1]), __float_as_uint(o[2]), __float_as_uint(o[3]));
+  }
+};
+template <> struct LpVec<bf16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void widen(const uint4& a, float* o) {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {   // a bf16 is the upper half of its f32
+      o[2 * i] = __uint_as_float(w[i] << 16);
+      o[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ uint4 narrow(const float* o) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 v = __floats2bfloat162_rn(o[2 * i], o[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+// maximum that lets a NaN through (fmaxf drops it)
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// Sums of a set of logits relative to its maximum m (never below -FLT_MAX, so that m itself stays finite in an empty set).
+// The reference of the exponent is m2 = round(m log2 e), not m log2 e itself: the rounding shifts every y alike, and log s and
+// t / s take the same shift back out, as long as it is small.  It is 2^-24 of m2, so above |m| = 1024 (where the f32 logits
+// themselves are 2^-14 apart) the difference x - m is taken first, which is exact near the maximum and cannot overflow in the product.
+struct LpSums {
+  float m, s, t;
+};
+__device__ __forceinline__ float lp_shift(float from, float to) {   // y of `from` relative to `to`
+  const float d = fabsf(to) > LP_BIG ? (from - to) * LP_LOG2E : __fmul_rn(from, LP_LOG2E) - __fmul_rn(to, LP_LOG2E);
+  return max_nan(d, LP_FLOOR);
+}
+__device__ __forceinline__ float lp_y(float x, float m) {           // the y of one logit
+  return fabsf(m) > LP_BIG ? (x - m) * LP_LOG2E : fmaf(x, LP_LOG2E, -__fmul_rn(m, LP_LOG2E));
+}
+__device__ __forceinline__ void lp_rebase(LpSums& a, float m) {
+  const float d = lp_shift(a.m, m), c = ex2(d);
+  a.t = c * fmaf(d, a.s, a.t);
+  a.s = c * a.s;
+  a.m = m;
+}
+
+// ordered bits of a logit: larger value, larger number; -0 and +0 alike, NaN below everything else but above 0 ("none")
+__device__ __forceinline__ uint32_t lp_order(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  if (x != x) return 1u;
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float lp_unorder(uint32_t o) {
+  return o == 1u ? __uint_as_float(0x7fc00000u) : __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+// candidates compare by value, then by lower index
+typedef unsigned long long lp_key;
+__device__ __forceinline__ lp_key lp_make(float x, uint32_t index) { return ((lp_key)lp_order(x) << 32) | (0xffffffffu - index); }
+
+// One warp: the n best of `count` distinct keys in shared memory, best first, written to out[0 .. n) (0 where there are
+// fewer).  Every lane keeps the best of its own keys below the last one taken.
+__device__ void lp_select(const lp_key* keys, int count, int n, lp_key* out) {
+  const int lane = threadIdx.x & 31;
+  lp_key mine = 0;
+  for (int i = lane; i < count; i += 32) mine = keys[i] > mine ? keys[i] : mine;
+  for (int k = 0; k < n; ++k) {
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(mine >> 32));
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(mine >> 32) == hi ? (uint32_t)mine : 0u);
+    const lp_key best = ((lp_key)hi << 32) | lo;
+    if (lane == 0) out[k] = best;
+    if (best == 0) {
+      for (int j = k + 1 + lane; j < n; j += 32) out[j] = 0;
+      break;
+    }
+    if (mine == best) {
+      mine = 0;
+      for (int i = lane; i < count; i += 32)
+        if (keys[i] < best && keys[i] > mine) mine = keys[i];
+    }
+  }
+  __syncwarp();
+}
+
+struct LpShared {
+  LpSums warp[LP_WARPS];
+  LpSums cta;                        // this CTA's sums, read by the cluster
+  lp_key bucket[LP_THREADS];         // per thread: best value, first vector that holds it
+  lp_key cand[LP_CAND];
+  lp_key best[LOGPROBS_MAX_TOP];     // this CTA's list, read by the cluster
+  lp_key joined[LP_MAX_CLUSTER * LOGPROBS_MAX_TOP];
+  lp_key last;
+  int count;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(LP_THREADS, 4)
+logprobs_kernel(const T* __restrict__ x, long long stride, const int* __restrict__ targets, int vocab, int top_n, int cluster,
+                float* __restrict__ logprob, float* __restrict__ entropy, float* __restrict__ lse_out, float* __restrict__ top_lp,
+                int* __restrict__ top_ids) {
+  constexpr int N = LpVec<T>::N;
+  __shared__ LpShared sh;
+  const int row = blockIdx.x / cluster, rank = blockIdx.x - row * cluster;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const T* xr = x + (long long)row * stride;
+  // [0, head) and [tail, vocab) lie outside the 16-byte vectors of the row
+  const int mis = (int)((reinterpret_cast<uintptr_t>(xr) & 15) / sizeof(T));
+  const int head = min(vocab, mis ? N - mis : 0);
+  const int vecs = (vocab - head) / N, tail = head + vecs * N, loose = head + (vocab - tail);
+  const uint4* xv = reinterpret_cast<const uint4*>(xr + head);
+  const int step = cluster * LP_THREADS, v0 = rank * LP_THREADS + tid;
+  if (tid == 0) sh.count = 0;
+
+  float best = -INFINITY;            // largest logit seen in a vector, and the first vector that holds it
+  int best_vec = v0;
+  LpSums a{-FLT_MAX, 0.f, 0.f};
+  auto take = [&](const uint4& raw, int v) {
+    float f[N];
+    LpVec<T>::widen(raw, f);
+    float mx = f[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) mx = fmaxf(mx, f[i]);
+    if (mx > best) {
+      best = mx; best_vec = v;
+      if (mx > a.m) lp_rebase(a, mx);
+    }
+    if (fabsf(a.m) > LP_BIG) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = (f[i] - a.m) * LP_LOG2E;
+    } else {
+      const float m2 = __fmul_rn(a.m, LP_LOG2E);
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = fmaf(f[i], LP_LOG2E, -m2);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float y = max_nan(f[i], LP_FLOOR), e = ex2(y);
+      a.s += e;
+      a.t = fmaf(y, e, a.t);
+    }
+  };
+  int v = v0;
+  for (; v + (LP_UNROLL - 1) * step < vecs; v += LP_UNROLL * step) {
+    uint4 raw[LP_UNROLL];
+#pragma unroll
+    for (int u = 0; u < LP_UNROLL; ++u) raw[u] = __ldg(xv + v + u * step);
+#pragma unroll
+    for (int u = 0; u < LP_UNROLL; ++u) take(raw[u], v + u * step);
+  }
+  for (; v < vecs; v += step) take(__ldg(xv + v), v);
+  const bool has_vec = v0 < vecs;
+  if (rank == 0 && tid < loose) {    // the loose ends, one per thread
+    const float f = to_f32<T>(xr[tid < head ? tid : tail + tid - head]);
+    if (f > a.m) lp_rebase(a, f);
+    const float y = max_nan(lp_y(f, a.m), LP_FLOOR), e = ex2(y);
+    a.s += e;
+    a.t = fmaf(y, e, a.t);
+  }
+
+  // ---- join the threads ----
+  float m = a.m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  lp_rebase(a, m);
+  a.s = warp_sum(a.s);
+  a.t = warp_sum(a.t);
+  if (lane == 0) sh.warp[warp] = a;
+  if (top_n > 0) sh.bucket[tid] = has_vec ? ((lp_key)lp_order(best) << 32) | (0xffffffffu - (uint32_t)best_vec) : 0;
+  __syncthreads();
+  if (tid == 0) {
+    float mm = sh.warp[0].m;
+    for (int w = 1; w < LP_WARPS; ++w) mm = fmaxf(mm, sh.warp[w].m);
+    LpSums c{mm, 0.f, 0.f};
+    for (int w = 0; w < LP_WARPS; ++w) {
+      LpSums b = sh.warp[w];
+      lp_rebase(b, mm);
+      c.s += b.s;
+      c.t += b.t;
+    }
+    sh.cta = c;
+  }
+
+  // ---- this CTA's best top_n ----
+  if (top_n > 0) {
+    if (warp == 1) lp_select(sh.bucket, LP_THREADS, top_n, sh.best);
+    __syncthreads();
+    const lp_key bound = sh.best[top_n - 1];        // 0: fewer vectors than that, everything is a candidate
+    const uint32_t bound_value = (uint32_t)(bound >> 32), bound_vec = 0xffffffffu - (uint32_t)bound;
+    auto offer = [&](float f, uint32_t index) {
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < LP_CAND) sh.cand[at] = lp_make(f, index);
+    };
+    if (rank == 0 && tid < loose) {
+      const int i = tid < head ? tid : tail + tid - head;
+      offer(to_f32<T>(xr[i]), i);
+    }
+    const lp_key mine = sh.bucket[tid];
+    unsigned hot = __ballot_sync(0xffffffffu, mine != 0 && mine >= bound);
+    while (hot) {                                   // the warp reads one hot thread's vectors again
+      const int l = __ffs(hot) - 1;
+      hot &= hot - 1;
+      for (long long w = rank * LP_THREADS + warp * 32 + l + (long long)lane * step; w < vecs; w += 32ll * step) {
+        float f[N];
+        LpVec<T>::widen(__ldg(xv + w), f);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const uint32_t o = lp_order(f[i]);
+          if (o > bound_value || (o == bound_value && (uint32_t)w <= bound_vec)) offer(f[i], head + (uint32_t)w * N + i);
+        }
+      }
+    }
+    __syncthreads();
+    if (sh.count <= LP_CAND) {
+      if (warp == 0) lp_select(sh.cand, sh.count, top_n, sh.best);
+    } else {
+      // Thousands of logits above the bound: the best ones sit in a few threads' vectors.  Take the row top_n times, each time the best
+      // below the last one.
+      if (tid == 0) sh.last = ~0ull;
+      __syncthreads();
+      for (int k = 0; k < top_n; ++k) {
+        const lp_key last = sh.last;
+        lp_key mx = 0;
+        auto look = [&](float f, uint32_t index) {
+          const lp_key key = lp_make(f, index);
+          if (key < last && key > mx) mx = key;
+        };
+        for (int w = v0; w < vecs; w += step) {
+          float f[N];
+          LpVec<T>::widen(__ldg(xv + w), f);
+#pragma unroll
+          for (int i = 0; i < N; ++i) look(f[i], head + (uint32_t)w * N + i);
+        }
+        if (rank == 0 && tid < loose) {
+          const int i = tid < head ? tid : tail + tid - head;
+          look(to_f32<T>(xr[i]), i);
+        }
+        sh.bucket[tid] = mx;
+        __syncthreads();
+        if (warp == 0) {
+          lp_select(sh.bucket, LP_THREADS, 1, sh.best + k);
+          if (lane == 0) sh.last = sh.best[k];
+        }
+        __syncthreads();
+      }
+    }
+  }
+
+  // ---- join the cluster, write the row ----
+  LpSums total{};
+  const lp_key* list = sh.best;
+  if (cluster > 1) {
+    cg::cluster_group cl = cg::this_cluster();
+    cl.sync();
+    if (rank == 0) {
+      if (tid == 0) {
+        float mm = -FLT_MAX;
+        for (int r = 0; r < cluster; ++r) mm = fmaxf(mm, cl.map_shared_rank(&sh.cta, r)->m);
+        total.m = mm;
+        for (int r = 0; r < cluster; ++r) {
+          LpSums b = *cl.map_shared_rank(&sh.cta, r);
+          lp_rebase(b, mm);
+          total.s += b.s;
+          total.t += b.t;
+        }
+      }
+      for (int i = tid; i < cluster * top_n; i += LP_THREADS) {
+        const int r = i / top_n;
+        sh.joined[i] = cl.map_shared_rank(sh.best, r)[i - r * top_n];
+      }
+    }
+    cl.sync();                                      // the others' shared memory has been read; they may leave
+    if (rank != 0) return;
+    if (tid == 0) sh.cta = total;
+    if (top_n > 0) {
+      if (warp == 0) lp_select(sh.joined, cluster * top_n, top_n, sh.bucket);
+      list = sh.bucket;
+    }
+  }
+  __syncthreads();
+  total = sh.cta;
+  // y - log2 s keeps the small numbers small: the log probability of a near-certain token is accurate relative to itself
+  const float l2 = log2f(total.s);
+  const bool empty = total.s == 0.f;                // nothing but -inf
+  auto log_p = [&](float f) {
+    if (empty) return f != f ? f : -INFINITY;
+    if (fabsf(f) > LP_BIG || fabsf(total.m) > LP_BIG) return (f - total.m) - l2 * LP_LN2;   // the lowest finite value stays finite
+    return (lp_y(f, total.m) - l2) * LP_LN2;
+  };
+  if (tid == 0) {
+    const float lse = empty ? -INFINITY : fabsf(total.m) > LP_BIG ? fmaf(l2, LP_LN2, total.m) : (__fmul_rn(total.m, LP_LOG2E) + l2) * LP_LN2;
+    if (lse_out) lse_out[row] = lse;
+    if (entropy) entropy[row] = empty ? 0.f : max_nan((l2 - total.t / total.s) * LP_LN2, 0.f);
+    if (logprob) {
+      const int t = targets ? targets[row] : -1;
+      logprob[row] = t < 0 ? 0.f : t >= vocab ? __uint_as_float(0x7fc00000u) : log_p(to_f32<T>(xr[t]));
+    }
+  }
+  if (tid < top_n) {
+    const lp_key key = list[tid];
+    top_ids[(long long)row * top_n + tid] = key ? (int)(0xffffffffu - (uint32_t)key) : -1;
+    top_lp[(long long)row * top_n + tid] = key ? log_p(lp_unorder((uint32_t)(key >> 32))) : __uint_as_float(0x7fc00000u);
+  }
+}
+
+// Gradient: one read and one write of the logits' size, everything else is per row.  A CTA takes a run of one row; the 16-byte path needs
+// the logits' and the gradient's row equally far from a 16-byte boundary, the element path takes what is left.
+template <typename T>
+__global__ void __launch_bounds__(LP_THREADS)
+logprobs_backward_kernel(const T* x, long long stride, const int* __restrict__ targets, const float* __restrict__ lse,
+                         const float* __restrict__ entropy, const float* __restrict__ grad_lp, const float* __restrict__ grad_h, int vocab,
+                         int runs, T* grad, long long grad_stride) {
+  constexpr int N = LpVec<T>::N, RUN = LP_THREADS * LP_UNROLL;    // vectors per CTA
+  const int row = blockIdx.x / runs, run = blockIdx.x - row * runs;
+  const T* xr = x + (long long)row * stride;
+  T* gr = grad + (long long)row * grad_stride;
+  const int target = targets ? targets[row] : -1;
+  const float z = lse[row], h = grad_h ? entropy[row] : 0.f, gh = grad_h ? grad_h[row] : 0.f;
+  float gl = grad_lp && target >= 0 ? grad_lp[row] : 0.f;
+  if (target >= vocab) gl = __uint_as_float(0x7fc00000u);
+  const bool empty = z == -INFINITY;
+  auto one = [&](float f, int index) {
+    const float d = f - z, p = ex2(d * LP_LOG2E);
+    // d is -inf at a masked logit, where p is 0
+    const float g = fmaf(-gh * p, max_nan(d, LP_FLOOR) + h, gl * ((index == target ? 1.f : 0.f) - p));
+    return empty ? (f == f ? 0.f * gl : f) : g;
+  };
+  const int mis = (int)((reinterpret_cast<uintptr_t>(xr) & 15) / sizeof(T));
+  const bool wide = ((reinterpret_cast<uintptr_t>(xr) ^ reinterpret_cast<uintptr_t>(gr)) & 15) == 0;
+  if (!wide) {
+    const int end = (int)min((long long)vocab, (long long)(run + 1) * RUN * N);
+    for (int i = run * RUN * N + (int)threadIdx.x; i < end; i += LP_THREADS) gr[i] = from_f32<T>(one(to_f32<T>(xr[i]), i));
+    return;
+  }
+  const int head = min(vocab, mis ? N - mis : 0), vecs = (vocab - head) / N, tail = head + vecs * N;
+  if (run == 0 && (int)threadIdx.x < head + (vocab - tail)) {
+    const int i = (int)threadIdx.x < head ? threadIdx.x : tail + threadIdx.x - head;
+    gr[i] = from_f32<T>(one(to_f32<T>(xr[i]), i));
+  }
+  const uint4* xv = reinterpret_cast<const uint4*>(xr + head);
+  uint4* gv = reinterpret_cast<uint4*>(gr + head);
+  uint4 raw[LP_UNROLL];
+#pragma unroll
+  for (int u = 0; u < LP_UNROLL; ++u) {
+    const int v = run * RUN + u * LP_THREADS + threadIdx.x;
+    if (v < vecs) raw[u] = xv[v];
+  }
+#pragma unroll
+  for (int u = 0; u < LP_UNROLL; ++u) {
+    const int v = run * RUN + u * LP_THREADS + threadIdx.x;
+    if (v >= vecs) continue;
+    float f[N];
+    LpVec<T>::widen(raw[u], f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = one(f[i], head + v * N + i);
+    gv[v] = LpVec<T>::narrow(f);
+  }
+}
+
+int lp_fail(char* msg, int len, int code, const char* text) {
+  if (msg && len > 0) snprintf(msg, len, "%s", text);
+  return code;
+}
+
+template <typename T>
+cudaError_t launch_forward(const void* x, long long stride, const int* targets, int rows, int vocab, int top_n, float* logprob, float* entropy,
+                           float* lse, float* top_lp, int* top_ids, cudaStream_t st) {
+  // A row's CTAs: as many as fill the machine (a CTA is 256 threads, four fit an SM), but with a full round of loads for each.
+  int cluster = 1;
+  const long long vecs = vocab / LpVec<T>::N;
+  while (cluster < LP_MAX_CLUSTER && (long long)rows * cluster * 2 <= 4 * 148 && vecs >= (long long)cluster * 2 * LP_THREADS) cluster *= 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(rows * cluster));
+  cfg.blockDim = dim3(LP_THREADS);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  count_launch();
+  return cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, (const T*)x, stride, targets, vocab, top_n, cluster, logprob, entropy, lse, top_lp, top_ids);
+}
+
+}  // namespace
+}  // namespace moe
+
+using namespace moe;
+
+extern "C" {
+
+int32_t logprobs_forward(const void* x, int64_t row_stride, const int32_t* targets, int32_t rows, int32_t vocab, int32_t top_n,
+                         int32_t precision, float* logprob, float* entropy, float* lse, float* top_logprob, int32_t* top_ids,
+                         void* stream, char* message, int32_t message_len) {
+  if (precision != MOE_PRECISION_F32 && precision != MOE_PRECISION_BF16)
+    return lp_fail(message, message_len, MOE_INVALID_CONFIG, "InvalidConfig: logits are f32 or bf16");
+  if (rows < 0 || vocab <= 0 || row_stride < vocab)
+    return lp_fail(message, message_len, MOE_INVALID_INPUT, "InvalidInput: rows >= 0, vocab > 0 and row_stride >= vocab");
+  if (top_n < 0 || top_n > LOGPROBS_MAX_TOP || top_n > vocab)
+    return lp_fail(message, message_len, MOE_INVALID_INPUT, "InvalidInput: top_n is 0 .. min(vocab, 32)");
+  if (rows == 0) return MOE_OK;
+  if (!x || (top_n > 0 && (!top_logprob || !top_ids))) return lp_fail(message, message_len, MOE_INVALID_INPUT, "InvalidInput: null buffer");
+  const size_t elem = precision == MOE_PRECISION_BF16 ? 2 : 4;
+  if (reinterpret_cast<uintptr_t>(x) % elem) return lp_fail(message, message_len, MOE_INVALID_INPUT, "InvalidInput: logits are not aligned to their type");
+  const cudaError_t e = precision == MOE_PRECISION_BF16
+      ? launch_forward<bf16>(x, row_stride, targets, rows, vocab, top_n, logprob, entropy, lse, top_logprob, top_ids, (cudaStream_t)stream)
+      : launch_forward<float>(x, row_stride, targets, rows, vocab, top_n, logprob, entropy, lse, top_logprob, top_ids, (cudaStream_t)stream);
+  return e == cudaSuccess ? MOE_OK : lp_fail(message, message_len, MOE_CUDA_ERROR, cudaGetErrorString(e));
+}
+
+int32_t logprobs_backward(const void* x, int64_t row_stride, const int32_t* targets, const float* lse, const float* entropy,
+                          const float* grad_logprob, const float* grad_entropy, int32_t rows, int32_t vocab, int32_t precision,
+                          void* grad_x, int64_t grad_stride, void* stream, char* message, int32_t message_len) {
+  if (precision != MOE_PRECISION_F32 && precision != MOE_PRECISION_BF16)
+    return lp_fail(message, message_len, MOE_INVALID_CONFIG, "InvalidConfig: logits are f32 or bf16");
+  if (rows < 0 || vocab <= 0 || row_stride < vocab || grad_stride < vocab)
+    return lp_fail(message, message_len, MOE_INVALID_INPUT, "InvalidInput: rows >= 0, vocab > 0 and strides >= vocab");
+  if (rows == 0) return MOE_OK;
+  if (!x || !grad_x || !lse || (grad_entropy && !entropy)) return lp_fail(message, message_len, MOE_INVALID_INPUT, "InvalidInput: null buffer");
+  if (x == grad_x && row_stride != grad_stride)
+    return lp_fail(message, message_len, MOE_INVALID_INPUT, "InvalidInput: a gradient in place has the logits' row stride");
+  const size_t elem = precision == MOE_PRECISION_BF16 ? 2 : 4;
+  if (reinterpret_cast<uintptr_t>(x) % elem || reinterpret_cast<uintptr_t>(grad_x) % elem)
+    return lp_fail(message, message_len, MOE_INVALID_INPUT, "InvalidInput: buffers are not aligned to their type");
+  const long long per_run = (long long)LP_THREADS * LP_UNROLL * (16 / elem);
+  const long long runs = (vocab + per_run - 1) / per_run;
+  if (runs * rows > 0x7fffffffll) return lp_fail(message, message_len, MOE_INVALID_INPUT, "InvalidInput: too many rows");
+  const unsigned grid = (unsigned)(runs * rows);
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (precision == MOE_PRECISION_BF16)
+    logprobs_backward_kernel<bf16><<<grid, LP_THREADS, 0, st>>>((const bf16*)x, row_stride, targets, lse, entropy, grad_logprob, grad_entropy,
+                                                                vocab, (int)runs, (bf16*)grad_x, grad_stride);
+  else
+    logprobs_backward_kernel<float><<<grid, LP_THREADS, 0, st>>>((const float*)x, row_stride, targets, lse, entropy, grad_logprob, grad_entropy,
+                                                                 vocab, (int)runs, (float*)grad_x, grad_stride);
+  count_launch();
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? MOE_OK : lp_fail(message, message_len, MOE_CUDA_ERROR, cudaGetErrorString(e));
+}
+
+}  // extern "C"

@@ -1,0 +1,84 @@
+"""Token log probabilities of device logits, with entropy and the most likely tokens, and their gradient: the C ABI of
+include/logprobs_b200.h.  Device tensors in, device tensors out; no host implementation behind it.
+
+``TransformerLm.score_batch`` gives the same numbers for the tokens of a batch without the logits leaving the device.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+from . import _lib
+from ._torch import issue
+from .moe import CudaError, InvalidConfig, InvalidInput
+
+MAX_TOP = 32
+
+_ERRORS = {_lib.INVALID_CONFIG: InvalidConfig, _lib.INVALID_INPUT: InvalidInput, _lib.UNSUPPORTED: InvalidConfig}
+
+
+class TokenLogProbs(NamedTuple):
+    """What ``token_logprobs`` returns; every field is f32 [rows] but the alternatives, [rows, top] (None without them)."""
+    logprob: "torch.Tensor"                    # log p of the given token; 0 where there is none
+    entropy: "torch.Tensor"
+    lse: "torch.Tensor"                        # log of the sum of the exponentials, which the gradient takes
+    top_ids: Optional["torch.Tensor"]          # int32, the most likely first, the lower id first among equal logits
+    top_logprobs: Optional["torch.Tensor"]
+
+
+def _check_logits(t, name):
+    import torch
+    if t.dim() != 2 or not t.is_cuda or t.dtype not in (torch.float32, torch.bfloat16):
+        raise InvalidInput("%s must be an f32 or bf16 device tensor [rows, vocab]" % name)
+    rows, vocab = t.shape
+    if vocab == 0 or (vocab > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < vocab):
+        raise InvalidInput("the logits of a row of %s are adjacent, and rows do not overlap" % name)
+    return rows, vocab, max(t.stride(0), vocab), _lib.PRECISION_BF16 if t.dtype == torch.bfloat16 else _lib.PRECISION_F32
+
+
+def _check_row(t, rows, dtype, like, name):
+    if t is None:
+        return None
+    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != rows or t.device != like.device or not t.is_contiguous():
+        raise InvalidInput("%s must be a contiguous %s tensor of %d values on the logits' device" % (name, dtype, rows))
+    return t.data_ptr()
+
+
+def token_logprobs(logits, targets=None, top: int = 0, stream=None) -> TokenLogProbs:
+    """``logits`` [rows, vocab], f32 or bf16, rows any distance apart; ``targets`` int32 [rows], negative for "no token" (None: no row
+    has one); ``top`` alternatives per row, at most 32 and at most vocab."""
+    import torch
+    rows, vocab, stride, precision = _check_logits(logits, "logits")
+    t = _check_row(targets, rows, torch.int32, logits, "targets")
+    if not 0 <= top <= min(vocab, MAX_TOP):
+        raise InvalidInput("top is 0 .. %d, got %d" % (min(vocab, MAX_TOP), top))
+    lp, h, lse = torch.empty((3, rows), dtype=torch.float32, device=logits.device).unbind(0)
+    ids = tlp = None
+    if top:
+        ids = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
+        tlp = torch.empty((rows, top), dtype=torch.float32, device=logits.device)
+    issue(_lib.lib().logprobs_forward, logits, stream, _ERRORS, CudaError, logits.data_ptr(), stride, t, rows, vocab, top, precision,
+          lp.data_ptr(), h.data_ptr(), lse.data_ptr(), tlp.data_ptr() if top else None, ids.data_ptr() if top else None)
+    return TokenLogProbs(lp, h, lse, ids, tlp)
+
+
+def token_logprobs_backward(logits, targets, lse, entropy=None, grad_logprob=None, grad_entropy=None, out=None, stream=None):
+    """dL/dlogits from dL/dlogprob and dL/dentropy [rows] (either may be None).  ``lse`` and ``entropy`` are the forward call's; ``out``
+    (default: a new tensor) has the logits' shape and type and may be ``logits`` itself."""
+    import torch
+    rows, vocab, stride, precision = _check_logits(logits, "logits")
+    if out is None:
+        out = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
+    elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
+        raise InvalidInput("out must match the logits")
+    _, _, out_stride, _ = _check_logits(out, "out")
+    if lse is None or (grad_entropy is not None and entropy is None):
+        raise InvalidInput("the gradient needs lse, and the entropy for a gradient of it")
+    f32 = torch.float32
+    issue(_lib.lib().logprobs_backward, logits, stream, _ERRORS, CudaError, logits.data_ptr(), stride,
+          _check_row(targets, rows, torch.int32, logits, "targets"), _check_row(lse, rows, f32, logits, "lse"),
+          _check_row(entropy, rows, f32, logits, "entropy"), _check_row(grad_logprob, rows, f32, logits, "grad_logprob"),
+          _check_row(grad_entropy, rows, f32, logits, "grad_entropy"), rows, vocab, precision, out.data_ptr(), out_stride)
+    return out
+
+
+__all__ = ["TokenLogProbs", "token_logprobs", "token_logprobs_backward", "MAX_TOP"]
