@@ -3,10 +3,10 @@
 //
 // Forward is one pass over the logits, bound by HBM: every thread keeps a running maximum m, s = sum 2^y and
 // t = sum y 2^y with y = (x - m) log2(e), rescaled when the maximum moves.  The entropy is then log s - t / s: both
-// terms are >= 0, so nothing cancels.  The alternatives cost no second pass: a thread remembers which of its 16-byte
-// vectors first reached its maximum, the top_n-th best of those (value, vector) pairs is a lower bound for the top_n-th best
-// logit, and only the threads above the bound (top_n of them) have their share of the row read again, by a whole
-// warp and out of L2.  What passes the bound is a few dozen values, sorted by one warp.
+// terms are >= 0, so nothing cancels.  The alternatives cost no second pass: a thread keeps the maximum of each of four
+// sets of its vectors and the vector that first reached it, the top_n-th best of 32 such (value, vector) pairs is a lower bound for the top_n-th best
+// logit, and only the buckets that reach the bound (a twentieth of the row for 20 alternatives) are read again, by the whole CTA and out of L2.  What
+// passes the bound is a few dozen values, each put in its place by counting the larger ones.
 //
 // One CTA takes a row.  When there are fewer rows than would fill the machine, a cluster of 2, 4 or 8 CTAs takes one and
 // joins its sums and candidate lists through distributed shared memory: still one launch and no workspace.
@@ -25,14 +25,17 @@ namespace cg = cooperative_groups;
 namespace moe {
 namespace {
 
-constexpr int LP_THREADS = 256;
+constexpr int LP_THREADS = 128;              // 8192 x 32000 bf16 take 94 us; with 256 or 512 threads a CTA 105 and 131 (measured)
+constexpr int LP_CTAS = 7;                   // CTAs an SM: 72 registers; 8 of them (64 registers, some spilled) take 96 us
 constexpr int LP_WARPS = LP_THREADS / 32;
 constexpr int LP_UNROLL = 4;                  // 16-byte loads in flight per thread
+constexpr int LP_BUCKETS = LP_THREADS * LP_UNROLL;
 constexpr int LP_CAND = 768;                  // candidates kept; more of them take the slow way
 constexpr int LP_MAX_CLUSTER = 8;
 constexpr float LP_LOG2E = 1.4426950408889634f;
 constexpr float LP_LN2 = 0.6931471805599453f;
 constexpr float LP_BIG = 1024.f;              // |m| above this: x - m is taken first, see LpSums
+constexpr float LP_LOW = -1e30f;              // a logit below this has probability 0 when |m| <= LP_BIG
 constexpr float LP_FLOOR = -1000.f;           // 2^-1000 is 0 in f32; keeps y finite, so that 0 * y is 0
 
 template <typename T> struct LpVec;
@@ -76,6 +79,54 @@ __device__ __forceinline__ float ex2(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
+}
+
+// two f32 lanes in one instruction
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Largest value of a 16-byte vector (a NaN is passed over), and a vector with what lies below LP_LOW raised to it: its
+// exponential is 0 either way, and a finite y keeps 0 * y at 0.  Both work on the packed values.
+__device__ __forceinline__ uint4 vec_none(float) { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }   // -inf
+__device__ __forceinline__ uint4 vec_none(bf16) { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+__device__ __forceinline__ float vec_max(const uint4& a, float) {
+  return fmaxf(fmaxf(__uint_as_float(a.x), __uint_as_float(a.y)), fmaxf(__uint_as_float(a.z), __uint_as_float(a.w)));
+}
+__device__ __forceinline__ float vec_max(const uint4& a, bf16) {
+  const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&a);
+  const __nv_bfloat162 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+  return fmaxf(__low2float(m), __high2float(m));
+}
+__device__ __forceinline__ uint4 vec_raise(const uint4& a, float) {
+  return make_uint4(__float_as_uint(max_nan(__uint_as_float(a.x), LP_LOW)), __float_as_uint(max_nan(__uint_as_float(a.y), LP_LOW)),
+                    __float_as_uint(max_nan(__uint_as_float(a.z), LP_LOW)), __float_as_uint(max_nan(__uint_as_float(a.w), LP_LOW)));
+}
+__device__ __forceinline__ uint4 vec_raise(uint4 a, bf16) {
+  const __nv_bfloat162 low = __float2bfloat162_rn(LP_LOW);
+  __nv_bfloat162* p = reinterpret_cast<__nv_bfloat162*>(&a);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) p[i] = __hmax2_nan(p[i], low);
+  return a;
 }
 
 // Sums of a set of logits relative to its maximum m (never below -FLT_MAX, so that m itself stays finite in an empty set).
@@ -136,19 +187,75 @@ __device__ void lp_select(const lp_key* keys, int count, int n, lp_key* out) {
   __syncwarp();
 }
 
+// The whole CTA: the n best of `count` distinct keys (or 0), each key's place being the number of larger ones.  `keys` has room for
+// one more.
+__device__ void lp_rank(lp_key* keys, int count, int n, lp_key* out) {
+  if (threadIdx.x == 0) keys[count] = 0;
+  if (threadIdx.x < n) out[threadIdx.x] = 0;
+  __syncthreads();
+  const ulonglong2* two = reinterpret_cast<const ulonglong2*>(keys);
+  for (int at = threadIdx.x; at < count; at += LP_THREADS) {
+    const lp_key mine = keys[at];
+    int place = 0;
+    for (int i = 0; i < (count + 1) / 2; ++i) {
+      const ulonglong2 k = two[i];
+      place += (k.x > mine) + (k.y > mine);
+    }
+    if (place < n && mine != 0) out[place] = mine;
+  }
+  __syncthreads();
+}
+
+// One warp: a bound that at least n buckets reach, and the list of those that do.  Lane l takes the best of the buckets l, l + 32, ...;
+// the n-th best of these 32 is the bound (of 512 buckets, about 30 reach it for n = 20 and 5 for n = 5).  0: fewer than n lanes have a
+// vector at all, and every value is a candidate.
+__device__ lp_key lp_bound(const lp_key* bucket, int n, lp_key* best_of_lane, int* hot, int* hot_count) {
+  const int lane = threadIdx.x & 31;
+  lp_key mine = 0;
+#pragma unroll
+  for (int i = 0; i < LP_BUCKETS / 32; ++i) {
+    const lp_key k = bucket[i * 32 + lane];
+    mine = k > mine ? k : mine;
+  }
+  best_of_lane[lane] = mine;
+  __syncwarp();
+  const ulonglong2* two = reinterpret_cast<const ulonglong2*>(best_of_lane);
+  int place = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const ulonglong2 k = two[i];
+    place += (k.x > mine) + (k.y > mine);
+  }
+  const unsigned at = __ballot_sync(0xffffffffu, mine != 0 && place == n - 1);
+  const lp_key bound = at ? __shfl_sync(0xffffffffu, mine, __ffs(at) - 1) : 0;
+  int count = 0;
+#pragma unroll
+  for (int i = 0; i < LP_BUCKETS / 32; ++i) {
+    const lp_key k = bucket[i * 32 + lane];
+    const bool is_hot = k != 0 && k >= bound;
+    const unsigned all = __ballot_sync(0xffffffffu, is_hot);
+    if (is_hot) hot[count + __popc(all & ((1u << lane) - 1))] = i * 32 + lane;
+    count += __popc(all);
+  }
+  if (lane == 0) *hot_count = count;
+  return bound;
+}
+
 struct LpShared {
   LpSums warp[LP_WARPS];
   LpSums cta;                        // this CTA's sums, read by the cluster
-  lp_key bucket[LP_THREADS];         // per thread: best value, first vector that holds it
-  lp_key cand[LP_CAND];
+  lp_key bucket[LP_BUCKETS];         // best value, first vector that holds it
+  alignas(16) lp_key cand[LP_CAND];
   lp_key best[LOGPROBS_MAX_TOP];     // this CTA's list, read by the cluster
-  lp_key joined[LP_MAX_CLUSTER * LOGPROBS_MAX_TOP];
-  lp_key last;
-  int count;
+  alignas(16) lp_key joined[LP_MAX_CLUSTER * LOGPROBS_MAX_TOP + 2];
+  alignas(16) lp_key lane_best[32];
+  int hot[LP_BUCKETS];               // buckets whose vectors are read again
+  lp_key bound, last;
+  int count, hot_count;
 };
 
 template <typename T>
-__global__ void __launch_bounds__(LP_THREADS, 4)
+__global__ void __launch_bounds__(LP_THREADS, LP_CTAS)
 logprobs_kernel(const T* __restrict__ x, long long stride, const int* __restrict__ targets, int vocab, int top_n, int cluster,
                 float* __restrict__ logprob, float* __restrict__ entropy, float* __restrict__ lse_out, float* __restrict__ top_lp,
                 int* __restrict__ top_ids) {
@@ -165,44 +272,87 @@ logprobs_kernel(const T* __restrict__ x, long long stride, const int* __restrict
   const int step = cluster * LP_THREADS, v0 = rank * LP_THREADS + tid;
   if (tid == 0) sh.count = 0;
 
-  float best = -INFINITY;            // largest logit seen in a vector, and the first vector that holds it
-  int best_vec = v0;
-  LpSums a{-FLT_MAX, 0.f, 0.f};
-  auto take = [&](const uint4& raw, int v) {
-    float f[N];
-    LpVec<T>::widen(raw, f);
-    float mx = f[0];
+  // A thread's vectors fall into LP_UNROLL buckets by their place in a round: the largest logit of each, and the first vector with it.
+  float best[LP_UNROLL];
+  int best_vec[LP_UNROLL];
 #pragma unroll
-    for (int i = 1; i < N; ++i) mx = fmaxf(mx, f[i]);
-    if (mx > best) {
-      best = mx; best_vec = v;
-      if (mx > a.m) lp_rebase(a, mx);
-    }
-    if (fabsf(a.m) > LP_BIG) {
+  for (int u = 0; u < LP_UNROLL; ++u) { best[u] = -INFINITY; best_vec[u] = v0 + u * step; }
+  float m = -FLT_MAX, m2 = 0.f;      // the maximum that the sums refer to, and round(m log2 e) of one within LP_BIG
+  uint64_t s2 = 0, t2 = 0;           // s and t, each as two halves
+  auto sums = [&] {
+    float s0, s1, t0, t1;
+    unpack2(s2, s0, s1);
+    unpack2(t2, t0, t1);
+    return LpSums{m, s0 + s1, t0 + t1};
+  };
+  auto load = [&](uint4* raw, int v) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = (f[i] - a.m) * LP_LOG2E;
-    } else {
-      const float m2 = __fmul_rn(a.m, LP_LOG2E);
-#pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = fmaf(f[i], LP_LOG2E, -m2);
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float y = max_nan(f[i], LP_FLOOR), e = ex2(y);
-      a.s += e;
-      a.t = fmaf(y, e, a.t);
+    for (int u = 0; u < LP_UNROLL; ++u) {
+      raw[u] = vec_none(T());
+      if (v + u * step < vecs) raw[u] = __ldg(xv + v + u * step);
     }
   };
-  int v = v0;
-  for (; v + (LP_UNROLL - 1) * step < vecs; v += LP_UNROLL * step) {
-    uint4 raw[LP_UNROLL];
+  auto take = [&](const uint4* raw, int v) {
+    float top = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < LP_UNROLL; ++u) raw[u] = __ldg(xv + v + u * step);
+    for (int u = 0; u < LP_UNROLL; ++u) {
+      const float mx = vec_max(raw[u], T());
+      if (mx > best[u]) { best[u] = mx; best_vec[u] = v + u * step; }
+      top = fmaxf(top, mx);
+    }
+    if (top > m) {
+      LpSums a = sums();
+      lp_rebase(a, top);
+      m = top;
+      m2 = __fmul_rn(m, LP_LOG2E);
+      s2 = pack2(a.s, 0.f);
+      t2 = pack2(a.t, 0.f);
+    }
+    if (fabsf(m) <= LP_BIG) {
+      // two logits an instruction but for the exponential, of which an SM does 16 a cycle
+      const uint64_t mm = pack2(-m2, -m2), ll = pack2(LP_LOG2E, LP_LOG2E);
 #pragma unroll
-    for (int u = 0; u < LP_UNROLL; ++u) take(raw[u], v + u * step);
+      for (int u = 0; u < LP_UNROLL; ++u) {
+        float f[N];
+        LpVec<T>::widen(vec_raise(raw[u], T()), f);
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+          const uint64_t y = fma2(pack2(f[i], f[i + 1]), ll, mm);
+          float y0, y1;
+          unpack2(y, y0, y1);
+          const uint64_t e = pack2(ex2(y0), ex2(y1));
+          s2 = add2(s2, e);
+          t2 = fma2(y, e, t2);
+        }
+      }
+    } else {
+      LpSums a = sums();
+#pragma unroll
+      for (int u = 0; u < LP_UNROLL; ++u) {
+        float f[N];
+        LpVec<T>::widen(raw[u], f);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float y = max_nan((f[i] - m) * LP_LOG2E, LP_FLOOR), e = ex2(y);
+          a.s += e;
+          a.t = fmaf(y, e, a.t);
+        }
+      }
+      s2 = pack2(a.s, 0.f);
+      t2 = pack2(a.t, 0.f);
+    }
+  };
+  // the next round's loads are in flight while a round is summed
+  uint4 even[LP_UNROLL], odd[LP_UNROLL];
+  constexpr int R = LP_UNROLL;
+  load(even, v0);
+  for (int v = v0; v < vecs; v += 2 * R * step) {
+    load(odd, v + R * step);
+    take(even, v);
+    load(even, v + 2 * R * step);
+    if (v + R * step < vecs) take(odd, v + R * step);
   }
-  for (; v < vecs; v += step) take(__ldg(xv + v), v);
-  const bool has_vec = v0 < vecs;
+  LpSums a = sums();
   if (rank == 0 && tid < loose) {    // the loose ends, one per thread
     const float f = to_f32<T>(xr[tid < head ? tid : tail + tid - head]);
     if (f > a.m) lp_rebase(a, f);
@@ -212,14 +362,18 @@ logprobs_kernel(const T* __restrict__ x, long long stride, const int* __restrict
   }
 
   // ---- join the threads ----
-  float m = a.m;
+  m = a.m;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   lp_rebase(a, m);
   a.s = warp_sum(a.s);
   a.t = warp_sum(a.t);
   if (lane == 0) sh.warp[warp] = a;
-  if (top_n > 0) sh.bucket[tid] = has_vec ? ((lp_key)lp_order(best) << 32) | (0xffffffffu - (uint32_t)best_vec) : 0;
+  if (top_n > 0) {
+#pragma unroll
+    for (int u = 0; u < LP_UNROLL; ++u)
+      sh.bucket[u * LP_THREADS + tid] = v0 + u * step < vecs ? ((lp_key)lp_order(best[u]) << 32) | (0xffffffffu - (uint32_t)best_vec[u]) : 0;
+  }
   __syncthreads();
   if (tid == 0) {
     float mm = sh.warp[0].m;
@@ -236,9 +390,12 @@ logprobs_kernel(const T* __restrict__ x, long long stride, const int* __restrict
 
   // ---- this CTA's best top_n ----
   if (top_n > 0) {
-    if (warp == 1) lp_select(sh.bucket, LP_THREADS, top_n, sh.best);
+    if (warp == 1) {
+      const lp_key b = lp_bound(sh.bucket, top_n, sh.lane_best, sh.hot, &sh.hot_count);
+      if (lane == 0) sh.bound = b;
+    }
     __syncthreads();
-    const lp_key bound = sh.best[top_n - 1];        // 0: fewer vectors than that, everything is a candidate
+    const lp_key bound = sh.bound;                  // 0: everything is a candidate
     const uint32_t bound_value = (uint32_t)(bound >> 32), bound_vec = 0xffffffffu - (uint32_t)bound;
     auto offer = [&](float f, uint32_t index) {
       const int at = atomicAdd(&sh.count, 1);
@@ -248,23 +405,24 @@ logprobs_kernel(const T* __restrict__ x, long long stride, const int* __restrict
       const int i = tid < head ? tid : tail + tid - head;
       offer(to_f32<T>(xr[i]), i);
     }
-    const lp_key mine = sh.bucket[tid];
-    unsigned hot = __ballot_sync(0xffffffffu, mine != 0 && mine >= bound);
-    while (hot) {                                   // the warp reads one hot thread's vectors again
-      const int l = __ffs(hot) - 1;
-      hot &= hot - 1;
-      for (long long w = rank * LP_THREADS + warp * 32 + l + (long long)lane * step; w < vecs; w += 32ll * step) {
-        float f[N];
-        LpVec<T>::widen(__ldg(xv + w), f);
+    const int each = (vecs + LP_UNROLL * step - 1) / (LP_UNROLL * step), again = sh.hot_count * each;
+#pragma unroll 2
+    for (int i = tid; i < again; i += LP_THREADS) {
+      const int h = i / each, bucket = sh.hot[h], u = bucket / LP_THREADS;
+      const int w = rank * LP_THREADS + (bucket - u * LP_THREADS) + ((i - h * each) * LP_UNROLL + u) * step;
+      if (w >= vecs) continue;
+      float f[N];
+      LpVec<T>::widen(__ldg(xv + w), f);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const uint32_t o = lp_order(f[i]);
-          if (o > bound_value || (o == bound_value && (uint32_t)w <= bound_vec)) offer(f[i], head + (uint32_t)w * N + i);
-        }
+      for (int k = 0; k < N; ++k) {
+        const uint32_t o = lp_order(f[k]);
+        if (o > bound_value || (o == bound_value && (uint32_t)w <= bound_vec)) offer(f[k], head + (uint32_t)w * N + k);
       }
     }
     __syncthreads();
-    if (sh.count <= LP_CAND) {
+    if (sh.count <= 2 * LP_THREADS) {
+      lp_rank(sh.cand, sh.count, top_n, sh.best);
+    } else if (sh.count <= LP_CAND) {
       if (warp == 0) lp_select(sh.cand, sh.count, top_n, sh.best);
     } else {
       // Thousands of logits above the bound: the best ones sit in a few threads' vectors.  Take the row top_n times, each time the best
@@ -326,7 +484,7 @@ logprobs_kernel(const T* __restrict__ x, long long stride, const int* __restrict
     if (rank != 0) return;
     if (tid == 0) sh.cta = total;
     if (top_n > 0) {
-      if (warp == 0) lp_select(sh.joined, cluster * top_n, top_n, sh.bucket);
+      lp_rank(sh.joined, cluster * top_n, top_n, sh.bucket);
       list = sh.bucket;
     }
   }
@@ -372,10 +530,11 @@ logprobs_backward_kernel(const T* x, long long stride, const int* __restrict__ t
   float gl = grad_lp && target >= 0 ? grad_lp[row] : 0.f;
   if (target >= vocab) gl = __uint_as_float(0x7fc00000u);
   const bool empty = z == -INFINITY;
+  // d is -inf at a masked logit, where p is 0; the target's own gl comes on top
+  const float c = -fmaf(gh, h, gl);
   auto one = [&](float f, int index) {
     const float d = f - z, p = ex2(d * LP_LOG2E);
-    // d is -inf at a masked logit, where p is 0
-    const float g = fmaf(-gh * p, max_nan(d, LP_FLOOR) + h, gl * ((index == target ? 1.f : 0.f) - p));
+    const float g = fmaf(p, fmaf(-gh, max_nan(d, LP_FLOOR), c), index == target ? gl : 0.f);
     return empty ? (f == f ? 0.f * gl : f) : g;
   };
   const int mis = (int)((reinterpret_cast<uintptr_t>(xr) & 15) / sizeof(T));
@@ -402,10 +561,23 @@ logprobs_backward_kernel(const T* x, long long stride, const int* __restrict__ t
   for (int u = 0; u < LP_UNROLL; ++u) {
     const int v = run * RUN + u * LP_THREADS + threadIdx.x;
     if (v >= vecs) continue;
+    const int base = head + v * N;
     float f[N];
     LpVec<T>::widen(raw[u], f);
+    if (empty || (unsigned)(target - base) < (unsigned)N) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = one(f[i], head + v * N + i);
+      for (int i = 0; i < N; ++i) f[i] = one(f[i], base + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        const uint64_t d = add2(pack2(f[i], f[i + 1]), pack2(-z, -z));
+        float d0, d1, y0, y1;
+        unpack2(d, d0, d1);
+        unpack2(mul2(d, pack2(LP_LOG2E, LP_LOG2E)), y0, y1);
+        const uint64_t w = fma2(pack2(max_nan(d0, LP_FLOOR), max_nan(d1, LP_FLOOR)), pack2(-gh, -gh), pack2(c, c));
+        unpack2(mul2(pack2(ex2(y0), ex2(y1)), w), f[i], f[i + 1]);
+      }
+    }
     gv[v] = LpVec<T>::narrow(f);
   }
 }
@@ -418,10 +590,10 @@ int lp_fail(char* msg, int len, int code, const char* text) {
 template <typename T>
 cudaError_t launch_forward(const void* x, long long stride, const int* targets, int rows, int vocab, int top_n, float* logprob, float* entropy,
                            float* lse, float* top_lp, int* top_ids, cudaStream_t st) {
-  // A row's CTAs: as many as fill the machine (a CTA is 256 threads, four fit an SM), but with a full round of loads for each.
+  // A row's CTAs: as many as fill the machine, but with two vectors for each thread.
   int cluster = 1;
   const long long vecs = vocab / LpVec<T>::N;
-  while (cluster < LP_MAX_CLUSTER && (long long)rows * cluster * 2 <= 4 * 148 && vecs >= (long long)cluster * 2 * LP_THREADS) cluster *= 2;
+  while (cluster < LP_MAX_CLUSTER && (long long)rows * cluster * 2 <= LP_CTAS * 148 && vecs >= (long long)cluster * 2 * LP_THREADS) cluster *= 2;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(rows * cluster));
   cfg.blockDim = dim3(LP_THREADS);
