@@ -155,6 +155,11 @@ def lib() -> C.CDLL:
         "rmsnorm_backward": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, f32, i32, vp, C.c_char_p, i32]),
         "logprobs_forward": (i32, [vp, C.c_int64, vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, C.c_char_p, i32]),
         "logprobs_backward": (i32, [vp, C.c_int64, vp, vp, vp, vp, vp, i32, i32, i32, vp, C.c_int64, vp, C.c_char_p, i32]),
+        "q4_linear_packed_bytes": (C.c_int64, [i32, i32, i32]),
+        "q4_linear_pack": (i32, [vp, vp, vp, i32, i32, i32, vp, C.c_char_p, i32]),
+        "q4_linear_quantize": (i32, [vp, vp, i32, i32, i32, vp, C.c_char_p, i32]),
+        "q4_linear_dequantize": (i32, [vp, vp, i32, i32, i32, vp, C.c_char_p, i32]),
+        "q4_linear_forward": (i32, [vp, C.c_int64, vp, vp, C.c_int64, i32, i32, i32, i32, i32, vp, C.c_char_p, i32]),
         "moe_debug_tc_gemm": (i32, [i32, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp, vp]),
         "moe_debug_launch_count": (C.c_int64, []),
         "moe_debug_set_tc_pair": (i32, [i32]),
