@@ -11,7 +11,17 @@
  *
  * The reference decodes one sequence per call; here `sequences` caches advance together, each with its
  * own length.  All pointers are device pointers unless said otherwise.  Status codes are the moe_status
- * values of moe_b200.h.
+ * values of moe_b200.h.  Calls on one cache are ordered by the caller (one stream, or events between streams): they share its lengths and
+ * its workspace; two captured graphs of one cache may be replayed one after the other, not at once.
+ *
+ * A cache of MOE_PRECISION_Q4 holds 4 bits a channel.  For every position, kv head and run of 32 channels of its key (after the rotation)
+ * and of its value:
+ *     step = bf16((high - low) / 15),  base = bf16(low),  code = clamp(round((x - base) / step), 0, 15)   (0 where step is 0)
+ *     what the cache stands for = code * step + base
+ * in f32 arithmetic, rounding to even, rotation included (two products and their sum, not contracted; the angles are computed in 64 bits).
+ * A step's own new positions are read back from the cache like all others.  If a position's key or value of a kv head holds a NaN, an
+ * infinity or a number above 2^126 in magnitude, its key and value stand for NaN: what attends to it is NaN, what does not is untouched.
+ * Neither call below allocates on such a cache, so every step can be captured; q is left alone.
  */
 #ifndef KV_ATTENTION_B200_H
 #define KV_ATTENTION_B200_H
@@ -33,7 +43,8 @@ typedef struct {
   int32_t max_seq_len;  /* length of the RoPE tables (rope.rs:71-97); capacity <= max_seq_len */
   float rope_base;      /* 10000.0 in the reference's configs */
   int32_t rope;         /* 0: no rotation (rope_enabled == false) */
-  int32_t precision;    /* MOE_PRECISION_F32 (0) or MOE_PRECISION_BF16 (1): type of q, k, v, out and of the cache */
+  int32_t precision;    /* MOE_PRECISION_F32 (0) or MOE_PRECISION_BF16 (1): type of q, k, v, out and of the cache;
+                           MOE_PRECISION_Q4 (3): bf16 q, k, v and out, the cache in 4 bits (head_dim 32, 64, 128 or 256) */
   int32_t device;
 } kv_cache_config_t;
 
@@ -74,6 +85,21 @@ int32_t kv_attention_forward_cached(kv_cache_t* cache, int32_t first_sequence, i
 /* Drops the newest positions of a sequence (all sequences when sequence < 0) so that `length` remain;
  * a length above the current one is InvalidInput.  Used to replay a decode step at a fixed history. */
 int32_t kv_cache_truncate(kv_cache_t* cache, int32_t sequence, int32_t length, void* stream);
+
+/* KvCache::append (attention.rs:65-78) without a query: rotates and stores rows new keys and values for each sequence of the range, layout
+ * as above, and moves the lengths on.  Fills a cache whose attention output is not wanted (a prompt's prefix, a cache handed over). */
+int32_t kv_cache_append(kv_cache_t* cache, int32_t first_sequence, int32_t n_sequences, const void* k, const void* v,
+                        int32_t rows_per_sequence, void* stream);
+
+/* Takes back the newest rows of each sequence of the range (draft tokens that were not accepted).  Unlike kv_cache_truncate it counts from
+ * each sequence's own length, on the device, so that a captured step can contain it; a sequence whose step was skipped for want of room is
+ * left alone.  More rows than a sequence holds are InvalidInput. */
+int32_t kv_cache_rollback(kv_cache_t* cache, int32_t first_sequence, int32_t n_sequences, int32_t rows_per_sequence, void* stream);
+
+/* The newest rows of each sequence of the range as the cache holds them, into device memory: f32
+ * [n_sequences * rows_per_sequence, kv_heads * head_dim] each. */
+int32_t kv_cache_newest(kv_cache_t* cache, int32_t first_sequence, int32_t n_sequences, int32_t rows_per_sequence, float* keys,
+                        float* values, void* stream);
 
 /* Read-only views for tests and for handing a cache back: keys / values of one sequence,
  * [len, kv_heads * head_dim] as f32, into host memory. */

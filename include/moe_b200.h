@@ -46,7 +46,8 @@ typedef enum {
 typedef enum {
   MOE_PRECISION_F32 = 0,  /* f32 storage and f32 FMA products (TransformerBuilder::mixed_precision(false)) */
   MOE_PRECISION_BF16 = 1, /* bf16 activations and weights on the tensor cores, f32 accumulate and f32 master weights */
-  MOE_PRECISION_Q8 = 2    /* inference only: int8 expert weights with one f32 scale per output row, bf16 activations */
+  MOE_PRECISION_Q8 = 2,   /* inference only: int8 expert weights with one f32 scale per output row, bf16 activations */
+  MOE_PRECISION_Q4 = 3    /* KV caches only (kv_attention_b200.h): keys and values in 4 bits, bf16 activations */
 } moe_precision;
 
 /* Which projection of the layer; order follows MoeLayer::params_mut (moe.rs:516-525). */

@@ -12,7 +12,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmoe_b200.so")
 
 OK, INVALID_CONFIG, INVALID_INPUT, CUDA_ERROR, OUT_OF_MEMORY, UNSUPPORTED, TIMEOUT, COMM_ERROR, POISONED = range(9)
-PRECISION_F32, PRECISION_BF16, PRECISION_Q8 = 0, 1, 2
+PRECISION_F32, PRECISION_BF16, PRECISION_Q8, PRECISION_Q4 = 0, 1, 2, 3
 W_ROUTER, W_GATE, W_UP, W_DOWN, W_SHARED_GATE, W_SHARED_UP, W_SHARED_DOWN = range(7)
 
 
@@ -149,6 +149,9 @@ def lib() -> C.CDLL:
         "kv_cache_truncate": (i32, [vp, i32, i32, vp]),
         "kv_cache_lengths": (i32, [vp, ip, vp]),
         "kv_attention_forward_cached": (i32, [vp, i32, i32, vp, vp, vp, i32, vp, vp]),
+        "kv_cache_append": (i32, [vp, i32, i32, vp, vp, i32, vp]),
+        "kv_cache_rollback": (i32, [vp, i32, i32, i32, vp]),
+        "kv_cache_newest": (i32, [vp, i32, i32, i32, vp, vp, vp]),
         "kv_cache_read": (i32, [vp, i32, fp, fp, vp]),
         "rmsnorm_forward": (i32, [vp, vp, vp, i32, i32, f32, i32, vp, C.c_char_p, i32]),
         "rmsnorm_scratch_bytes": (C.c_int64, [i32, i32]),

@@ -26,6 +26,7 @@
 #include "../../include/kv_attention_b200.h"
 #include "../../include/moe_b200.h"
 #include "common.cuh"
+#include "kv_q4.cuh"
 
 namespace moe {
 namespace {
@@ -537,6 +538,32 @@ __global__ void kv_set_lengths_kernel(int* lengths, int* full, int first, int co
   if (i < count) { lengths[first + i] = value; full[first + i] = 0; }
 }
 
+// A call that stores rows without attending to anything moves the lengths on by itself; a sequence without room is marked.
+__global__ void kv_advance_kernel(int* lengths, int* full, int first, int count, int rows, int cap) {
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= count) return;
+  if (lengths[first + i] + rows > cap) full[first + i] = 1;
+  else lengths[first + i] += rows;
+}
+
+// Takes the newest rows of every sequence back.  A sequence whose last step was skipped for want of room has nothing to take back.
+__global__ void kv_rollback_kernel(int* lengths, const int* full, int first, int count, int rows) {
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i < count && !full[first + i]) lengths[first + i] = max(0, lengths[first + i] - rows);
+}
+
+// The newest `rows` positions of every sequence as f32, one CTA per position; a position that is not held reads 0.
+template <typename T>
+__global__ void kv_newest_kernel(const T* __restrict__ keys, const T* __restrict__ values, const int* __restrict__ lengths, int first, int rows,
+                                 int cap, int W, float* __restrict__ keys_out, float* __restrict__ values_out) {
+  const int seq = first + blockIdx.x / rows, pos = lengths[seq] - rows + blockIdx.x % rows;
+  const size_t src = ((size_t)seq * cap + max(pos, 0)) * W, dst = (size_t)blockIdx.x * W;
+  for (int i = threadIdx.x; i < W; i += blockDim.x) {
+    keys_out[dst + i] = pos >= 0 ? to_f32<T>(keys[src + i]) : 0.f;
+    values_out[dst + i] = pos >= 0 ? to_f32<T>(values[src + i]) : 0.f;
+  }
+}
+
 template <typename T>
 __global__ void kv_to_f32_kernel(const T* __restrict__ src, float* __restrict__ dst, long long n) {
   const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
@@ -550,8 +577,9 @@ using namespace moe;
 
 struct kv_cache {
   kv_cache_config_t cfg{};
-  void* keys = nullptr;
+  void* keys = nullptr;             // 4-bit caches: the pages, keys and values together
   void* values = nullptr;
+  int* tickets = nullptr;           // 4-bit caches: CTAs of a sequence that are done with it, zero between calls
   int* lengths = nullptr;           // device, one per sequence
   int* full = nullptr;              // device, one per sequence: set by a step that found no room (a replayed graph can get there)
   std::vector<int> host_full;
@@ -684,6 +712,56 @@ int forward_t(kv_cache* c, int first, int n_seq, void* q, const void* k, const v
   return MOE_OK;
 }
 
+q4::Cache q4_view(const kv_cache* c) {
+  const kv_cache_config_t& g = c->cfg;
+  return q4::Cache{(unsigned char*)c->keys, c->lengths, c->full, c->tickets, c->cos_t, c->sin_t, g.num_heads, g.kv_heads, g.head_dim, g.capacity, g.rope};
+}
+
+// The step on a 4-bit cache: one launch where the new rows' queries fit one pass and a cluster joins the slices.  Nothing is allocated.
+int forward_q4(kv_cache* c, int first, int n_seq, const void* q, const void* k, const void* v, int rows, void* merged, cudaStream_t st) {
+  const kv_cache_config_t& g = c->cfg;
+  const q4::Cache view = q4_view(c);
+  int longest = 0;
+  for (int i = 0; i < n_seq; ++i) longest = std::max(longest, c->host_len[first + i] + rows);
+  const long long nq = (long long)rows * (g.num_heads / g.kv_heads);
+  const int per_pass = q4::queries_per_pass(g.head_dim, (int)std::min<long long>(nq, 1 << 20));
+  const long long passes = (nq + per_pass - 1) / per_pass, ctas = (long long)n_seq * g.kv_heads * passes;
+  // about four CTAs per SM, a page or more for each warp
+  const int pages = ceil_div(longest, q4::PAGE);
+  int splits = (int)std::min<long long>(KV_MAX_SPLITS, std::max<long long>(1, (4ll * c->sm_count + ctas - 1) / ctas));
+  splits = std::max(1, std::min(splits, ceil_div(pages, 4)));
+  if (splits > q4::CLUSTER && ((size_t)n_seq * rows * g.num_heads * splits * (g.head_dim + 2) > c->part_floats)) splits = q4::CLUSTER;
+  if (ctas * splits > 0x7fffffffll) return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: too many rows");
+  const bool append = passes == 1;   // one CTA per slice: it stores the slice's new positions itself
+  if (!append) KCK(q4::launch_append(view, (const bf16*)k, (const bf16*)v, first, n_seq, rows, st));
+  const float scale_log2 = LOG2E / sqrtf((float)g.head_dim);
+  KCK(q4::launch_attention(view, (const bf16*)q, (const bf16*)k, (const bf16*)v, first, n_seq, rows, splits, append, scale_log2, (bf16*)merged, c->part, st));
+  if (splits > q4::CLUSTER) {
+    const KvShape s{g.num_heads, g.kv_heads, g.head_dim, g.capacity, rows, first};
+    kv_merge_kernel<bf16><<<n_seq * rows * g.num_heads, std::min(256, g.head_dim), 0, st>>>(c->part, (bf16*)merged, c->lengths, c->full, s, splits);
+    count_launch();
+    KCK(cudaGetLastError());
+  }
+  for (int i = 0; i < n_seq; ++i) c->host_len[first + i] += rows;
+  return MOE_OK;
+}
+
+// The checks that every call with new rows makes.
+int check_step(kv_cache* c, int first, int n_seq, int rows) {
+  const kv_cache_config_t& g = c->cfg;
+  if (first < 0 || n_seq <= 0 || first + n_seq > g.sequences)
+    return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: sequences %d .. %d of %d", first, first + n_seq - 1, g.sequences);
+  if (rows <= 0) return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: empty step or null buffer");
+  if ((long long)n_seq * rows * g.num_heads > 0x7fffffffll) return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: too many rows");
+  return MOE_OK;
+}
+int check_room(kv_cache* c, int first, int n_seq, int rows) {
+  for (int i = 0; i < n_seq; ++i)
+    if (c->host_len[first + i] + rows > c->cfg.capacity)
+      return kv_fail(c, MOE_INVALID_INPUT, "SequenceTooLong: length %d, max_seq_len %d (sequence %d)", c->host_len[first + i] + rows, c->cfg.capacity, first + i);
+  return MOE_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -703,17 +781,30 @@ int32_t kv_cache_create(const kv_cache_config_t* config, kv_cache_t** out) {
   if (g.head_dim <= 0 || g.head_dim % 2 != 0)
     return kv_fail(c, MOE_INVALID_CONFIG, "InvalidConfig: rope head_dim must be even and non-zero, got %d", g.head_dim);
   if (!head_dim_ok(g.head_dim)) return kv_fail(c, MOE_UNSUPPORTED, "Unsupported: head_dim %d (8, 16, 32, 64, 128, 256)", g.head_dim);
-  if (g.precision != MOE_PRECISION_F32 && g.precision != MOE_PRECISION_BF16)
-    return kv_fail(c, MOE_INVALID_CONFIG, "InvalidConfig: precision is f32 or bf16");
+  const bool is_q4 = g.precision == MOE_PRECISION_Q4;
+  if (g.precision != MOE_PRECISION_F32 && g.precision != MOE_PRECISION_BF16 && !is_q4)
+    return kv_fail(c, MOE_INVALID_CONFIG, "InvalidConfig: precision is f32, bf16 or q4");
+  if (is_q4 && !q4::head_dim_ok(g.head_dim)) return kv_fail(c, MOE_UNSUPPORTED, "Unsupported: head_dim %d of a 4-bit cache (32, 64, 128, 256)", g.head_dim);
   if (g.max_seq_len < g.capacity) return kv_fail(c, MOE_INVALID_CONFIG, "InvalidConfig: capacity %d exceeds max_seq_len %d", g.capacity, g.max_seq_len);
   KCK(cudaSetDevice(g.device));
   cudaDeviceProp prop;
   KCK(cudaGetDeviceProperties(&prop, g.device));
   c->sm_count = prop.multiProcessorCount;
-  const size_t bytes = (size_t)g.sequences * g.capacity * g.kv_heads * g.head_dim * elem_size(c);
-  if (cudaMalloc(&c->keys, bytes) != cudaSuccess || cudaMalloc(&c->values, bytes) != cudaSuccess) {
-    cudaGetLastError();
-    return kv_fail(c, MOE_OUT_OF_MEMORY, "OutOfMemory: two cache buffers of %zu bytes", bytes);
+  if (is_q4) {
+    const size_t bytes = (size_t)g.sequences * g.kv_heads * q4::head_pages(g.capacity) * q4::page_bytes(g.head_dim);
+    if (cudaMalloc(&c->keys, bytes) != cudaSuccess) {
+      cudaGetLastError();
+      return kv_fail(c, MOE_OUT_OF_MEMORY, "OutOfMemory: a cache buffer of %zu bytes", bytes);
+    }
+    KCK(cudaMemset(c->keys, 0, bytes));   // what lies behind the last position is multiplied by 0: it has to be finite
+    KCK(cudaMalloc(&c->tickets, sizeof(int) * g.sequences));
+    KCK(cudaMemset(c->tickets, 0, sizeof(int) * g.sequences));
+  } else {
+    const size_t bytes = (size_t)g.sequences * g.capacity * g.kv_heads * g.head_dim * elem_size(c);
+    if (cudaMalloc(&c->keys, bytes) != cudaSuccess || cudaMalloc(&c->values, bytes) != cudaSuccess) {
+      cudaGetLastError();
+      return kv_fail(c, MOE_OUT_OF_MEMORY, "OutOfMemory: two cache buffers of %zu bytes", bytes);
+    }
   }
   KCK(cudaMalloc(&c->lengths, sizeof(int) * g.sequences));
   KCK(cudaMemset(c->lengths, 0, sizeof(int) * g.sequences));
@@ -729,8 +820,15 @@ int32_t kv_cache_create(const kv_cache_config_t* config, kv_cache_t** out) {
     c->part = nullptr; c->part_floats = 0;
     return kv_fail(c, MOE_OUT_OF_MEMORY, "OutOfMemory: slice results");
   }
-  // the tables of Rope::new (rope.rs:77-90), in f32 arithmetic like the reference
   const int half = g.head_dim / 2;
+  if (is_q4) {   // no counterpart in the reference to agree with: the angles of far positions in 64 bits
+    KCK(cudaMalloc(&c->cos_t, (size_t)g.max_seq_len * half * sizeof(float)));
+    KCK(cudaMalloc(&c->sin_t, (size_t)g.max_seq_len * half * sizeof(float)));
+    KCK(q4::launch_tables(c->cos_t, c->sin_t, g.max_seq_len, g.head_dim, g.rope_base, nullptr));
+    KCK(cudaStreamSynchronize(nullptr));
+    return MOE_OK;
+  }
+  // the tables of Rope::new (rope.rs:77-90), in f32 arithmetic like the reference
   std::vector<float> co((size_t)g.max_seq_len * half), si((size_t)g.max_seq_len * half);
   for (int p = 0; p < g.max_seq_len; ++p)
     for (int ch = 0; ch < half; ++ch) {
@@ -750,7 +848,7 @@ int32_t kv_cache_create(const kv_cache_config_t* config, kv_cache_t** out) {
 void kv_cache_destroy(kv_cache_t* c) {
   if (!c) return;
   cudaFree(c->keys); cudaFree(c->values); cudaFree(c->lengths); cudaFree(c->full); cudaFree(c->cos_t); cudaFree(c->sin_t);
-  cudaFree(c->part); cudaFree(c->read_buf);
+  cudaFree(c->part); cudaFree(c->read_buf); cudaFree(c->tickets);
   delete c;
 }
 
@@ -796,16 +894,81 @@ int32_t kv_attention_forward_cached(kv_cache_t* c, int32_t first, int32_t n_seq,
                                     int32_t rows, void* merged, void* stream) {
   if (!c) return MOE_INVALID_INPUT;
   const kv_cache_config_t& g = c->cfg;
-  if (first < 0 || n_seq <= 0 || first + n_seq > g.sequences)
-    return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: sequences %d .. %d of %d", first, first + n_seq - 1, g.sequences);
-  if (rows <= 0 || !q || !k || !v || !merged) return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: empty step or null buffer");
-  if ((long long)n_seq * rows * g.num_heads > 0x7fffffffll) return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: too many rows");
-  for (int i = 0; i < n_seq; ++i)
-    if (c->host_len[first + i] + rows > g.capacity)
-      return kv_fail(c, MOE_INVALID_INPUT, "SequenceTooLong: length %d, max_seq_len %d (sequence %d)", c->host_len[first + i] + rows, g.capacity, first + i);
+  int rc = check_step(c, first, n_seq, rows);
+  if (rc != MOE_OK) return rc;
+  if (!q || !k || !v || !merged) return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: empty step or null buffer");
+  if ((rc = check_room(c, first, n_seq, rows)) != MOE_OK) return rc;
   KCK(cudaSetDevice(g.device));
+  if (g.precision == MOE_PRECISION_Q4) return forward_q4(c, first, n_seq, q, k, v, rows, merged, (cudaStream_t)stream);
   return g.precision == MOE_PRECISION_BF16 ? forward_t<bf16>(c, first, n_seq, q, k, v, rows, merged, (cudaStream_t)stream)
                                            : forward_t<float>(c, first, n_seq, q, k, v, rows, merged, (cudaStream_t)stream);
+}
+
+int32_t kv_cache_append(kv_cache_t* c, int32_t first, int32_t n_seq, const void* k, const void* v, int32_t rows, void* stream) {
+  if (!c) return MOE_INVALID_INPUT;
+  const kv_cache_config_t& g = c->cfg;
+  int rc = check_step(c, first, n_seq, rows);
+  if (rc != MOE_OK) return rc;
+  if (!k || !v) return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: empty step or null buffer");
+  if ((rc = check_room(c, first, n_seq, rows)) != MOE_OK) return rc;
+  KCK(cudaSetDevice(g.device));
+  cudaStream_t st = (cudaStream_t)stream;
+  if (g.precision == MOE_PRECISION_Q4) {
+    KCK(q4::launch_append(q4_view(c), (const bf16*)k, (const bf16*)v, first, n_seq, rows, st));
+  } else {
+    const KvShape s{0, g.kv_heads, g.head_dim, g.capacity, rows, first};   // no query heads to rotate
+    if (g.precision == MOE_PRECISION_BF16)
+      kv_append_kernel<bf16><<<n_seq * rows, 256, 0, st>>>(nullptr, (const bf16*)k, (const bf16*)v, (bf16*)c->keys, (bf16*)c->values, c->lengths, c->cos_t, c->sin_t, s, g.rope);
+    else
+      kv_append_kernel<float><<<n_seq * rows, 256, 0, st>>>(nullptr, (const float*)k, (const float*)v, (float*)c->keys, (float*)c->values, c->lengths, c->cos_t, c->sin_t, s, g.rope);
+    count_launch();
+    KCK(cudaGetLastError());
+  }
+  kv_advance_kernel<<<ceil_div(n_seq, 256), 256, 0, st>>>(c->lengths, c->full, first, n_seq, rows, g.capacity);
+  count_launch();
+  KCK(cudaGetLastError());
+  for (int i = 0; i < n_seq; ++i) c->host_len[first + i] += rows;
+  return MOE_OK;
+}
+
+int32_t kv_cache_rollback(kv_cache_t* c, int32_t first, int32_t n_seq, int32_t rows, void* stream) {
+  if (!c) return MOE_INVALID_INPUT;
+  const int rc = check_step(c, first, n_seq, rows);
+  if (rc != MOE_OK) return rc;
+  for (int i = 0; i < n_seq; ++i)
+    if (c->host_len[first + i] < rows)
+      return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: sequence %d holds %d positions, cannot drop %d", first + i, c->host_len[first + i], rows);
+  KCK(cudaSetDevice(c->cfg.device));
+  kv_rollback_kernel<<<ceil_div(n_seq, 256), 256, 0, (cudaStream_t)stream>>>(c->lengths, c->full, first, n_seq, rows);
+  count_launch();
+  KCK(cudaGetLastError());
+  for (int i = 0; i < n_seq; ++i) c->host_len[first + i] -= rows;
+  return MOE_OK;
+}
+
+int32_t kv_cache_newest(kv_cache_t* c, int32_t first, int32_t n_seq, int32_t rows, float* keys, float* values, void* stream) {
+  if (!c) return MOE_INVALID_INPUT;
+  const kv_cache_config_t& g = c->cfg;
+  const int rc = check_step(c, first, n_seq, rows);
+  if (rc != MOE_OK) return rc;
+  if (!keys || !values) return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: null buffer");
+  for (int i = 0; i < n_seq; ++i)
+    if (c->host_len[first + i] < rows)
+      return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: sequence %d holds %d positions, not %d", first + i, c->host_len[first + i], rows);
+  KCK(cudaSetDevice(g.device));
+  cudaStream_t st = (cudaStream_t)stream;
+  if (g.precision == MOE_PRECISION_Q4) {
+    KCK(q4::launch_values(q4_view(c), first, n_seq, -1, rows, keys, values, st));
+    return MOE_OK;
+  }
+  const int W = g.kv_heads * g.head_dim;
+  if (g.precision == MOE_PRECISION_BF16)
+    kv_newest_kernel<bf16><<<n_seq * rows, 128, 0, st>>>((const bf16*)c->keys, (const bf16*)c->values, c->lengths, first, rows, g.capacity, W, keys, values);
+  else
+    kv_newest_kernel<float><<<n_seq * rows, 128, 0, st>>>((const float*)c->keys, (const float*)c->values, c->lengths, first, rows, g.capacity, W, keys, values);
+  count_launch();
+  KCK(cudaGetLastError());
+  return MOE_OK;
 }
 
 int32_t kv_cache_read(kv_cache_t* c, int32_t sequence, float* keys_host, float* values_host, void* stream) {
@@ -814,11 +977,21 @@ int32_t kv_cache_read(kv_cache_t* c, int32_t sequence, float* keys_host, float* 
   const size_t W = (size_t)g.kv_heads * g.head_dim, n = (size_t)c->host_len[sequence] * W;
   if (n == 0) return MOE_OK;
   cudaStream_t st = (cudaStream_t)stream;
-  if (n > c->read_floats) {
+  const bool is_q4 = g.precision == MOE_PRECISION_Q4;   // keys and values come out of one launch
+  const size_t need = is_q4 ? 2 * n : n;
+  if (is_q4) KCK(cudaSetDevice(g.device));
+  if (need > c->read_floats) {
     cudaFree(c->read_buf);
     c->read_buf = nullptr; c->read_floats = 0;
-    KCK(cudaMalloc(&c->read_buf, n * sizeof(float)));
-    c->read_floats = n;
+    KCK(cudaMalloc(&c->read_buf, need * sizeof(float)));
+    c->read_floats = need;
+  }
+  if (is_q4) {
+    KCK(q4::launch_values(q4_view(c), sequence, 1, 0, c->host_len[sequence], c->read_buf, c->read_buf + n, st));
+    if (keys_host) KCK(cudaMemcpyAsync(keys_host, c->read_buf, n * sizeof(float), cudaMemcpyDeviceToHost, st));
+    if (values_host) KCK(cudaMemcpyAsync(values_host, c->read_buf + n, n * sizeof(float), cudaMemcpyDeviceToHost, st));
+    KCK(cudaStreamSynchronize(st));
+    return MOE_OK;
   }
   for (int which = 0; which < 2; ++which) {
     float* host = which == 0 ? keys_host : values_host;

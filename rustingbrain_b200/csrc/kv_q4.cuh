@@ -1,0 +1,43 @@
+// The 4-bit side of the KV cache (kv_q4.cu), driven by kv_attention.cu.
+#pragma once
+#include "common.cuh"
+
+namespace moe {
+namespace q4 {
+
+constexpr int PAGE = 64;               // positions of one sequence and kv head that lie together
+constexpr int GROUP = 32;              // channels that share a step and a base
+constexpr int CLUSTER = 8;             // slices that one cluster joins; more go through the caller's slice buffer
+
+inline long long page_bytes(int head_dim) { return 80ll * head_dim; }   // two codes of 4 bits and 2 x 4 bytes per 32 channels, 64 times
+inline long long head_pages(int capacity) { return (capacity + PAGE - 1) / PAGE; }
+inline bool head_dim_ok(int hd) { return hd == 32 || hd == 64 || hd == 128 || hd == 256; }
+
+struct Cache {
+  unsigned char* pages;                // [sequence][kv head][page], page_bytes each
+  int* lengths;                        // [sequence]
+  int* full;                           // [sequence]: a step found no room
+  int* tickets;                        // [sequence], zero between calls
+  const float *cos_t, *sin_t;          // [position][head_dim / 2]
+  int H, Hkv, HD, cap, rope;
+};
+
+// cos and sin of position * base^(-2 c / head_dim), the angles in 64 bits
+cudaError_t launch_tables(float* cos_t, float* sin_t, int positions, int head_dim, float base, cudaStream_t st);
+
+// Rotates, quantises and stores rows new keys and values of each sequence behind its length; lengths stay as they are.
+cudaError_t launch_append(const Cache& c, const bf16* k, const bf16* v, int first, int n_seq, int rows, cudaStream_t st);
+
+// Queries that one pass over the cache serves, per kv head.
+int queries_per_pass(int head_dim, int queries);
+// One attention step.  With append set (only if rows * group fit one pass) it stores the new rows itself.  splits <= CLUSTER: writes merged and
+// advances the lengths; more: leaves slice results in part, for kv_merge_kernel.
+cudaError_t launch_attention(const Cache& c, const bf16* q, const bf16* k, const bf16* v, int first, int n_seq, int rows, int splits, bool append,
+                             float scale_log2, bf16* merged, float* part, cudaStream_t st);
+
+// Values of `count` positions of each of n_seq sequences as f32 [n_seq * count, Hkv * HD]: positions from .. from + count - 1, or the
+// newest `count` when from < 0.  Positions that are not held read 0.
+cudaError_t launch_values(const Cache& c, int first, int n_seq, int from, int count, float* keys, float* values, cudaStream_t st);
+
+}  // namespace q4
+}  // namespace moe

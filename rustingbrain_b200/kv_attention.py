@@ -15,17 +15,21 @@ from . import _lib
 from .moe import CudaError, InvalidConfig, InvalidInput, NetworkError, _stream
 
 _ERRORS = {_lib.INVALID_CONFIG: InvalidConfig, _lib.INVALID_INPUT: InvalidInput, _lib.UNSUPPORTED: InvalidConfig}
+_PRECISIONS = {"f32": _lib.PRECISION_F32, "bf16": _lib.PRECISION_BF16, "q4": _lib.PRECISION_Q4}
 
 
 class KvCache:
     """``sequences`` caches of ``capacity`` positions (KvCache::with_capacity, attention.rs:39-48) and the
-    RoPE tables for ``max_seq_len`` positions (Rope::new, rope.rs:71-97)."""
+    RoPE tables for ``max_seq_len`` positions (Rope::new, rope.rs:71-97).
+
+    ``precision`` is the type of the activations and of the cache, "f32" or "bf16"; "q4" keeps the cache in 4 bits with a step and a base
+    per 32 channels of a head (bf16 activations, head_dim 32, 64, 128 or 256): a third of the bytes of a bf16 cache."""
 
     def __init__(self, sequences: int, num_heads: int, kv_heads: int, head_dim: int, capacity: int,
                  max_seq_len: Optional[int] = None, rope_base: float = 10000.0, rope: bool = True,
                  precision: str = "bf16", device: int = 0):
-        if precision not in ("f32", "bf16"):
-            raise InvalidConfig("precision is 'f32' or 'bf16'")
+        if precision not in _PRECISIONS:
+            raise InvalidConfig("precision is 'f32', 'bf16' or 'q4'")
         self.sequences, self.num_heads, self.kv_heads, self.head_dim = sequences, num_heads, kv_heads, head_dim
         self.capacity = capacity
         self.precision = precision
@@ -33,8 +37,9 @@ class KvCache:
         cfg = _lib.KvCacheConfigC(sequences=sequences, num_heads=num_heads, kv_heads=kv_heads, head_dim=head_dim,
                                   capacity=capacity, max_seq_len=max_seq_len if max_seq_len is not None else capacity,
                                   rope_base=rope_base, rope=1 if rope else 0,
-                                  precision=_lib.PRECISION_BF16 if precision == "bf16" else _lib.PRECISION_F32,
-                                  device=device)
+                                  precision=_PRECISIONS[precision], device=device)
+        self.device = device
+        self._forward = _lib.lib().kv_attention_forward_cached
         rc = _lib.lib().kv_cache_create(C.byref(cfg), C.byref(self._h))
         if rc != _lib.OK:
             text = _lib.lib().kv_cache_last_error(self._h).decode(errors="replace") if self._h else "kv_cache_create failed"
@@ -45,7 +50,7 @@ class KvCache:
 
     def __del__(self):
         h = getattr(self, "_h", None)
-        if h:
+        if h and _lib is not None and _lib.lib is not None:      # both are gone at the interpreter's own end
             _lib.lib().kv_cache_destroy(h)
             self._h = C.c_void_p()
 
@@ -85,19 +90,50 @@ class KvCache:
         import torch
         n_seq = self.sequences - first_sequence if n_sequences is None else n_sequences
         rows = n_seq * rows_per_sequence
-        dt = torch.bfloat16 if self.precision == "bf16" else torch.float32
-        want = ((rows, self.num_heads * self.head_dim), (rows, self.kv_heads * self.head_dim), (rows, self.kv_heads * self.head_dim))
-        for t, shape, name in zip((q, k, v), want, "qkv"):
-            if not (t.is_cuda and t.is_contiguous() and t.dtype == dt and tuple(t.shape) == shape):
-                raise InvalidInput("%s must be a contiguous %s device tensor of shape %s" % (name, dt, shape))
+        W = self.kv_heads * self.head_dim
+        self._rows(q, rows, self.num_heads * self.head_dim, "q")
+        self._rows(k, rows, W, "k")
+        self._rows(v, rows, W, "v")
         if out is None:
             out = torch.empty_like(q)
-        if stream is None:
-            stream = torch.cuda.current_stream().cuda_stream
-        self._check(_lib.lib().kv_attention_forward_cached(self._h, first_sequence, n_seq, C.c_void_p(q.data_ptr()),
-                                                          C.c_void_p(k.data_ptr()), C.c_void_p(v.data_ptr()),
-                                                          rows_per_sequence, C.c_void_p(out.data_ptr()), _stream(stream)))
+        self._check(self._forward(self._h, first_sequence, n_seq, q.data_ptr(), k.data_ptr(), v.data_ptr(), rows_per_sequence,
+                                  out.data_ptr(), self._on(stream)))
         return out
+
+    def _rows(self, t, rows, width, name) -> None:
+        import torch
+        dt = torch.float32 if self.precision == "f32" else torch.bfloat16
+        if not (t.is_cuda and t.is_contiguous() and t.dtype == dt and tuple(t.shape) == (rows, width)):
+            raise InvalidInput("%s must be a contiguous %s device tensor of shape %s" % (name, dt, (rows, width)))
+
+    def _on(self, stream):
+        """The given stream, or the current one of the cache's device."""
+        import torch
+        return torch._C._cuda_getCurrentRawStream(self.device) if stream is None else int(stream)
+
+    def append(self, k, v, rows_per_sequence: int = 1, first_sequence: int = 0, n_sequences: Optional[int] = None, stream=None) -> None:
+        """``KvCache::append`` (attention.rs:65-78): stores new keys (rotated here) and values without attending to anything."""
+        n_seq = self.sequences - first_sequence if n_sequences is None else n_sequences
+        W = self.kv_heads * self.head_dim
+        self._rows(k, n_seq * rows_per_sequence, W, "k")
+        self._rows(v, n_seq * rows_per_sequence, W, "v")
+        self._check(_lib.lib().kv_cache_append(self._h, first_sequence, n_seq, k.data_ptr(), v.data_ptr(), rows_per_sequence, self._on(stream)))
+
+    def rollback(self, rows_per_sequence: int, first_sequence: int = 0, n_sequences: Optional[int] = None, stream=None) -> None:
+        """Takes back the newest rows of every sequence of the range, as after draft tokens that were not accepted."""
+        n_seq = self.sequences - first_sequence if n_sequences is None else n_sequences
+        self._check(_lib.lib().kv_cache_rollback(self._h, first_sequence, n_seq, rows_per_sequence, self._on(stream)))
+
+    def newest(self, rows_per_sequence: int = 1, first_sequence: int = 0, n_sequences: Optional[int] = None, stream=None):
+        """The newest rows of every sequence of the range as the cache holds them: f32 device tensors
+        [n_sequences * rows_per_sequence, kv_heads * head_dim], keys (after the rotation) and values."""
+        import torch
+        n_seq = self.sequences - first_sequence if n_sequences is None else n_sequences
+        shape = (max(n_seq, 0) * max(rows_per_sequence, 0), self.kv_heads * self.head_dim)
+        keys = torch.empty(shape, dtype=torch.float32, device="cuda:%d" % self.device)
+        values = torch.empty_like(keys)
+        self._check(_lib.lib().kv_cache_newest(self._h, first_sequence, n_seq, rows_per_sequence, keys.data_ptr(), values.data_ptr(), self._on(stream)))
+        return keys, values
 
 
 __all__ = ["KvCache", "NetworkError"]
