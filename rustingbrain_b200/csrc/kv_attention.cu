@@ -726,10 +726,11 @@ int forward_q4(kv_cache* c, int first, int n_seq, const void* q, const void* k, 
   const long long nq = (long long)rows * (g.num_heads / g.kv_heads);
   const int per_pass = q4::queries_per_pass(g.head_dim, (int)std::min<long long>(nq, 1 << 20));
   const long long passes = (nq + per_pass - 1) / per_pass, ctas = (long long)n_seq * g.kv_heads * passes;
-  // about four CTAs per SM, a page or more for each warp
+  // as many CTAs as are resident at once, a page or more for each warp
   const int pages = ceil_div(longest, q4::PAGE);
-  int splits = (int)std::min<long long>(KV_MAX_SPLITS, std::max<long long>(1, (4ll * c->sm_count + ctas - 1) / ctas));
+  int splits = (int)std::min<long long>(KV_MAX_SPLITS, std::max<long long>(1, 4ll * c->sm_count / ctas));
   splits = std::max(1, std::min(splits, ceil_div(pages, 4)));
+  if (const char* v = getenv("KV_B200_SPLITS")) splits = std::max(1, std::min(KV_MAX_SPLITS, atoi(v)));   // experiments
   if (splits > q4::CLUSTER && ((size_t)n_seq * rows * g.num_heads * splits * (g.head_dim + 2) > c->part_floats)) splits = q4::CLUSTER;
   if (ctas * splits > 0x7fffffffll) return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: too many rows");
   const bool append = passes == 1;   // one CTA per slice: it stores the slice's new positions itself

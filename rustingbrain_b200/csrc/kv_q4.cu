@@ -9,16 +9,19 @@
 // reduction.  So the few queries that share a kv head fill the small side of the product, and both K and V are the A operand:
 // a lane's 32-bit word holds 8 codes that it needs itself, keys as 8 channels of one position, values as 8 positions of one channel,
 // so that a word costs seven instructions to become four pairs of bf16 numbers 128 + code.
-//   keys:   the sum over 32 channels starts at -128 sum(q) and then takes step and base in f32: S += step * sum + base * sum(q).
+//   keys:   S = sum over groups of step * sum_c (128 + code) q + (base - 128 step) * sum_c q.  The first product takes its step in f32; the
+//           second part, base and step against the queries' sums in three bf16 pieces, is one more small product on the tensor cores.
 //           Nothing of the key is rounded.
 //   values: step and base belong to the position, which is what the product sums over, so they go on before it: two packed
 //           bf16 instructions, one rounding of the value to bf16 (2^-9 of it; P is rounded alike).
 //
 // Page layout, HD = head_dim, NG = HD / 32:
 //   keys    [64 positions][4 t][NG g] words: channels 32 g + 8 t + 2 i + e at nibble i + 4 e
+//   key parameters [64 positions][NG / 2][step of two groups, base of two groups] (bf16 pairs); NG = 1: step and base in one word
 //   values  [HD channels][4 t][2 w] words: positions 16 (2 w + i / 2) + 8 (i % 2) + 2 t + e at nibble i + 4 e
-//   key step | base      [64 positions][NG] (two bf16)
 //   value step, value base  [NG][64] bf16 each, position p at value_slot(p)
+// A warp streams half pages (keys, then values) through its own ring in shared memory.  The warp whose page takes a step's new positions
+// quantises them into its copy of the page and into the cache: nobody else reads them, so nobody has to wait.
 
 #include <cooperative_groups.h>
 #include <algorithm>
@@ -34,14 +37,19 @@ namespace q4 {
 namespace {
 
 constexpr int WARPS = 4, THREADS = WARPS * 32;
+constexpr float RISE = 8.f;                     // weights stay below 2^8 against the reference
 constexpr float HUGE_VALUE = 8.507059e37f;      // 2^126: a larger number counts as an infinity, so that high - low stays finite
 
 template <int HD> struct Layout {
-  static constexpr int NG = HD / GROUP, KEYS = 0, VALUES = 32 * HD, KPAR = 64 * HD, VSTEP = 72 * HD, VBASE = VSTEP + NG * 128, BYTES = 80 * HD;
+  static constexpr int NG = HD / GROUP, KEYS = 0, KPAR = 32 * HD, HALF = 40 * HD, VALUES = HALF, VSTEP = 72 * HD, VBASE = VSTEP + NG * 128, BYTES = 80 * HD;
 };
 __host__ __device__ inline int value_word(int p) { return ((p & 7) >> 1) * 2 + (p >> 5); }
 __host__ __device__ inline int value_nibble(int p) { return ((p >> 4) & 1) * 2 + ((p >> 3) & 1) + 4 * (p & 1); }
 __host__ __device__ inline int value_slot(int p) { return ((p & 7) >> 1) * 16 + (p >> 4) * 4 + ((p >> 3) & 1) * 2 + (p & 1); }
+
+// byte offset of a key's step in the page's key parameters; its base is base_after bytes behind
+__host__ __device__ inline int key_param(int slot, int g, int NG) { return slot * NG * 4 + (NG == 1 ? 0 : (g >> 1) * 8 + (g & 1) * 2); }
+__host__ __device__ inline int key_base_after(int NG) { return NG == 1 ? 2 : 4; }
 
 __device__ __forceinline__ unsigned char* page_at(const Cache& c, int seq, int kvh, int page) {
   const long long pages = (c.cap + PAGE - 1) / PAGE;
@@ -68,21 +76,18 @@ __device__ __forceinline__ void quantise(const float* x, uint32_t* code, uint32_
   }
 }
 
-// The CTA stores `count` new positions, first_slot .. of one page.  k and v point to the first new row of this head, `stride` elements apart;
-// pos0 is the first one's position in the sequence.  `codes` is [64][HD] bytes of shared memory.
+// One warp: the codes, steps and bases of one new position; lane l holds channels 32 g + l.  k and v point to the head's row.
 template <int HD>
-__device__ void append_page(const Cache& c, unsigned char* page, const bf16* k, const bf16* v, long long stride, int first_slot, int count,
-                            int pos0, unsigned char* codes) {
-  using L = Layout<HD>;
-  constexpr int NG = L::NG;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int r = warp; r < count; r += WARPS) {
-    const int slot = first_slot + r, pos = pos0 + r;
+struct Row {
+  static constexpr int NG = HD / GROUP;
+  uint32_t kcode[NG], kstep[NG], kbase[NG], vcode[NG], vstep[NG], vbase[NG];
+  __device__ __forceinline__ void make(const Cache& c, const bf16* __restrict__ k, const bf16* __restrict__ v, int pos) {
+    const int lane = threadIdx.x & 31;
     float x[NG], y[NG];
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      x[g] = __bfloat162float(k[r * stride + 32 * g + lane]);
-      y[g] = __bfloat162float(v[r * stride + 32 * g + lane]);
+      x[g] = __bfloat162float(k[32 * g + lane]);
+      y[g] = __bfloat162float(v[32 * g + lane]);
     }
     if (c.rope) {
       // the same steps as in 32-bit arithmetic without contraction, so that the codes can be reproduced
@@ -110,25 +115,46 @@ __device__ void append_page(const Cache& c, unsigned char* page, const bf16* k, 
 #pragma unroll
       for (int g = 0; g < NG; ++g) x[g] = y[g] = 0.f;
     }
-    uint32_t code[NG], step[NG], base[NG];
-    quantise<NG>(x, code, step, base);
-    uint32_t* kw = reinterpret_cast<uint32_t*>(page + L::KEYS) + slot * (HD / 8);
+    quantise<NG>(x, kcode, kstep, kbase);
+    quantise<NG>(y, vcode, vstep, vbase);
+    if (bad) {
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      uint32_t w = code[g] << (4 * (((lane & 7) >> 1) + 4 * (lane & 1)));
-      w |= __shfl_xor_sync(0xffffffffu, w, 1);
-      w |= __shfl_xor_sync(0xffffffffu, w, 2);
-      w |= __shfl_xor_sync(0xffffffffu, w, 4);
-      if ((lane & 7) == 0) kw[(lane >> 3) * NG + g] = w;
-      if (lane == 0) reinterpret_cast<uint32_t*>(page + L::KPAR)[slot * NG + g] = (bad ? 0x7fc0u : step[g]) | base[g] << 16;
+      for (int g = 0; g < NG; ++g) kstep[g] = 0x7fc0u;
     }
-    quantise<NG>(y, code, step, base);
+  }
+  // the key's word of group g, in every lane of the eight that hold its channels
+  __device__ __forceinline__ uint32_t key_word(int g) const {
+    const int lane = threadIdx.x & 31;
+    uint32_t w = kcode[g] << (4 * (((lane & 7) >> 1) + 4 * (lane & 1)));
+    w |= __shfl_xor_sync(0xffffffffu, w, 1);
+    w |= __shfl_xor_sync(0xffffffffu, w, 2);
+    return w | __shfl_xor_sync(0xffffffffu, w, 4);
+  }
+};
+
+// The CTA stores `count` new positions, first_slot .. of one page.  k and v point to the first new row of this head, `stride` elements apart;
+// pos0 is the first one's position in the sequence.  `codes` is [64][HD] bytes of shared memory.
+template <int HD>
+__device__ void append_page(const Cache& c, unsigned char* page, const bf16* k, const bf16* v, long long stride, int first_slot, int count,
+                            int pos0, unsigned char* codes) {
+  using L = Layout<HD>;
+  constexpr int NG = L::NG;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int r = warp; r < count; r += WARPS) {
+    const int slot = first_slot + r;
+    Row<HD> row;
+    row.make(c, k + r * stride, v + r * stride, pos0 + r);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      codes[r * HD + 32 * g + lane] = (unsigned char)code[g];
+      const uint32_t w = row.key_word(g);
+      if ((lane & 7) == 0) reinterpret_cast<uint32_t*>(page + L::KEYS)[slot * (HD / 8) + (lane >> 3) * NG + g] = w;
+      codes[r * HD + 32 * g + lane] = (unsigned char)row.vcode[g];
       if (lane == 0) {
-        reinterpret_cast<uint16_t*>(page + L::VSTEP)[g * 64 + value_slot(slot)] = (uint16_t)step[g];
-        reinterpret_cast<uint16_t*>(page + L::VBASE)[g * 64 + value_slot(slot)] = (uint16_t)base[g];
+        uint16_t* par = reinterpret_cast<uint16_t*>(page + L::KPAR + key_param(slot, g, NG));
+        par[0] = (uint16_t)row.kstep[g];
+        par[key_base_after(NG) / 2] = (uint16_t)row.kbase[g];
+        reinterpret_cast<uint16_t*>(page + L::VSTEP)[g * 64 + value_slot(slot)] = (uint16_t)row.vstep[g];
+        reinterpret_cast<uint16_t*>(page + L::VBASE)[g * 64 + value_slot(slot)] = (uint16_t)row.vbase[g];
       }
     }
   }
@@ -164,13 +190,19 @@ __global__ void __launch_bounds__(THREADS) append_kernel(Cache c, const bf16* __
 
 // ---- attention ----
 __device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// the same from zero
+__device__ __forceinline__ void mma16816_new(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 __device__ __forceinline__ void copy16(uint32_t smem, const void* gmem) {
@@ -181,14 +213,50 @@ __device__ __forceinline__ float ex2(float v) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
+// two f32 lanes in one instruction
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Bits that cut a pair of codes out of a word and place them behind the exponent of 128.  They are kernel parameters: as literals one
+// instruction could hold only one of the two.
+struct Bits { uint32_t mask, one28; };
+
 // codes i and i + 4 of a word as the bf16 pair (128 + code, 128 + code)
 template <int I>
-__device__ __forceinline__ uint32_t pair128(uint32_t w) { return ((w >> (4 * I)) & 0x000f000fu) | 0x43004300u; }
+__device__ __forceinline__ uint32_t pair128(uint32_t w, Bits b) { return ((w >> (4 * I)) & b.mask) | b.one28; }
 __device__ __forceinline__ __nv_bfloat162 as_pair(uint32_t v) { return *reinterpret_cast<const __nv_bfloat162*>(&v); }
 __device__ __forceinline__ uint32_t as_bits(__nv_bfloat162 v) { return *reinterpret_cast<const uint32_t*>(&v); }
 template <int I>
-__device__ __forceinline__ uint32_t value_pair(uint32_t w, uint32_t step, uint32_t base) {
-  return as_bits(__hfma2(__hsub2(as_pair(pair128<I>(w)), __float2bfloat162_rn(128.f)), as_pair(step), as_pair(base)));
+__device__ __forceinline__ uint32_t value_pair(uint32_t w, uint32_t step, uint32_t base, Bits b) {
+  return as_bits(__hfma2(__hsub2(as_pair(pair128<I>(w, b)), as_pair(b.one28)), as_pair(step), as_pair(base)));
+}
+
+// eight channels of a query's row, 0 for a query that does not exist
+__device__ __forceinline__ void load8(const bf16* src, int ch, bool ok, bool wide, float* x) {
+  if (!ok) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = 0.f;
+  } else if (wide) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(src + ch));
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __bfloat162float(src[ch + i]);
+  }
 }
 
 template <int N> struct Words { uint32_t w[N]; };
@@ -210,21 +278,26 @@ __device__ __forceinline__ Words<N> load_words(const unsigned char* p) {
   return r;
 }
 
-template <int HD> struct Ring { static constexpr int STAGES = HD == 32 ? 6 : HD == 64 ? 4 : 2; };
+// Half pages in a warp's ring.
+template <int HD> struct Ring { static constexpr int SLOTS = HD <= 64 ? 4 : 3; };
 
-template <int HD, int NQ>
-constexpr int smem_bytes() {
-  const int ring = WARPS * Ring<HD>::STAGES * Layout<HD>::BYTES, merge = NQ * 8 * (WARPS + 1) * (HD + 2) * 4, codes = PAGE * HD;
-  return ring > merge ? (ring > codes ? ring : codes) : (merge > codes ? merge : codes);
-}
+// The queries' fragments and the pieces of their sums, then per warp: the ring, and the new positions of one page (at most QT of them) until
+// the page has come: key words, value codes, steps and bases.  In the end the partial results take the place of all that.
+template <int HD, int NQ> struct Smem {
+  static constexpr int NG = Layout<HD>::NG, NP = NG == 1 ? 1 : NG / 2;
+  static constexpr int QUERIES = NQ * NG * 512, SUMS = NQ * NP * 128, FRONT = QUERIES + SUMS;
+  static constexpr int RING = Ring<HD>::SLOTS * Layout<HD>::HALF, ROW = HD / 2 + HD + 8 * NG, NEW = NQ * 8 * ROW, WARP = RING + (NEW + 127) / 128 * 128;
+  static constexpr int MERGE = NQ * 8 * (WARPS + 1) * (HD + 2) * 4;
+  static constexpr int BYTES = FRONT + WARPS * WARP > MERGE ? FRONT + WARPS * WARP : MERGE;
+};
 
 // grid: ((sequence * kv heads + kv head) * passes + pass) * splits + split; the splits of one are a cluster when it joins them
 template <int HD, int NQ>
 __global__ void __launch_bounds__(THREADS)
 attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v, int first, int rows, int splits,
-                 int passes, int append, float scale_log2, bf16* __restrict__ merged, float* __restrict__ part) {
+                 int passes, int append, float scale_log2, Bits bits, bf16* __restrict__ merged, float* __restrict__ part) {
   using L = Layout<HD>;
-  constexpr int NG = L::NG, CT = HD / 16, ST = Ring<HD>::STAGES, PW = HD + 2, QT = NQ * 8;
+  constexpr int NG = L::NG, CT = HD / 16, SLOTS = Ring<HD>::SLOTS, PW = HD + 2, QT = NQ * 8;
   extern __shared__ __align__(128) unsigned char sm[];
   const int block = blockIdx.x / splits, split = blockIdx.x - block * splits, head_at = block / passes, pass = block - head_at * passes;
   const int sj = head_at / c.Hkv, kvh = head_at - sj * c.Hkv, seq = first + sj;
@@ -247,54 +320,120 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
   const int last_row = (min(q0 + QT, nq) - 1) / group, seen_pages = (len + last_row) / PAGE + 1;
   const int pend = min(pg1, seen_pages);
   unsigned char* head = page_at(c, seq, kvh, 0);
+  // The warp's half pages, last page first (the new positions are in the last ones): unit 2 j is the keys and 2 j + 1 the values of page
+  // pg - j * WARPS.
+  using M = Smem<HD, NQ>;
+  unsigned char* ring = sm + M::FRONT + warp * M::WARP;
+  unsigned char* fresh = ring + M::RING;
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
+  int pg = pend - 1 - warp;
+  int issue_pg = pg, issue_half = 0, issue_slot = 0, slot = 0;
+  auto issue = [&] {
+    if (issue_pg >= pg0) {
+      const unsigned char* src = head + (long long)issue_pg * L::BYTES + issue_half + lane * 16;
+      const uint32_t dst = ring_at + issue_slot * L::HALF;
+#pragma unroll
+      for (int i = 0; i + 512 <= L::HALF; i += 512) copy16(dst + i, src + i);
+      if (L::HALF % 512 != 0 && lane * 16 < L::HALF % 512) copy16(dst + L::HALF / 512 * 512, src + L::HALF / 512 * 512);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    issue_slot = issue_slot + 1 == SLOTS ? 0 : issue_slot + 1;
+    if (issue_half) issue_pg -= WARPS;
+    issue_half = issue_half ? 0 : L::HALF;
+  };
+  auto next_half = [&]() -> unsigned char* {
+    asm volatile("cp.async.wait_group %0;" ::"n"(SLOTS - 2) : "memory");
+    __syncwarp();                                     // every lane's copies of the half have landed, and the one before is used up
+    issue();
+    unsigned char* p = ring + slot * L::HALF;
+    slot = slot + 1 == SLOTS ? 0 : slot + 1;
+    return p;
+  };
+#pragma unroll
+  for (int i = 0; i < SLOTS - 1; ++i) issue();
 
-  if (append) {
-    const long long W = (long long)c.Hkv * HD;
-    for (int pg = max(pg0, len / PAGE); pg < pg1; ++pg) {
-      const int p0 = max(len, pg * PAGE), p1 = min(total, (pg + 1) * PAGE);
-      const long long at = ((long long)sj * rows + p0 - len) * W + kvh * HD;
-      append_page<HD>(c, head + (long long)pg * L::BYTES, k + at, v + at, W, p0 - pg * PAGE, p1 - p0, p0, sm);
-      __threadfence();
-      __syncthreads();
+  // ---- this warp's new positions, if its first page has any: quantised while the page and the queries are under way.  A row in `fresh` is
+  // the key's words in page order, the value's codes, then step | base of the key's and of the value's groups. ----
+  const int new0 = max(len, pg * PAGE), news = append && pg >= pg0 ? max(0, min(total, (pg + 1) * PAGE) - new0) : 0;
+  for (int r = 0; r < news; ++r) {
+    const long long at = (((long long)sj * rows + new0 + r - len) * c.Hkv + kvh) * HD;
+    unsigned char* f = fresh + r * M::ROW;
+    Row<HD> row;
+    row.make(c, k + at, v + at, new0 + r);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const uint32_t w = row.key_word(g);
+      if ((lane & 7) == 0) reinterpret_cast<uint32_t*>(f)[(lane >> 3) * NG + g] = w;
+      f[HD / 2 + 32 * g + lane] = (unsigned char)row.vcode[g];
+      if (lane < 2) reinterpret_cast<uint32_t*>(f + HD / 2 + HD)[lane * NG + g] = lane ? row.vstep[g] | row.vbase[g] << 16 : row.kstep[g] | row.kbase[g] << 16;
     }
   }
 
-  // ---- queries: rotated, scaled to base 2, rounded to bf16 once; lane (gid, tig) holds query gid's channels 32 g + 8 tig .. + 7 ----
-  uint32_t qf[NQ][NG][4];
-  float qs[NQ][NG][2];                                // sum over the group of queries 2 tig and 2 tig + 1
-  int lim[NQ][2];                                     // positions that they see
+  // ---- queries: rotated, scaled to base 2, rounded to bf16 once; eight channels of one query a thread and turn ----
+  {
+    const bool wide = (reinterpret_cast<uintptr_t>(q) & 15) == 0;     // a head's row is a multiple of 16 bytes
+    uint4* frag = reinterpret_cast<uint4*>(sm);
+    uint16_t* sums = reinterpret_cast<uint16_t*>(sm + M::QUERIES);
 #pragma unroll
-  for (int nt = 0; nt < NQ; ++nt) {
-    const int qi = q0 + nt * 8 + gid, ok = qi < nq, r = ok ? qi / group : 0, h = ok ? qi - r * group : 0;
-    const bf16* src = q + (((long long)sj * rows + r) * c.H + kvh * group + h) * HD;
-    const float* ct = c.cos_t + (long long)(len + r) * (HD / 2);
-    const float* st = c.sin_t + (long long)(len + r) * (HD / 2);
+    for (int i0 = 0; i0 < QT * HD / 8; i0 += THREADS) {
+      const int i = i0 + THREADS - 32 - (int)(threadIdx.x & ~31u) + lane, at = i / (HD / 8), ch = 8 * (i % (HD / 8)), g = ch / 32, t = (ch / 8) & 3;
+      if (QT * HD / 8 < THREADS && i >= QT * HD / 8) break;           // whole warps; the first ones have new positions to see to
+      const int qi = q0 + at, ok = qi < nq, r = ok ? qi / group : 0, h = ok ? qi - r * group : 0;
+      const bf16* src = q + (((long long)sj * rows + r) * c.H + kvh * group + h) * HD;
+      const int low = ch < HD / 2, f = low ? ch : ch - HD / 2;
+      float x[8], sum = 0.f;
+      load8(src, ch, ok, wide, x);
+      if (c.rope && ok) {
+        const float* ct = c.cos_t + (long long)(len + r) * (HD / 2) + f;
+        const float* st = c.sin_t + (long long)(len + r) * (HD / 2) + f;
+        float other[8], co[8], si[8];
+        load8(src, low ? ch + HD / 2 : f, ok, wide, other);
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const int ch = 32 * g + 8 * tig;
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int at = ch + 2 * i + e;
-          float a = ok ? __bfloat162float(src[at]) : 0.f;
-          if (ok && c.rope) {
-            const int low = at < HD / 2, f = low ? at : at - HD / 2;
-            const float other = __bfloat162float(src[low ? at + HD / 2 : f]);
-            a = low ? a * ct[f] - other * st[f] : a * ct[f] + other * st[f];
-          }
-          x[e] = a * scale_log2;
+        for (int j = 0; j < 8; j += 4) {
+          *reinterpret_cast<float4*>(co + j) = __ldg(reinterpret_cast<const float4*>(ct + j));
+          *reinterpret_cast<float4*>(si + j) = __ldg(reinterpret_cast<const float4*>(st + j));
         }
-        const __nv_bfloat162 p = __floats2bfloat162_rn(x[0], x[1]);
-        qf[nt][g][i] = as_bits(p);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = low ? x[j] * co[j] - other[j] * si[j] : x[j] * co[j] + other[j] * si[j];
+      }
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const __nv_bfloat162 p = __floats2bfloat162_rn(x[2 * j] * scale_log2, x[2 * j + 1] * scale_log2);
+        w[j] = as_bits(p);
         sum += __low2float(p) + __high2float(p);
       }
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      const int nt = at >> 3, to = (at & 7) * 4 + t;                  // the lane that multiplies these channels
+      frag[(nt * NG + g) * 32 + to] = make_uint4(w[0], w[1], w[2], w[3]);
+      // the sum as three bf16 numbers, one for each of the lanes t = 0, 1, 2
+      const bf16 s0 = __float2bfloat16_rn(sum), s1 = __float2bfloat16_rn(sum - __bfloat162float(s0));
+      const bf16 s2 = __float2bfloat16_rn(sum - __bfloat162float(s0) - __bfloat162float(s1));
+      const bf16 piece = t == 0 ? s0 : t == 1 ? s1 : t == 2 ? s2 : __float2bfloat16_rn(0.f);
+      uint16_t* d = sums + ((nt * M::NP + (NG == 1 ? 0 : g >> 1)) * 32 + to) * 2;
+      if (NG == 1) {
+        d[0] = __bfloat16_as_ushort(__hmul(piece, __float2bfloat16_rn(-128.f)));
+        d[1] = __bfloat16_as_ushort(piece);
+      } else {
+        d[g & 1] = __bfloat16_as_ushort(piece);
+      }
+    }
+  }
+  __syncthreads();
+  uint32_t qf[NQ][NG][4], qb[NQ][M::NP], qst[NQ][M::NP];   // fragments; sums against the bases; sums times -128 against the steps
+  int lim[NQ][2];                                     // positions that queries 2 tig and 2 tig + 1 see
 #pragma unroll
-      for (int e = 0; e < 2; ++e) qs[nt][g][e] = __shfl_sync(0xffffffffu, sum, (2 * tig + e) * 4);
+  for (int nt = 0; nt < NQ; ++nt) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const uint4 w = reinterpret_cast<const uint4*>(sm)[(nt * NG + g) * 32 + lane];
+      qf[nt][g][0] = w.x; qf[nt][g][1] = w.y; qf[nt][g][2] = w.z; qf[nt][g][3] = w.w;
+    }
+#pragma unroll
+    for (int j = 0; j < M::NP; ++j) {
+      qb[nt][j] = reinterpret_cast<const uint32_t*>(sm + M::QUERIES)[(nt * M::NP + j) * 32 + lane];
+      qst[nt][j] = NG == 1 ? 0u : as_bits(__hmul2(as_pair(qb[nt][j]), __float2bfloat162_rn(-128.f)));
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -304,35 +443,39 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
   }
   const int all_see = len + q0 / group + 1;           // positions below this are seen by every query of the pass
 
-  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(sm) + warp * (ST * L::BYTES);
-  const unsigned char* ring_ptr = sm + warp * (ST * L::BYTES);
-  float m[NQ][2], l[NQ][2], o[NQ][CT][4];
+  // A weight is 2^(score - ref): ref is the maximum when it was last looked up and stays until a score passes it
+  // by RISE; until then neither the sums nor the products have to be scaled.
+  float ref[NQ][2], l[NQ][2], o[NQ][CT][4];
+
 #pragma unroll
   for (int nt = 0; nt < NQ; ++nt) {
-    m[nt][0] = m[nt][1] = -INFINITY;
+    ref[nt][0] = ref[nt][1] = -INFINITY;
     l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) o[nt][ct][0] = o[nt][ct][1] = o[nt][ct][2] = o[nt][ct][3] = 0.f;
   }
-  auto issue = [&](int pg, int stage) {
-    if (pg < pend) {
-      const unsigned char* src = head + (long long)pg * L::BYTES + lane * 16;
-      const uint32_t dst = ring + stage * L::BYTES + lane * 16;
-#pragma unroll
-      for (int i = 0; i < L::BYTES; i += 512) copy16(dst + i, src + i);
+  for (; pg >= pg0; pg -= WARPS) {
+    unsigned char* page = next_half();
+    const bool has_new = news > 0 && new0 / PAGE == pg;
+    unsigned char* out = head + (long long)pg * L::BYTES;
+    if (has_new) {                                    // new keys into the page and into the cache
+      for (int r = 0; r < news; ++r) {
+        const unsigned char* f = fresh + r * M::ROW;
+        const int at = new0 + r - pg * PAGE;
+        for (int i = lane; i < HD / 8; i += 32) {
+          const uint32_t w = reinterpret_cast<const uint32_t*>(f)[i];
+          reinterpret_cast<uint32_t*>(page + L::KEYS)[at * (HD / 8) + i] = w;
+          reinterpret_cast<uint32_t*>(out + L::KEYS)[at * (HD / 8) + i] = w;
+        }
+        if (lane < 2 * NG) {
+          const int g = lane >> 1, par = L::KPAR + key_param(at, g, NG) + (lane & 1) * key_base_after(NG);
+          const uint16_t b = reinterpret_cast<const uint16_t*>(f + HD / 2 + HD)[lane];
+          *reinterpret_cast<uint16_t*>(page + par) = b;
+          *reinterpret_cast<uint16_t*>(out + par) = b;
+        }
+      }
+      __syncwarp();
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-  const int my0 = pg0 + warp;
-#pragma unroll
-  for (int i = 0; i < ST - 1; ++i) issue(my0 + i * WARPS, i);
-  int stage = 0;
-  for (int pg = my0; pg < pend; pg += WARPS) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
-    __syncwarp();                                     // every lane's copies of the page have landed, and the stage before is free
-    issue(pg + (ST - 1) * WARPS, (stage + ST - 1) % ST);
-    const unsigned char* page = ring_ptr + stage * L::BYTES;
-    stage = (stage + 1) % ST;
 
     // ---- scores ----
     float s[NQ][4][4];
@@ -343,23 +486,29 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
       const Words<NG> plo = load_words<NG>(page + L::KPAR + (16 * mt + gid) * NG * 4);
       const Words<NG> phi = load_words<NG>(page + L::KPAR + (16 * mt + gid + 8) * NG * 4);
 #pragma unroll
-      for (int nt = 0; nt < NQ; ++nt) s[nt][mt][0] = s[nt][mt][1] = s[nt][mt][2] = s[nt][mt][3] = 0.f;
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const uint32_t a0 = pair128<0>(lo.w[g]), a1 = pair128<0>(hi.w[g]), a2 = pair128<1>(lo.w[g]), a3 = pair128<1>(hi.w[g]);
-        const uint32_t b0 = pair128<2>(lo.w[g]), b1 = pair128<2>(hi.w[g]), b2 = pair128<3>(lo.w[g]), b3 = pair128<3>(hi.w[g]);
-        const float st0 = __uint_as_float(plo.w[g] << 16), ba0 = __uint_as_float(plo.w[g] & 0xffff0000u);
-        const float st1 = __uint_as_float(phi.w[g] << 16), ba1 = __uint_as_float(phi.w[g] & 0xffff0000u);
+      for (int j = 0; j < M::NP; ++j)
 #pragma unroll
         for (int nt = 0; nt < NQ; ++nt) {
-          const float n0 = -128.f * qs[nt][g][0], n1 = -128.f * qs[nt][g][1];
-          float acc[4] = {n0, n1, n0, n1};
-          mma16816(acc, a0, a1, a2, a3, qf[nt][g][0], qf[nt][g][1]);
+          const uint32_t a0 = NG == 1 ? plo.w[0] : plo.w[2 * j + 1], a1 = NG == 1 ? phi.w[0] : phi.w[2 * j + 1];
+          const uint32_t a2 = NG == 1 ? 0u : plo.w[2 * j], a3 = NG == 1 ? 0u : phi.w[2 * j];
+          if (j == 0) mma16816_new(s[nt][mt], a0, a1, a2, a3, qb[nt][j], qst[nt][j]);
+          else mma16816(s[nt][mt], a0, a1, a2, a3, qb[nt][j], qst[nt][j]);
+        }
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const uint32_t a0 = pair128<0>(lo.w[g], bits), a1 = pair128<0>(hi.w[g], bits), a2 = pair128<1>(lo.w[g], bits), a3 = pair128<1>(hi.w[g], bits);
+        const uint32_t b0 = pair128<2>(lo.w[g], bits), b1 = pair128<2>(hi.w[g], bits), b2 = pair128<3>(lo.w[g], bits), b3 = pair128<3>(hi.w[g], bits);
+        const uint32_t w0 = plo.w[NG == 1 ? 0 : g & ~1], w1 = phi.w[NG == 1 ? 0 : g & ~1];
+        const float st0 = __uint_as_float(g & 1 ? w0 & 0xffff0000u : w0 << 16), st1 = __uint_as_float(g & 1 ? w1 & 0xffff0000u : w1 << 16);
+#pragma unroll
+        for (int nt = 0; nt < NQ; ++nt) {
+          float acc[4];
+          mma16816_new(acc, a0, a1, a2, a3, qf[nt][g][0], qf[nt][g][1]);
           mma16816(acc, b0, b1, b2, b3, qf[nt][g][2], qf[nt][g][3]);
-          s[nt][mt][0] = fmaf(st0, acc[0], fmaf(ba0, qs[nt][g][0], s[nt][mt][0]));
-          s[nt][mt][1] = fmaf(st0, acc[1], fmaf(ba0, qs[nt][g][1], s[nt][mt][1]));
-          s[nt][mt][2] = fmaf(st1, acc[2], fmaf(ba1, qs[nt][g][0], s[nt][mt][2]));
-          s[nt][mt][3] = fmaf(st1, acc[3], fmaf(ba1, qs[nt][g][1], s[nt][mt][3]));
+          s[nt][mt][0] = fmaf(st0, acc[0], s[nt][mt][0]);
+          s[nt][mt][1] = fmaf(st0, acc[1], s[nt][mt][1]);
+          s[nt][mt][2] = fmaf(st1, acc[2], s[nt][mt][2]);
+          s[nt][mt][3] = fmaf(st1, acc[3], s[nt][mt][3]);
         }
       }
     }
@@ -374,41 +523,73 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
             if (pg * PAGE + 16 * mt + gid + 8 * (e >> 1) >= lim[nt][e & 1]) s[nt][mt][e] = -INFINITY;
     }
     uint32_t p[NQ][4][2];
+    bool rise = false;
+    float mx[NQ][2];
 #pragma unroll
-    for (int nt = 0; nt < NQ; ++nt) {
-      float corr[2], ref[2];
+    for (int nt = 0; nt < NQ; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float mx = fmaxf(s[nt][0][e], s[nt][0][e + 2]);
+        float a = fmaxf(s[nt][0][e], s[nt][0][e + 2]);
 #pragma unroll
-        for (int mt = 1; mt < 4; ++mt) mx = fmaxf(mx, fmaxf(s[nt][mt][e], s[nt][mt][e + 2]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        const float now = fmaxf(m[nt][e], mx);
-        ref[e] = now > -INFINITY ? now : 0.f;         // nothing seen yet: every weight is 0
-        corr[e] = ex2(m[nt][e] - ref[e]);
-        m[nt][e] = now;
-        l[nt][e] *= corr[e];
+        for (int mt = 1; mt < 4; ++mt) a = fmaxf(a, fmaxf(s[nt][mt][e], s[nt][mt][e + 2]));
+        mx[nt][e] = a;
+        rise |= a > ref[nt][e] + RISE;
       }
+    if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt) {
-        float w[4];
+      for (int nt = 0; nt < NQ; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          w[e] = ex2(s[nt][mt][e] - ref[e & 1]);
-          l[nt][e & 1] += w[e];
+        for (int e = 0; e < 2; ++e) {
+          float a = mx[nt][e];
+          a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 4));
+          a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 8));
+          a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 16));
+          a = fmaxf(a, ref[nt][e]);
+          const float corr = a > -INFINITY ? ex2(ref[nt][e] - a) : 1.f;
+          ref[nt][e] = a;
+          l[nt][e] *= corr;
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) { o[nt][ct][e] *= corr; o[nt][ct][e + 2] *= corr; }
         }
-        p[nt][mt][0] = transpose8x8(as_bits(__floats2bfloat162_rn(w[0], w[1])));
-        p[nt][mt][1] = transpose8x8(as_bits(__floats2bfloat162_rn(w[2], w[3])));
-      }
+    }
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        o[nt][ct][0] *= corr[0]; o[nt][ct][1] *= corr[1];
-        o[nt][ct][2] *= corr[0]; o[nt][ct][3] *= corr[1];
-      }
+    for (int nt = 0; nt < NQ; ++nt) {
+      // a query that has seen nothing yet has scores of -inf only: weights of 0 against any finite number
+      const uint64_t minus = pack2(ref[nt][0] > -INFINITY ? -ref[nt][0] : 0.f, ref[nt][1] > -INFINITY ? -ref[nt][1] : 0.f);
+      uint64_t sum = pack2(l[nt][0], l[nt][1]);
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float y0, y1;
+          unpack2(add2(pack2(s[nt][mt][2 * h], s[nt][mt][2 * h + 1]), minus), y0, y1);
+          const float w0 = ex2(y0), w1 = ex2(y1);
+          sum = add2(sum, pack2(w0, w1));
+          p[nt][mt][h] = transpose8x8(as_bits(__floats2bfloat162_rn(w0, w1)));
+        }
+      unpack2(sum, l[nt][0], l[nt][1]);
     }
     // ---- values ----
+    page = next_half() - L::HALF;                     // so that the page's offsets hold
+    if (has_new) {                                    // ... and new values
+      for (int r = 0; r < news; ++r) {
+        const unsigned char* f = fresh + r * M::ROW + HD / 2;
+        const int at = new0 + r - pg * PAGE, w = value_word(at), n = 4 * value_nibble(at);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          uint32_t* word = reinterpret_cast<uint32_t*>(page + L::VALUES) + (32 * g + lane) * 8 + w;
+          *word = (*word & ~(15u << n)) | (uint32_t)f[32 * g + lane] << n;
+          reinterpret_cast<uint32_t*>(out + L::VALUES)[(32 * g + lane) * 8 + w] = *word;
+        }
+        if (lane < 2 * NG) {
+          const int off = (lane & 1 ? L::VBASE : L::VSTEP) + ((lane >> 1) * 64 + value_slot(at)) * 2;
+          const uint16_t b = reinterpret_cast<const uint16_t*>(f + HD + 4 * NG)[lane];
+          *reinterpret_cast<uint16_t*>(page + off) = b;
+          *reinterpret_cast<uint16_t*>(out + off) = b;
+        }
+      }
+      __syncwarp();
+    }
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       const Words<8> step = load_words<8>(page + L::VSTEP + g * 128 + tig * 32), base = load_words<8>(page + L::VBASE + g * 128 + tig * 32);
@@ -420,10 +601,10 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
           const int j = 4 * w;
-          const uint32_t a0 = value_pair<0>(lo.w[w], step.w[j], base.w[j]), a1 = value_pair<0>(hi.w[w], step.w[j], base.w[j]);
-          const uint32_t a2 = value_pair<1>(lo.w[w], step.w[j + 1], base.w[j + 1]), a3 = value_pair<1>(hi.w[w], step.w[j + 1], base.w[j + 1]);
-          const uint32_t b0 = value_pair<2>(lo.w[w], step.w[j + 2], base.w[j + 2]), b1 = value_pair<2>(hi.w[w], step.w[j + 2], base.w[j + 2]);
-          const uint32_t b2 = value_pair<3>(lo.w[w], step.w[j + 3], base.w[j + 3]), b3 = value_pair<3>(hi.w[w], step.w[j + 3], base.w[j + 3]);
+          const uint32_t a0 = value_pair<0>(lo.w[w], step.w[j], base.w[j], bits), a1 = value_pair<0>(hi.w[w], step.w[j], base.w[j], bits);
+          const uint32_t a2 = value_pair<1>(lo.w[w], step.w[j + 1], base.w[j + 1], bits), a3 = value_pair<1>(hi.w[w], step.w[j + 1], base.w[j + 1], bits);
+          const uint32_t b0 = value_pair<2>(lo.w[w], step.w[j + 2], base.w[j + 2], bits), b1 = value_pair<2>(hi.w[w], step.w[j + 2], base.w[j + 2], bits);
+          const uint32_t b2 = value_pair<3>(lo.w[w], step.w[j + 3], base.w[j + 3], bits), b3 = value_pair<3>(hi.w[w], step.w[j + 3], base.w[j + 3], bits);
 #pragma unroll
           for (int nt = 0; nt < NQ; ++nt) {
             mma16816(o[nt][ct], a0, a1, a2, a3, p[nt][2 * w][0], p[nt][2 * w][1]);
@@ -432,7 +613,6 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
         }
       }
     }
-    __syncwarp();
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
@@ -459,7 +639,7 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float* d = mb + ((nt * 8 + 2 * tig + e) * WARPS + warp) * PW + HD;
-        d[0] = m[nt][e];
+        d[0] = ref[nt][e];
         d[1] = l[nt][e];
       }
     }
@@ -531,13 +711,13 @@ __global__ void values_kernel(Cache c, int first, int from, int count, float* __
     if (pos >= 0 && pos < len) {
       const int kvh = i / c.HD, ch = i - kvh * c.HD, g = ch / GROUP, slot = pos % PAGE;
       const unsigned char* page = page_at(c, seq, kvh, pos / PAGE);
-      const uint32_t par = reinterpret_cast<const uint32_t*>(page + 64 * c.HD)[slot * NG + g];
+      const unsigned char* par = page + 32 * c.HD + key_param(slot, g, NG);
       const uint32_t kw = reinterpret_cast<const uint32_t*>(page)[slot * (c.HD / 8) + ((ch & 31) >> 3) * NG + g];
-      const uint32_t vw = reinterpret_cast<const uint32_t*>(page + 32 * c.HD)[ch * 8 + value_word(slot)];
+      const uint32_t vw = reinterpret_cast<const uint32_t*>(page + 40 * c.HD)[ch * 8 + value_word(slot)];
       const uint16_t* vstep = reinterpret_cast<const uint16_t*>(page + 72 * c.HD) + g * 64 + value_slot(slot);
       const float kc = (float)((kw >> (4 * (((ch & 7) >> 1) + 4 * (ch & 1)))) & 15u), vc = (float)((vw >> (4 * value_nibble(slot))) & 15u);
-      const float ks = __uint_as_float(par << 16);
-      kv = fmaf(kc, ks, __uint_as_float(par & 0xffff0000u));
+      const float ks = __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(par) << 16);
+      kv = fmaf(kc, ks, __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(par + key_base_after(NG)) << 16));
       vv = fmaf(vc, __uint_as_float((uint32_t)vstep[0] << 16), __uint_as_float((uint32_t)vstep[NG * 64] << 16));
       if (ks != ks) kv = vv = ks;
     }
@@ -549,7 +729,7 @@ __global__ void values_kernel(Cache c, int first, int from, int count, float* __
 template <int HD, int NQ>
 cudaError_t go(const Cache& c, const bf16* q, const bf16* k, const bf16* v, int first, int n_seq, int rows, int splits, bool append, float scale_log2,
                bf16* merged, float* part, cudaStream_t st) {
-  constexpr int smem = smem_bytes<HD, NQ>();
+  constexpr int smem = Smem<HD, NQ>::BYTES;
   auto kernel = attention_kernel<HD, NQ>;
   static std::atomic<unsigned long long> raised{0};   // devices on which the kernel's shared-memory limit has been raised
   int device = 0;
@@ -573,7 +753,7 @@ cudaError_t go(const Cache& c, const bf16* q, const bf16* k, const bf16* v, int 
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   count_launch();
-  return cudaLaunchKernelEx(&cfg, kernel, c, q, k, v, first, rows, splits, passes, append ? 1 : 0, scale_log2, merged, part);
+  return cudaLaunchKernelEx(&cfg, kernel, c, q, k, v, first, rows, splits, passes, append ? 1 : 0, scale_log2, Bits{0x000f000fu, 0x43004300u}, merged, part);
 }
 
 }  // namespace
