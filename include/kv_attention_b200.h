@@ -20,7 +20,7 @@
  *     what the cache stands for = code * step + base
  * in f32 arithmetic, rounding to even, rotation included (two products and their sum, not contracted; the angles are computed in 64 bits).
  * A step's own new positions are read back from the cache like all others.  If a position's key or value of a kv head holds a NaN, an
- * infinity or a number above 2^126 in magnitude, its key and value stand for NaN: what attends to it is NaN, what does not is untouched.
+ * infinity or a number above 2^40 in magnitude, its key and value stand for NaN: what attends to it is NaN, what does not is untouched.
  * Neither call below allocates on such a cache, so every step can be captured; q is left alone.
  */
 #ifndef KV_ATTENTION_B200_H

@@ -55,7 +55,7 @@ class Q4CacheOracle:
             k = self._rotate(np.asarray(k, np.float32).reshape(n, self.Hkv, self.hd), len(self), np.float32)
         v = np.asarray(v, np.float32).reshape(n, self.Hkv, self.hd)
         with np.errstate(invalid="ignore"):
-            bad = ~(np.abs(k) <= 2.0 ** 126).all(-1, keepdims=True) | ~(np.abs(v) <= 2.0 ** 126).all(-1, keepdims=True)
+            bad = ~(np.abs(k) <= 2.0 ** 40).all(-1, keepdims=True) | ~(np.abs(v) <= 2.0 ** 40).all(-1, keepdims=True)
         kq, _ = quantise(np.where(bad, 0, k).astype(np.float32))
         vq, _ = quantise(np.where(bad, 0, v).astype(np.float32))
         self.keys = np.concatenate([self.keys, np.where(bad, np.float32(np.nan), kq)])

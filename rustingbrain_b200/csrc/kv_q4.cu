@@ -7,19 +7,21 @@
 // The 64 positions of a page lie together, as the tensor cores want them: one warp takes a page, S^T = K Q^T has the positions as
 // the 16 rows and the queries as the 8 columns of mma.sync m16n8k16, O^T = V^T P^T has the channels as rows and the positions as the
 // reduction.  So the few queries that share a kv head fill the small side of the product, and both K and V are the A operand:
-// a lane's 32-bit word holds 8 codes that it needs itself, keys as 8 channels of one position, values as 8 positions of one channel,
-// so that a word costs seven instructions to become four pairs of bf16 numbers 128 + code.
-//   keys:   S = sum over groups of step * sum_c (128 + code) q + (base - 128 step) * sum_c q.  The first product takes its step in f32; the
-//           second part, base and step against the queries' sums in three bf16 pieces, is one more small product on the tensor cores.
-//           Nothing of the key is rounded.
-//   values: step and base belong to the position, which is what the product sums over, so they go on before it: two packed
-//           bf16 instructions, one rounding of the value to bf16 (2^-9 of it; P is rounded alike).
+// a lane's 32-bit word holds 8 codes that it needs itself, keys as 8 channels of one position, values as 8 positions of one channel.
+// Bits 0 .. 7 of a bf16 are a number linear in them, bits * 2^-133: below 128 it is subnormal, and the next binade goes on in the same steps.  So
+// a code needs no conversion, only to be cut out, at weight 1 (bits 0 .. 3) or 16 (bits 4 .. 7): five instructions a word.  The other
+// factor makes up for the 2^-133, and for the 16 at the places that have it.
+//   keys:   S = sum over groups of step * sum_c code q + base * sum_c q.  The first product takes its step in f32; the second part, bases
+//           against the queries' sums in three bf16 pieces, is one more small product on the tensor cores.  Nothing of the key is rounded.
+//   values: step and base belong to the position, which is what the product sums over, so they go on before it: one packed bf16
+//           instruction, one rounding of the value to bf16 (2^-9 of it; P is rounded alike).
+// What bounds it is the issue of those instructions: 148 SMs would have to do a page of 64 x 64 channels every 215 cycles to keep up with HBM.
 //
 // Page layout, HD = head_dim, NG = HD / 32:
 //   keys    [64 positions][4 t][NG g] words: channels 32 g + 8 t + 2 i + e at nibble i + 4 e
 //   key parameters [64 positions][NG / 2][step of two groups, base of two groups] (bf16 pairs); NG = 1: step and base in one word
 //   values  [HD channels][4 t][2 w] words: positions 16 (2 w + i / 2) + 8 (i % 2) + 2 t + e at nibble i + 4 e
-//   value step, value base  [NG][64] bf16 each, position p at value_slot(p)
+//   value step * 2^STEP_UP (another / 16 where the codes weigh 16), value base  [NG][64] bf16 each, position p at value_slot(p)
 // A warp streams half pages (keys, then values) through its own ring in shared memory.  The warp whose page takes a step's new positions
 // quantises them into its copy of the page and into the cache: nobody else reads them, so nobody has to wait.
 
@@ -38,7 +40,16 @@ namespace {
 
 constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr float RISE = 8.f;                     // weights stay below 2^8 against the reference
-constexpr float HUGE_VALUE = 8.507059e37f;      // 2^126: a larger number counts as an infinity, so that high - low stays finite
+constexpr float HUGE_VALUE = 1.099511627776e12f; // 2^40: a larger number counts as an infinity (a step times 2^STEP_UP is a bf16 number)
+constexpr int RAW = 133;                        // bits 0 .. 7 of a bf16 are worth bits * 2^-RAW
+constexpr int Q_UP = 80, STEP_UP = 90;          // queries times 2^Q_UP against raw key codes; value steps
+__host__ __device__ constexpr float pow2(int e) {
+  float v = 1.f;
+  for (int i = 0; i < (e < 0 ? -e : e); ++i) v *= e < 0 ? 0.5f : 2.f;
+  return v;
+}
+// whether a value's code weighs 16 in its word
+__host__ __device__ inline int value_heavy(int p) { return (p >> 3) & 1; }
 
 template <int HD> struct Layout {
   static constexpr int NG = HD / GROUP, KEYS = 0, KPAR = 32 * HD, HALF = 40 * HD, VALUES = HALF, VSTEP = 72 * HD, VBASE = VSTEP + NG * 128, BYTES = 80 * HD;
@@ -62,12 +73,9 @@ template <int NG>
 __device__ __forceinline__ void quantise(const float* x, uint32_t* code, uint32_t* step, uint32_t* base) {
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
-    float lo = x[g], hi = x[g];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
+    float lo, hi;                                     // over the warp; the values are finite
+    asm volatile("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(lo) : "f"(x[g]));
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(hi) : "f"(x[g]));
     const bf16 s = __float2bfloat16_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f)), b = __float2bfloat16_rn(lo);
     const float sf = __bfloat162float(s), bf = __bfloat162float(b);
     code[g] = sf > 0.f ? (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[g], bf), sf)), 0.f), 15.f) : 0u;
@@ -117,6 +125,9 @@ struct Row {
     }
     quantise<NG>(x, kcode, kstep, kbase);
     quantise<NG>(y, vcode, vstep, vbase);
+#pragma unroll
+    for (int g = 0; g < NG; ++g)                      // exact: a power of two
+      vstep[g] = __bfloat16_as_ushort(__float2bfloat16_rn(__uint_as_float(vstep[g] << 16) * pow2(value_heavy(pos) ? STEP_UP - 4 : STEP_UP)));
     if (bad) {
 #pragma unroll
       for (int g = 0; g < NG; ++g) kstep[g] = 0x7fc0u;
@@ -200,6 +211,10 @@ __device__ __forceinline__ void mma16816_new(float* d, uint32_t a0, uint32_t a1,
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
+__device__ __forceinline__ void mma1688_new(float* d, uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%7, %7, %7, %7};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(b0), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -225,19 +240,21 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
 
-// Bits that cut a pair of codes out of a word and place them behind the exponent of 128.  They are kernel parameters: as literals one
-// instruction could hold only one of the two.
-struct Bits { uint32_t mask, one28; };
-
-// codes i and i + 4 of a word as the bf16 pair (128 + code, 128 + code)
+// codes i and i + 4 of a word as raw bf16 numbers, of weight 16 where i is odd
 template <int I>
-__device__ __forceinline__ uint32_t pair128(uint32_t w, Bits b) { return ((w >> (4 * I)) & b.mask) | b.one28; }
+__device__ __forceinline__ uint32_t raw_pair(uint32_t w) { return (I < 2 ? w : w >> 8) & (I & 1 ? 0x00f000f0u : 0x000f000fu); }
 __device__ __forceinline__ __nv_bfloat162 as_pair(uint32_t v) { return *reinterpret_cast<const __nv_bfloat162*>(&v); }
 __device__ __forceinline__ uint32_t as_bits(__nv_bfloat162 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+// ... and as values times 2^(STEP_UP - RAW); base has that factor already
 template <int I>
-__device__ __forceinline__ uint32_t value_pair(uint32_t w, uint32_t step, uint32_t base, Bits b) {
-  return as_bits(__hfma2(__hsub2(as_pair(pair128<I>(w, b)), as_pair(b.one28)), as_pair(step), as_pair(base)));
+__device__ __forceinline__ uint32_t value_pair(uint32_t w, uint32_t step, uint32_t base) {
+  return as_bits(__hfma2(as_pair(raw_pair<I>(w)), as_pair(step), as_pair(base)));
 }
 
 // eight channels of a query's row, 0 for a query that does not exist
@@ -295,7 +312,7 @@ template <int HD, int NQ> struct Smem {
 template <int HD, int NQ>
 __global__ void __launch_bounds__(THREADS)
 attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v, int first, int rows, int splits,
-                 int passes, int append, float scale_log2, Bits bits, bf16* __restrict__ merged, float* __restrict__ part) {
+                 int passes, int append, float scale_log2, bf16* __restrict__ merged, float* __restrict__ part) {
   using L = Layout<HD>;
   constexpr int NG = L::NG, CT = HD / 16, SLOTS = Ring<HD>::SLOTS, PW = HD + 2, QT = NQ * 8;
   extern __shared__ __align__(128) unsigned char sm[];
@@ -400,11 +417,12 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const __nv_bfloat162 p = __floats2bfloat162_rn(x[2 * j] * scale_log2, x[2 * j + 1] * scale_log2);
-        w[j] = as_bits(p);
+        w[j] = as_bits(__hmul2(p, __float2bfloat162_rn(pow2(j & 1 ? Q_UP - 4 : Q_UP))));
         sum += __low2float(p) + __high2float(p);
       }
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      sum *= pow2(Q_UP - RAW);
       const int nt = at >> 3, to = (at & 7) * 4 + t;                  // the lane that multiplies these channels
       frag[(nt * NG + g) * 32 + to] = make_uint4(w[0], w[1], w[2], w[3]);
       // the sum as three bf16 numbers, one for each of the lanes t = 0, 1, 2
@@ -413,7 +431,7 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
       const bf16 piece = t == 0 ? s0 : t == 1 ? s1 : t == 2 ? s2 : __float2bfloat16_rn(0.f);
       uint16_t* d = sums + ((nt * M::NP + (NG == 1 ? 0 : g >> 1)) * 32 + to) * 2;
       if (NG == 1) {
-        d[0] = __bfloat16_as_ushort(__hmul(piece, __float2bfloat16_rn(-128.f)));
+        d[0] = 0;                                                     // against the step that shares the word with the base
         d[1] = __bfloat16_as_ushort(piece);
       } else {
         d[g & 1] = __bfloat16_as_ushort(piece);
@@ -421,7 +439,14 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
     }
   }
   __syncthreads();
-  uint32_t qf[NQ][NG][4], qb[NQ][M::NP], qst[NQ][M::NP];   // fragments; sums against the bases; sums times -128 against the steps
+  if (joins && threadIdx.x == 0) {
+    // Advance the length: this CTA has read it, and the last CTA of the sequence to say so moves it on.
+    if (atomicAdd(c.tickets + seq, 1) == splits * passes * c.Hkv - 1) {
+      c.tickets[seq] = 0;
+      c.lengths[seq] = total;
+    }
+  }
+  uint32_t qf[NQ][NG][4], qb[NQ][M::NP];              // fragments; pieces of the sums
   int lim[NQ][2];                                     // positions that queries 2 tig and 2 tig + 1 see
 #pragma unroll
   for (int nt = 0; nt < NQ; ++nt) {
@@ -433,7 +458,6 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
 #pragma unroll
     for (int j = 0; j < M::NP; ++j) {
       qb[nt][j] = reinterpret_cast<const uint32_t*>(sm + M::QUERIES)[(nt * M::NP + j) * 32 + lane];
-      qst[nt][j] = NG == 1 ? 0u : as_bits(__hmul2(as_pair(qb[nt][j]), __float2bfloat162_rn(-128.f)));
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -444,7 +468,8 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
   const int all_see = len + q0 / group + 1;           // positions below this are seen by every query of the pass
 
   // A weight is 2^(score - ref): ref is the maximum when it was last looked up and stays until a score passes it
-  // by RISE; until then neither the sums nor the products have to be scaled.
+  // by RISE; until then neither the sums nor the products have to be scaled.  Scores and ref are kept times 2^(Q_UP - RAW), values times
+  // 2^(STEP_UP - RAW).
   float ref[NQ][2], l[NQ][2], o[NQ][CT][4];
 
 #pragma unroll
@@ -485,19 +510,22 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
       const Words<NG> hi = load_words<NG>(page + L::KEYS + (16 * mt + gid + 8) * (HD / 2) + tig * NG * 4);
       const Words<NG> plo = load_words<NG>(page + L::KPAR + (16 * mt + gid) * NG * 4);
       const Words<NG> phi = load_words<NG>(page + L::KPAR + (16 * mt + gid + 8) * NG * 4);
+      // bases: the word of two groups' bases is the same for the lanes of a position, each lane has its piece of the queries' sums
 #pragma unroll
-      for (int j = 0; j < M::NP; ++j)
+      for (int nt = 0; nt < NQ; ++nt) {
+        if constexpr (M::NP == 1) {
+          mma1688_new(s[nt][mt], plo.w[NG - 1], phi.w[NG - 1], qb[nt][0]);
+        } else {
+          mma16816_new(s[nt][mt], plo.w[1], phi.w[1], plo.w[3], phi.w[3], qb[nt][0], qb[nt][1]);
 #pragma unroll
-        for (int nt = 0; nt < NQ; ++nt) {
-          const uint32_t a0 = NG == 1 ? plo.w[0] : plo.w[2 * j + 1], a1 = NG == 1 ? phi.w[0] : phi.w[2 * j + 1];
-          const uint32_t a2 = NG == 1 ? 0u : plo.w[2 * j], a3 = NG == 1 ? 0u : phi.w[2 * j];
-          if (j == 0) mma16816_new(s[nt][mt], a0, a1, a2, a3, qb[nt][j], qst[nt][j]);
-          else mma16816(s[nt][mt], a0, a1, a2, a3, qb[nt][j], qst[nt][j]);
+          for (int j = 2; j < M::NP; j += 2)
+            mma16816(s[nt][mt], plo.w[2 * j + 1], phi.w[2 * j + 1], plo.w[2 * j + 3], phi.w[2 * j + 3], qb[nt][j], qb[nt][j + 1]);
         }
+      }
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        const uint32_t a0 = pair128<0>(lo.w[g], bits), a1 = pair128<0>(hi.w[g], bits), a2 = pair128<1>(lo.w[g], bits), a3 = pair128<1>(hi.w[g], bits);
-        const uint32_t b0 = pair128<2>(lo.w[g], bits), b1 = pair128<2>(hi.w[g], bits), b2 = pair128<3>(lo.w[g], bits), b3 = pair128<3>(hi.w[g], bits);
+        const uint32_t a0 = raw_pair<0>(lo.w[g]), a1 = raw_pair<0>(hi.w[g]), a2 = raw_pair<1>(lo.w[g]), a3 = raw_pair<1>(hi.w[g]);
+        const uint32_t b0 = raw_pair<2>(lo.w[g]), b1 = raw_pair<2>(hi.w[g]), b2 = raw_pair<3>(lo.w[g]), b3 = raw_pair<3>(hi.w[g]);
         const uint32_t w0 = plo.w[NG == 1 ? 0 : g & ~1], w1 = phi.w[NG == 1 ? 0 : g & ~1];
         const float st0 = __uint_as_float(g & 1 ? w0 & 0xffff0000u : w0 << 16), st1 = __uint_as_float(g & 1 ? w1 & 0xffff0000u : w1 << 16);
 #pragma unroll
@@ -533,7 +561,7 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
 #pragma unroll
         for (int mt = 1; mt < 4; ++mt) a = fmaxf(a, fmaxf(s[nt][mt][e], s[nt][mt][e + 2]));
         mx[nt][e] = a;
-        rise |= a > ref[nt][e] + RISE;
+        rise |= a > ref[nt][e] + RISE * pow2(Q_UP - RAW);
       }
     if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
@@ -545,7 +573,7 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
           a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 8));
           a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 16));
           a = fmaxf(a, ref[nt][e]);
-          const float corr = a > -INFINITY ? ex2(ref[nt][e] - a) : 1.f;
+          const float corr = a > -INFINITY ? ex2((ref[nt][e] - a) * pow2(RAW - Q_UP)) : 1.f;
           ref[nt][e] = a;
           l[nt][e] *= corr;
 #pragma unroll
@@ -555,14 +583,15 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
 #pragma unroll
     for (int nt = 0; nt < NQ; ++nt) {
       // a query that has seen nothing yet has scores of -inf only: weights of 0 against any finite number
-      const uint64_t minus = pack2(ref[nt][0] > -INFINITY ? -ref[nt][0] : 0.f, ref[nt][1] > -INFINITY ? -ref[nt][1] : 0.f);
+      const uint64_t up = pack2(pow2(RAW - Q_UP), pow2(RAW - Q_UP));
+      const uint64_t minus = pack2(ref[nt][0] > -INFINITY ? ref[nt][0] * -pow2(RAW - Q_UP) : 0.f, ref[nt][1] > -INFINITY ? ref[nt][1] * -pow2(RAW - Q_UP) : 0.f);
       uint64_t sum = pack2(l[nt][0], l[nt][1]);
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float y0, y1;
-          unpack2(add2(pack2(s[nt][mt][2 * h], s[nt][mt][2 * h + 1]), minus), y0, y1);
+          unpack2(fma2(pack2(s[nt][mt][2 * h], s[nt][mt][2 * h + 1]), up, minus), y0, y1);
           const float w0 = ex2(y0), w1 = ex2(y1);
           sum = add2(sum, pack2(w0, w1));
           p[nt][mt][h] = transpose8x8(as_bits(__floats2bfloat162_rn(w0, w1)));
@@ -592,7 +621,10 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
     }
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      const Words<8> step = load_words<8>(page + L::VSTEP + g * 128 + tig * 32), base = load_words<8>(page + L::VBASE + g * 128 + tig * 32);
+      const Words<8> step = load_words<8>(page + L::VSTEP + g * 128 + tig * 32);
+      Words<8> base = load_words<8>(page + L::VBASE + g * 128 + tig * 32);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) base.w[j] = as_bits(__hmul2(as_pair(base.w[j]), __float2bfloat162_rn(pow2(STEP_UP - RAW))));
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int ct = 2 * g + half;
@@ -601,10 +633,10 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
           const int j = 4 * w;
-          const uint32_t a0 = value_pair<0>(lo.w[w], step.w[j], base.w[j], bits), a1 = value_pair<0>(hi.w[w], step.w[j], base.w[j], bits);
-          const uint32_t a2 = value_pair<1>(lo.w[w], step.w[j + 1], base.w[j + 1], bits), a3 = value_pair<1>(hi.w[w], step.w[j + 1], base.w[j + 1], bits);
-          const uint32_t b0 = value_pair<2>(lo.w[w], step.w[j + 2], base.w[j + 2], bits), b1 = value_pair<2>(hi.w[w], step.w[j + 2], base.w[j + 2], bits);
-          const uint32_t b2 = value_pair<3>(lo.w[w], step.w[j + 3], base.w[j + 3], bits), b3 = value_pair<3>(hi.w[w], step.w[j + 3], base.w[j + 3], bits);
+          const uint32_t a0 = value_pair<0>(lo.w[w], step.w[j], base.w[j]), a1 = value_pair<0>(hi.w[w], step.w[j], base.w[j]);
+          const uint32_t a2 = value_pair<1>(lo.w[w], step.w[j + 1], base.w[j + 1]), a3 = value_pair<1>(hi.w[w], step.w[j + 1], base.w[j + 1]);
+          const uint32_t b0 = value_pair<2>(lo.w[w], step.w[j + 2], base.w[j + 2]), b1 = value_pair<2>(hi.w[w], step.w[j + 2], base.w[j + 2]);
+          const uint32_t b2 = value_pair<3>(lo.w[w], step.w[j + 3], base.w[j + 3]), b3 = value_pair<3>(hi.w[w], step.w[j + 3], base.w[j + 3]);
 #pragma unroll
           for (int nt = 0; nt < NQ; ++nt) {
             mma16816(o[nt][ct], a0, a1, a2, a3, p[nt][2 * w][0], p[nt][2 * w][1]);
@@ -634,12 +666,12 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
     for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        mb[((nt * 8 + 2 * tig + (e & 1)) * WARPS + warp) * PW + 16 * ct + gid + 8 * (e >> 1)] = o[nt][ct][e];
+        mb[((nt * 8 + 2 * tig + (e & 1)) * WARPS + warp) * PW + 16 * ct + gid + 8 * (e >> 1)] = o[nt][ct][e] * pow2(RAW - STEP_UP);
     if (gid == 0) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float* d = mb + ((nt * 8 + 2 * tig + e) * WARPS + warp) * PW + HD;
-        d[0] = ref[nt][e];
+        d[0] = ref[nt][e] * pow2(RAW - Q_UP);
         d[1] = l[nt][e];
       }
     }
@@ -666,7 +698,7 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
   }
   if (!joins) return;                                 // kv_merge_kernel does the rest
 
-  // ---- join the slices, write the merged heads, advance the length ----
+  // ---- join the slices, write the merged heads ----
   cg::cluster_group cl = cg::this_cluster();
   if (splits > 1) cl.sync(); else __syncthreads();
   for (int i = split * THREADS + threadIdx.x; i < live * HD; i += splits * THREADS) {
@@ -683,14 +715,6 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
     merged[(((long long)sj * rows + qi / group) * c.H + kvh * group + qi % group) * HD + ch] = __float2bfloat16_rn(num / den);
   }
   if (splits > 1) cl.sync();                          // nobody leaves while its slice is being read
-  if (threadIdx.x == 0) {
-    // every CTA of the sequence has read the length long before it takes its ticket; the last one moves it on
-    const int ctas = splits * passes * c.Hkv;
-    if (atomicAdd(c.tickets + seq, 1) == ctas - 1) {
-      c.tickets[seq] = 0;
-      c.lengths[seq] = total;
-    }
-  }
 }
 
 __global__ void tables_kernel(float* cos_t, float* sin_t, int positions, int half, double base) {
@@ -718,7 +742,7 @@ __global__ void values_kernel(Cache c, int first, int from, int count, float* __
       const float kc = (float)((kw >> (4 * (((ch & 7) >> 1) + 4 * (ch & 1)))) & 15u), vc = (float)((vw >> (4 * value_nibble(slot))) & 15u);
       const float ks = __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(par) << 16);
       kv = fmaf(kc, ks, __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(par + key_base_after(NG)) << 16));
-      vv = fmaf(vc, __uint_as_float((uint32_t)vstep[0] << 16), __uint_as_float((uint32_t)vstep[NG * 64] << 16));
+      vv = fmaf(vc, __uint_as_float((uint32_t)vstep[0] << 16) * pow2(value_heavy(slot) ? 4 - STEP_UP : -STEP_UP), __uint_as_float((uint32_t)vstep[NG * 64] << 16));
       if (ks != ks) kv = vv = ks;
     }
     keys[(long long)row * W + i] = kv;
@@ -753,7 +777,7 @@ cudaError_t go(const Cache& c, const bf16* q, const bf16* k, const bf16* v, int 
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   count_launch();
-  return cudaLaunchKernelEx(&cfg, kernel, c, q, k, v, first, rows, splits, passes, append ? 1 : 0, scale_log2, Bits{0x000f000fu, 0x43004300u}, merged, part);
+  return cudaLaunchKernelEx(&cfg, kernel, c, q, k, v, first, rows, splits, passes, append ? 1 : 0, scale_log2, merged, part);
 }
 
 }  // namespace
