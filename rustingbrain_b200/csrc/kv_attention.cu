@@ -583,6 +583,7 @@ struct kv_cache {
   int* lengths = nullptr;           // device, one per sequence
   int* full = nullptr;              // device, one per sequence: set by a step that found no room (a replayed graph can get there)
   std::vector<int> host_full;
+  std::vector<int> pages;           // 4-bit caches: scratch of a step's host side
   std::vector<int> host_len;        // mirror: every change goes through this object
   float* cos_t = nullptr;
   float* sin_t = nullptr;
@@ -717,32 +718,66 @@ q4::Cache q4_view(const kv_cache* c) {
   return q4::Cache{(unsigned char*)c->keys, c->lengths, c->full, c->tickets, c->cos_t, c->sin_t, g.num_heads, g.kv_heads, g.head_dim, g.capacity, g.rope};
 }
 
-// The step on a 4-bit cache: one launch where the new rows' queries fit one pass and a cluster joins the slices.  Nothing is allocated.
+// The step on a 4-bit cache.  Nothing is allocated.
 int forward_q4(kv_cache* c, int first, int n_seq, const void* q, const void* k, const void* v, int rows, void* merged, cudaStream_t st) {
   const kv_cache_config_t& g = c->cfg;
   const q4::Cache view = q4_view(c);
-  int longest = 0;
-  for (int i = 0; i < n_seq; ++i) longest = std::max(longest, c->host_len[first + i] + rows);
+  int longest = 0;   // in pages, as far as the host knows: a replayed step is only cut less evenly
+  long long sum = 0;
+  c->pages.resize(n_seq);
+  for (int i = 0; i < n_seq; ++i) {
+    c->pages[i] = ceil_div(c->host_len[first + i] + rows, q4::PAGE);
+    longest = std::max(longest, c->pages[i]);
+    sum += c->pages[i];
+  }
   const long long nq = (long long)rows * (g.num_heads / g.kv_heads);
-  const int per_pass = q4::queries_per_pass(g.head_dim, (int)std::min<long long>(nq, 1 << 20));
-  const long long passes = (nq + per_pass - 1) / per_pass, ctas = (long long)n_seq * g.kv_heads * passes;
-  // as many CTAs as are resident at once, a page or more for each warp
-  const int pages = ceil_div(longest, q4::PAGE);
-  int splits = (int)std::min<long long>(KV_MAX_SPLITS, std::max<long long>(1, 4ll * c->sm_count / ctas));
-  splits = std::max(1, std::min(splits, ceil_div(pages, 4)));
-  if (const char* v = getenv("KV_B200_SPLITS")) splits = std::max(1, std::min(KV_MAX_SPLITS, atoi(v)));   // experiments
-  if (splits > q4::CLUSTER && ((size_t)n_seq * rows * g.num_heads * splits * (g.head_dim + 2) > c->part_floats)) splits = q4::CLUSTER;
+  const int queries = (int)std::min<long long>(nq, 1 << 20), per_pass = q4::queries_per_pass(g.head_dim, queries);
+  const long long passes = (nq + per_pass - 1) / per_pass, heads = g.kv_heads * passes, ctas = n_seq * heads;
+  const long long slots = (long long)c->sm_count * q4::ctas_per_sm(g.head_dim, queries, g.device);
+  // Two ways to cut a head's pages:
+  //  - a cluster of up to 8 slices that joins them itself.  One launch, but a cluster stays until its last CTA is done: for sequences of
+  //    one length;
+  //  - slices of one size for all sequences, joined by a second launch: for lengths that differ, and for a few long sequences.
+  // Chosen by what they would take, in microseconds: a page takes a CTA its share of 6000 bytes a nanosecond, though at least a quarter
+  // of the microsecond that a warp needs for one of 64 channels; a CTA's start and end and the second launch take about 3 each.
+  const double bytes = (double)q4::page_bytes(g.head_dim);
+  auto estimate = [&](long long active, int slice) {
+    const long long waves = (active + slots - 1) / slots;
+    const double page = std::max(0.25 * g.head_dim / 64, bytes * (double)std::min(active, slots) / 6e6);
+    return (double)waves * (slice * page + 3.0);
+  };
+  int splits = (int)std::min<long long>(q4::CLUSTER, std::max<long long>(1, slots / ctas));
+  splits = std::max(1, std::min(splits, ceil_div(longest, 4)));
+  int slice = ceil_div(longest, splits);
+  float* part = nullptr;
+  double best = estimate(ctas * splits, slice);
+  const long long room = (long long)(c->part_floats / ((size_t)n_seq * rows * g.num_heads * (g.head_dim + 2)));
+  const int most = (int)std::min<long long>(KV_MAX_SPLITS, room);
+  if (most >= 2 && n_seq <= 512 && (sum != (long long)longest * n_seq || splits == q4::CLUSTER)) {
+    for (int waves = 1; waves <= 3; ++waves) {
+      // the smallest slice whose CTAs fit that many times
+      int cut = (int)std::max<long long>(std::max(4, ceil_div(longest, most)), (sum * heads + waves * slots - 1) / (waves * slots));
+      long long active = 0;
+      for (;; cut += std::max(1, cut / 16)) {
+        active = 0;
+        for (int i = 0; i < n_seq; ++i) active += ceil_div(c->pages[i], cut);
+        active *= heads;
+        if (active <= waves * slots || cut >= longest) break;
+      }
+      const double time = estimate(active, cut) + 3.0;
+      if (time < best && cut < longest) {
+        best = time;
+        slice = cut;
+        splits = ceil_div(longest, cut);
+        part = c->part;
+      }
+    }
+  }
   if (ctas * splits > 0x7fffffffll) return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: too many rows");
   const bool append = passes == 1;   // one CTA per slice: it stores the slice's new positions itself
   if (!append) KCK(q4::launch_append(view, (const bf16*)k, (const bf16*)v, first, n_seq, rows, st));
   const float scale_log2 = LOG2E / sqrtf((float)g.head_dim);
-  KCK(q4::launch_attention(view, (const bf16*)q, (const bf16*)k, (const bf16*)v, first, n_seq, rows, splits, append, scale_log2, (bf16*)merged, c->part, st));
-  if (splits > q4::CLUSTER) {
-    const KvShape s{g.num_heads, g.kv_heads, g.head_dim, g.capacity, rows, first};
-    kv_merge_kernel<bf16><<<n_seq * rows * g.num_heads, std::min(256, g.head_dim), 0, st>>>(c->part, (bf16*)merged, c->lengths, c->full, s, splits);
-    count_launch();
-    KCK(cudaGetLastError());
-  }
+  KCK(q4::launch_attention(view, (const bf16*)q, (const bf16*)k, (const bf16*)v, first, n_seq, rows, splits, slice, append, scale_log2, (bf16*)merged, part, st));
   for (int i = 0; i < n_seq; ++i) c->host_len[first + i] += rows;
   return MOE_OK;
 }

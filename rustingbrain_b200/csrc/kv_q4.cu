@@ -308,11 +308,11 @@ template <int HD, int NQ> struct Smem {
   static constexpr int BYTES = FRONT + WARPS * WARP > MERGE ? FRONT + WARPS * WARP : MERGE;
 };
 
-// grid: ((sequence * kv heads + kv head) * passes + pass) * splits + split; the splits of one are a cluster when it joins them
+// grid: ((sequence * kv heads + kv head) * passes + pass) * splits + split; the splits of one are a cluster when `joins` is set
 template <int HD, int NQ>
 __global__ void __launch_bounds__(THREADS)
-attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v, int first, int rows, int splits,
-                 int passes, int append, float scale_log2, bf16* __restrict__ merged, float* __restrict__ part) {
+attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v, int first, int rows, int splits, int slice,
+                 int passes, int append, int joins, float scale_log2, bf16* __restrict__ merged, float* __restrict__ part) {
   using L = Layout<HD>;
   constexpr int NG = L::NG, CT = HD / 16, SLOTS = Ring<HD>::SLOTS, PW = HD + 2, QT = NQ * 8;
   extern __shared__ __align__(128) unsigned char sm[];
@@ -321,10 +321,9 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
   const int group = c.H / c.Hkv, nq = rows * group, q0 = pass * QT;
   const int len = c.lengths[seq], total = len + rows;
-  const bool joins = splits <= CLUSTER;               // the slices are a cluster
   if (total > c.cap) {                                // no room: nothing is stored or advanced, the step's rows are zeros
     if (threadIdx.x == 0) c.full[seq] = 1;
-    if (split == 0 && joins)
+    if (split == 0)
       for (int i = threadIdx.x; i < min(QT, nq - q0) * HD; i += THREADS) {
         const int qi = q0 + i / HD, r = qi / group, g = qi - r * group;
         merged[(((long long)sj * rows + r) * c.H + kvh * group + g) * HD + i % HD] = __float2bfloat16_rn(0.f);
@@ -332,10 +331,11 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
     return;
   }
   // pages of this slice, as far as the last query of the pass sees
-  const int pages = (total + PAGE - 1) / PAGE, chunk = (pages + splits - 1) / splits;
+  const int pages = (total + PAGE - 1) / PAGE, chunk = max(slice, (pages + splits - 1) / splits);
   const int pg0 = split * chunk, pg1 = min(pages, pg0 + chunk);
   const int last_row = (min(q0 + QT, nq) - 1) / group, seen_pages = (len + last_row) / PAGE + 1;
   const int pend = min(pg1, seen_pages);
+  if (!joins && pg0 >= pend) return;                  // no such slice: merge_kernel does not look for it either
   unsigned char* head = page_at(c, seq, kvh, 0);
   // The warp's half pages, last page first (the new positions are in the last ones): unit 2 j is the keys and 2 j + 1 the values of page
   // pg - j * WARPS.
@@ -656,6 +656,7 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
       l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 16);
     }
 
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // ---- join the warps: [query][warp][HD + 2], then this slice's [query][HD + 2] behind it ----
   float* mb = reinterpret_cast<float*>(sm);
   float* mine = mb + QT * WARPS * PW;
@@ -696,7 +697,7 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
     out[ch] = num;
     if (ch == 0) { out[HD] = mx; out[HD + 1] = den; }
   }
-  if (!joins) return;                                 // kv_merge_kernel does the rest
+  if (!joins) return;                                 // merge_kernel does the rest
 
   // ---- join the slices, write the merged heads ----
   cg::cluster_group cl = cg::this_cluster();
@@ -715,6 +716,75 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
     merged[(((long long)sj * rows + qi / group) * c.H + kvh * group + qi % group) * HD + ch] = __float2bfloat16_rn(num / den);
   }
   if (splits > 1) cl.sync();                          // nobody leaves while its slice is being read
+}
+
+// One CTA joins the slices of one row's head, each warp every fourth of them.
+template <int HD>
+__global__ void __launch_bounds__(THREADS)
+merge_kernel(Cache c, const float* __restrict__ part, int first, int rows, int splits, int slice, int per_pass, bf16* __restrict__ merged) {
+  constexpr int PW = HD + 2, CH = HD / 32, AHEAD = 4;
+  __shared__ float sums[WARPS][PW];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long at = blockIdx.x;                    // (sequence * rows + row) * heads + head
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the slices are written
+  const int row_at = (int)(at / c.H), h = (int)(at - (long long)row_at * c.H), sj = row_at / rows, row = row_at - sj * rows, seq = first + sj;
+  const int len = c.lengths[seq], total = len + rows, group = c.H / c.Hkv;
+  if (total > c.cap) return;                          // marked, and its rows zeroed, by the step
+  const int pages = (total + PAGE - 1) / PAGE, chunk = max(slice, (pages + splits - 1) / splits);
+  const int pass = (row * group + h % group) / per_pass, last_row = (min((pass + 1) * per_pass, rows * group) - 1) / group;
+  const int live = (min(pages, (len + last_row) / PAGE + 1) + chunk - 1) / chunk;
+  const float* src = part + at * splits * PW;
+  float ref = -INFINITY, den = 0.f, num[CH];
+#pragma unroll
+  for (int i = 0; i < CH; ++i) num[i] = 0.f;
+  for (int p0 = warp; p0 < live; p0 += WARPS * AHEAD) {
+    float m[AHEAD], l[AHEAD], x[AHEAD][CH];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const int p = p0 + a * WARPS, ok = p < live;
+      m[a] = ok ? __ldcg(src + p * PW + HD) : -INFINITY;
+      l[a] = ok ? __ldcg(src + p * PW + HD + 1) : 0.f;
+#pragma unroll
+      for (int i = 0; i < CH; ++i) x[a][i] = ok ? __ldcg(src + p * PW + 32 * i + lane) : 0.f;
+    }
+    float now = ref;
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) now = fmaxf(now, m[a]);
+    const float base = now > -INFINITY ? now : 0.f, corr = ex2(ref - base);
+    den *= corr;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) num[i] *= corr;
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const float w = ex2(m[a] - base);
+      den = fmaf(w, l[a], den);
+#pragma unroll
+      for (int i = 0; i < CH; ++i) num[i] = fmaf(w, x[a][i], num[i]);
+    }
+    ref = now;
+  }
+#pragma unroll
+  for (int i = 0; i < CH; ++i) sums[warp][32 * i + lane] = num[i];
+  if (lane == 0) { sums[warp][HD] = ref; sums[warp][HD + 1] = den; }
+  __syncthreads();
+  for (int ch = threadIdx.x; ch < HD; ch += THREADS) {
+    float mx = -INFINITY, n = 0.f, d = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) mx = fmaxf(mx, sums[w][HD]);
+    const float base = mx > -INFINITY ? mx : 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float wt = ex2(sums[w][HD] - base);
+      n = fmaf(wt, sums[w][ch], n);
+      d = fmaf(wt, sums[w][HD + 1], d);
+    }
+    merged[at * HD + ch] = __float2bfloat16_rn(n / d);
+  }
+  // every thread has read the length before the barrier above; the last CTA of the sequence moves it on
+  if (threadIdx.x == 0 && atomicAdd(c.tickets + seq, 1) == rows * c.H - 1) {
+    c.tickets[seq] = 0;
+    c.lengths[seq] = total;
+  }
 }
 
 __global__ void tables_kernel(float* cos_t, float* sin_t, int positions, int half, double base) {
@@ -751,20 +821,10 @@ __global__ void values_kernel(Cache c, int first, int from, int count, float* __
 }
 
 template <int HD, int NQ>
-cudaError_t go(const Cache& c, const bf16* q, const bf16* k, const bf16* v, int first, int n_seq, int rows, int splits, bool append, float scale_log2,
+cudaError_t go(const Cache& c, const bf16* q, const bf16* k, const bf16* v, int first, int n_seq, int rows, int splits, int slice, bool append, float scale_log2,
                bf16* merged, float* part, cudaStream_t st) {
   constexpr int smem = Smem<HD, NQ>::BYTES;
   auto kernel = attention_kernel<HD, NQ>;
-  static std::atomic<unsigned long long> raised{0};   // devices on which the kernel's shared-memory limit has been raised
-  int device = 0;
-  cudaError_t e = cudaGetDevice(&device);
-  if (e != cudaSuccess) return e;
-  const unsigned long long bit = 1ull << (device & 63);
-  if (!(raised.load(std::memory_order_relaxed) & bit)) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    raised.fetch_or(bit, std::memory_order_relaxed);
-  }
   const int nq = rows * (c.H / c.Hkv), passes = (nq + NQ * 8 - 1) / (NQ * 8);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(splits * passes * c.Hkv * n_seq));
@@ -773,11 +833,25 @@ cudaError_t go(const Cache& c, const bf16* q, const bf16* k, const bf16* v, int 
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = splits <= CLUSTER ? splits : 1; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  const bool joins = part == nullptr;
+  if (joins) { cfg.attrs = attr; cfg.numAttrs = 1; }
+  attr[0].val.clusterDim.x = splits;
   count_launch();
-  return cudaLaunchKernelEx(&cfg, kernel, c, q, k, v, first, rows, splits, passes, append ? 1 : 0, scale_log2, merged, part);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, c, q, k, v, first, rows, splits, slice, passes, append ? 1 : 0, joins ? 1 : 0, scale_log2, merged, part);
+  if (e != cudaSuccess || joins) return e;
+  // resident as soon as the step's last CTA has only its results to write
+  cudaLaunchConfig_t join{};
+  join.gridDim = dim3((unsigned)(n_seq * rows * c.H));
+  join.blockDim = dim3(THREADS);
+  join.stream = st;
+  cudaLaunchAttribute early[1];
+  early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early[0].val.programmaticStreamSerializationAllowed = 1;
+  join.attrs = early;
+  join.numAttrs = 1;
+  count_launch();
+  return cudaLaunchKernelEx(&join, merge_kernel<HD>, c, (const float*)part, first, rows, splits, slice, NQ * 8, merged);
 }
 
 }  // namespace
@@ -804,10 +878,10 @@ cudaError_t launch_append(const Cache& c, const bf16* k, const bf16* v, int firs
 
 int queries_per_pass(int head_dim, int queries) { return queries <= 8 || head_dim == 256 ? 8 : 16; }
 
-cudaError_t launch_attention(const Cache& c, const bf16* q, const bf16* k, const bf16* v, int first, int n_seq, int rows, int splits, bool append,
+cudaError_t launch_attention(const Cache& c, const bf16* q, const bf16* k, const bf16* v, int first, int n_seq, int rows, int splits, int slice, bool append,
                              float scale_log2, bf16* merged, float* part, cudaStream_t st) {
   const bool two = queries_per_pass(c.HD, rows * (c.H / c.Hkv)) == 16;
-#define Q4_GO(HD, NQ) go<HD, NQ>(c, q, k, v, first, n_seq, rows, splits, append, scale_log2, merged, part, st)
+#define Q4_GO(HD, NQ) go<HD, NQ>(c, q, k, v, first, n_seq, rows, splits, slice, append, scale_log2, merged, part, st)
   switch (c.HD) {
     case 32: return two ? Q4_GO(32, 2) : Q4_GO(32, 1);
     case 64: return two ? Q4_GO(64, 2) : Q4_GO(64, 1);
@@ -816,6 +890,31 @@ cudaError_t launch_attention(const Cache& c, const bf16* q, const bf16* k, const
     default: return cudaErrorInvalidValue;
   }
 #undef Q4_GO
+}
+
+template <int HD, int NQ>
+int resident(int device) {
+  static std::atomic<int> known[64] = {};             // per device, plus one
+  std::atomic<int>& slot = known[device & 63];
+  if (const int n = slot.load(std::memory_order_relaxed)) return n - 1;
+  int per_sm = 0;
+  cudaFuncSetAttribute(attention_kernel<HD, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<HD, NQ>::BYTES);
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, attention_kernel<HD, NQ>, THREADS, Smem<HD, NQ>::BYTES) != cudaSuccess) {
+    cudaGetLastError();
+    per_sm = 1;
+  }
+  slot.store(per_sm + 1, std::memory_order_relaxed);
+  return per_sm;
+}
+
+int ctas_per_sm(int head_dim, int queries, int device) {
+  const bool two = queries_per_pass(head_dim, queries) == 16;
+  switch (head_dim) {
+    case 32: return two ? resident<32, 2>(device) : resident<32, 1>(device);
+    case 64: return two ? resident<64, 2>(device) : resident<64, 1>(device);
+    case 128: return two ? resident<128, 2>(device) : resident<128, 1>(device);
+    default: return resident<256, 1>(device);
+  }
 }
 
 cudaError_t launch_values(const Cache& c, int first, int n_seq, int from, int count, float* keys, float* values, cudaStream_t st) {

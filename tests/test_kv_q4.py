@@ -123,6 +123,33 @@ def test_one_long_sequence(H, Hkv, hd, n, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,Hkv,hd,rows", [(8, 2, 64, 1), (4, 1, 128, 3), (2, 2, 256, 1), (24, 2, 32, 2)])
+def test_slices_of_sequences_that_differ_much(H, Hkv, hd, rows):
+    """From an empty sequence to a long one: slices of one size for all, most of them not there, joined by a second launch."""
+    lens = [3000, 0, 9000, 5, 63, 700, 4000]
+    S, cap = len(lens), 9100
+    cache, o = KvCache(S, H, Hkv, hd, cap, precision="q4"), [Q4CacheOracle(H, Hkv, hd, cap) for _ in lens]
+    for s, n in enumerate(lens):
+        if n:
+            _, k, v = _rows(n, H, Hkv, hd, 300 + s)
+            cache.append(_dev(k), _dev(v), rows_per_sequence=n, first_sequence=s, n_sequences=1)
+            o[s].append(k, v)
+    for step in range(2):
+        q, k, v = _rows(S * rows, H, Hkv, hd, 400 + step)
+        got = cache.forward_cached(_dev(q), _dev(k), _dev(v), rows_per_sequence=rows)
+        for s in range(S):
+            sl = slice(s * rows, (s + 1) * rows)
+            _close(got[sl], o[s].forward_cached(q[sl], k[sl], v[sl]))
+    assert cache.lengths() == [n + 2 * rows for n in lens]
+    q, k, v = _rows(2 * rows, H, Hkv, hd, 500)                 # a part of the cache: the others stay
+    got = cache.forward_cached(_dev(q), _dev(k), _dev(v), rows_per_sequence=rows, first_sequence=2, n_sequences=2)
+    for j, s in enumerate((2, 3)):
+        sl = slice(j * rows, (j + 1) * rows)
+        _close(got[sl], o[s].forward_cached(q[sl], k[sl], v[sl]))
+    assert cache.lengths() == [n + (3 if s in (2, 3) else 2) * rows for s, n in enumerate(lens)]
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("H,Hkv,hd,n", [(8, 2, 64, 200), (4, 1, 128, 97), (2, 2, 32, 64), (4, 4, 256, 70)])
 def test_a_prompt_at_once_equals_row_by_row(H, Hkv, hd, n):
     one, many, o = KvCache(1, H, Hkv, hd, 256, precision="q4"), KvCache(1, H, Hkv, hd, 256, precision="q4"), Q4CacheOracle(H, Hkv, hd, 256)
