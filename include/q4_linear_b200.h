@@ -4,12 +4,13 @@
  *
  *   y[r, n] = sum_k x[r, k] * w[n, k],    w[n, k] = scale[n, k / group] * code[n, k]
  *
- * code is -8 .. 7, scale a bf16 number, group 32, 64 or 128 input channels; d_in is a multiple of the group, d_out anything.
- * x and y are both f32 (MOE_PRECISION_F32) or both bf16 (MOE_PRECISION_BF16).  Products of codes and activations are exact, sums are f32,
- * y is rounded once; the order of the sums depends on the sizes only, so results do not depend on the run.  An infinity or a NaN of x
- * or of a scale appears in the outputs it takes part in.
+ * code is -8 .. 7, scale a bf16 number, group 32, 64 or 128 input channels; d_in is a multiple of the group and at most 65536, d_out anything.
+ * x and y are both f32 (MOE_PRECISION_F32) or both bf16 (MOE_PRECISION_BF16).  Products of codes and activations are exact (in bf16
+ * batches of more than 16 rows an activation is kept to 2^-17 of the largest of its row), sums are f32, y is rounded once; the order of the
+ * sums depends on the sizes only, so results do not depend on the run.  An infinity or a NaN of x or of a scale appears in the outputs it
+ * takes part in.
  *
- * Meant for decode batches: up to 64 rows read the weights once, more rows read them once for every 64.
+ * Meant for decode batches: up to 64 rows (fewer where d_in is very large) read the weights once, more rows read them once for every 64.
  *
  * Stateless: all pointers are device pointers of the current device, owned by the caller; nothing is allocated, no scratch is kept, every
  * call can be captured into a CUDA graph, and calls on different streams do not meet.  Status codes are the moe_status values of
@@ -41,7 +42,7 @@ int32_t q4_linear_dequantize(const void* packed, float* weights, int32_t d_out, 
                              int32_t message_len);
 
 /* x rows are ld_x elements apart and start on 16-byte boundaries; y rows are ld_y elements apart.  y does not overlap x.
- * rows == 0 is a call that does nothing. */
+ * rows is at most 65535; rows == 0 is a call that does nothing. */
 int32_t q4_linear_forward(const void* x, int64_t ld_x, const void* packed, void* y, int64_t ld_y, int32_t rows, int32_t d_in,
                           int32_t d_out, int32_t group, int32_t precision, void* stream, char* message, int32_t message_len);
 

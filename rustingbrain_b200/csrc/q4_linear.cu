@@ -1,18 +1,28 @@
 // Linear layer with 4-bit weights (the ABI of include/q4_linear_b200.h).
 //
 // For a decode batch the bytes of the weights are the time, so the layout is made for one pass over them: a block of 16 outputs x 64
-// input channels is 512 bytes, 16 for each lane of a warp, in the order in which the lane needs them as the A operand of mma.sync m16n8k16
-// (the outputs are the 16 rows, the batch rows the 8 columns).  A lane's 32-bit word holds 8 consecutive channels of one output;
-// since the channels of a product may come in any order, the activations' 8 channels are one 16-byte shared load of the B operand.
+// input channels is 512 bytes, 16 for each lane of a warp, in the order in which the lane needs them as the A operand of the tensor cores (the
+// outputs are the 16 rows, the batch rows the 8 columns).  A lane's 32-bit word holds 8 consecutive channels of one output; since the
+// channels of a product may come in any order, the activations' 8 channels are one 16-byte shared load of the B operand.  Two such blocks
+// (32 outputs) and their scales are a unit, which a warp brings into its own ring in shared memory, several units ahead.
 //
-// A code becomes a bf16 number by placing its four bits, plus 8, behind the exponent of 128 and subtracting 136: exact.  The products of a
-// group are summed by the tensor cores in f32 and the group's scale is applied to that sum, so neither code nor scale is ever rounded
-// and f32 activations lose nothing either: they are cut into three bf16 numbers that add up to them.
+// A code plus 8 needs no conversion.  Bits 0 .. 7 of a bf16 are a number linear in them, bits * 2^-133 (below 128 it is subnormal, and the
+// next binade goes on in the same steps), and bits 0 .. 3 of an e4m3 likewise, bits * 2^-9.  So a code is cut out of its word and is an
+// operand, at weight 1 or, where it comes out four bits further up, 16.  The activations make up for the powers of two, and the 8 that
+// the codes have too much is where the sum of a group starts: -8 times the sum of its activations.
+//   up to 16 rows, or f32:  activations as bf16 numbers, five instructions for eight codes.  Products are exact, and the group's scale is
+//                           applied to its f32 sum.  An f32 activation is three bf16 numbers that add up to it; there the 8 is taken off the
+//                           codes, whose sums then stay small enough for the accuracy of f32.
+//   more bf16 rows:         the tensor cores' time counts, and e4m3 products take a quarter of it: a bf16 activation, scaled so that its row's
+//                           largest is in 128 .. 256, is the sum of two e4m3 numbers (to 2^-17 of the largest), three instructions for eight codes.
 //
-// The reduction axis is split over the warps of a CTA and over the CTAs of a cluster, whose partial sums meet in (distributed)
-// shared memory, always in the same order: one launch, no workspace.
+// A CTA keeps the activations of up to 16 rows in shared memory and goes through tiles of outputs, weights arriving without a pause from
+// tile to tile; its warps split the reduction of a tile.  More rows are passes side by side, which find the weights in L2.  Where there
+// are fewer tiles than SMs the CTAs of a cluster split the reduction too.  Partial sums meet in (distributed) shared memory, always in
+// the same order: one launch, no workspace.
 
 #include <cooperative_groups.h>
+#include <cuda_fp16.h>
 #include <algorithm>
 #include <atomic>
 #include <cstdio>
@@ -26,67 +36,76 @@ namespace cg = cooperative_groups;
 namespace moe {
 namespace {
 
-constexpr int QL_WARPS = 8, QL_THREADS = QL_WARPS * 32;
-constexpr int QL_MT = 2;                 // 16-output blocks per warp: they share the B operand
-constexpr int QL_AHEAD = 4;              // weight blocks in flight per warp and 16 outputs
-constexpr int QL_ROWS = 64;              // batch rows per pass
+constexpr int QL_MAX_WARPS = 16;
+constexpr int QL_ROWS = 16;              // batch rows per pass
 constexpr int QL_MAX_CLUSTER = 8;
-constexpr int QL_SMEM = 64 * 1024;       // for the activations of a chunk; one unit of 64 f32 rows needs more
-constexpr int QL_SMEM_MAX = 3 * QL_ROWS * (QL_AHEAD * 128 + 64);
+constexpr int QL_MAX_IN = 1 << 16;       // a row of f32 activations, cut over a cluster, fits shared memory
+constexpr int QL_RAW = 133;              // bits 0 .. 7 of a bf16 are worth bits * 2^-QL_RAW
+constexpr int QL_UP = 88, QL_DOWN = 96;  // activations times 2^QL_UP, those of a row with one above 2^38 times 2^(QL_UP - QL_DOWN)
+constexpr float QL_LARGE = 274877906944.f;
 
+__host__ __device__ constexpr float ql_pow2(int e) {
+  float v = 1.f;
+  for (int i = 0; i < (e < 0 ? -e : e); ++i) v *= e < 0 ? 0.5f : 2.f;
+  return v;
+}
+
+// A unit: 32 outputs and 64 (group 128: 128) channels, codes [2 output blocks][blocks][512 bytes], then scales [2][scales][8][2] bf16.
+template <int GROUP> struct QlUnit {
+  static constexpr int BLOCKS = GROUP == 128 ? 2 : 1, SCALES = GROUP == 32 ? 2 : 1, CODES = 2 * BLOCKS * 512, BYTES = CODES + 2 * SCALES * 32;
+  static constexpr int CHANNELS = 64 * BLOCKS;
+};
 struct QlShape {
-  int d_in, d_out, group, kblocks, mtiles, sgroups;   // 64-channel blocks, 16-output blocks (padded to QL_MT), scale groups per output
+  int d_in, d_out, group, pairs, units, unit_bytes, channels;   // pairs of 16 outputs; units along the reduction
 };
 inline QlShape ql_shape(int d_out, int d_in, int group) {
   QlShape s;
   s.d_in = d_in; s.d_out = d_out; s.group = group;
-  s.kblocks = (d_in + 63) / 64;
-  s.mtiles = (d_out / 16 + (d_out % 16 != 0) + QL_MT - 1) / QL_MT * QL_MT;
-  s.sgroups = s.kblocks * 64 / group;
+  s.channels = group == 128 ? 128 : 64;
+  s.unit_bytes = group == 128 ? QlUnit<128>::BYTES : group == 64 ? QlUnit<64>::BYTES : QlUnit<32>::BYTES;
+  s.pairs = (d_out + 31) / 32;
+  s.units = (d_in + s.channels - 1) / s.channels;
   return s;
 }
-inline long long ql_code_bytes(const QlShape& s) { return (long long)s.mtiles * s.kblocks * 512; }
-inline long long ql_scale_bytes(const QlShape& s) { return (long long)s.mtiles * s.sgroups * 32; }
+inline long long ql_bytes(const QlShape& s) { return (long long)s.pairs * s.units * s.unit_bytes; }
 
-// Word of output n (of its 16-block) and 32-channel group g (of the 64-channel block) for channels 8 * tig .. + 7, in 32-bit units
-// from the block's start; inside it channel 2 i + e is nibble i + 4 e.
-__host__ __device__ inline int ql_word(int n, int g, int tig) { return ((n & 7) * 4 + tig) * 4 + 2 * g + (n >> 3); }
+// Byte offsets of output n's word for channels k .. k + 7 (k a multiple of 8), and of its scale; inside a word channel 2 i + e is nibble
+// i + 4 e.
+__device__ inline long long ql_word_at(const QlShape& s, int n, int k) {
+  const int unit = k / s.channels, blocks = s.channels / 64, block = (k % s.channels) / 64, g = (k >> 5) & 1, tig = (k >> 3) & 3;
+  return ((long long)(n >> 5) * s.units + unit) * s.unit_bytes + (((n >> 4) & 1) * blocks + block) * 512 + (((n & 7) * 4 + tig) * 4 + 2 * g + ((n >> 3) & 1)) * 4;
+}
+__device__ inline long long ql_scale_at(const QlShape& s, int n, int k) {
+  const int unit = k / s.channels, blocks = s.channels / 64, scales = s.group == 32 ? 2 : 1, g = s.group == 32 ? (k >> 5) & 1 : 0;
+  return ((long long)(n >> 5) * s.units + unit) * s.unit_bytes + 2 * blocks * 512 + (((n >> 4) & 1) * scales + g) * 32 + (n & 7) * 4 + ((n >> 3) & 1) * 2;
+}
 __host__ __device__ inline int ql_nibble(int c) { return ((c & 7) >> 1) + 4 * (c & 1); }
 
 // ---- packing (once per matrix) ----
-__global__ void ql_pack_kernel(const int8_t* __restrict__ codes, const bf16* __restrict__ scales, uint32_t* __restrict__ words,
-                               bf16* __restrict__ packed_scales, QlShape s) {
-  const long long words_total = (long long)s.mtiles * s.kblocks * 128, scales_total = (long long)s.mtiles * s.sgroups * 16;
-  const int groups = s.d_in / s.group;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < words_total + scales_total; i += (long long)gridDim.x * blockDim.x) {
-    if (i < words_total) {
-      const int word = (int)(i & 127), lane = word >> 2, g = (word >> 1) & 1, hi = word & 1;
-      const long long block = i >> 7;
-      const int mt = (int)(block / s.kblocks), kb = (int)(block - (long long)mt * s.kblocks);
-      const int n = mt * 16 + (lane >> 2) + 8 * hi, c0 = kb * 64 + g * 32 + (lane & 3) * 8;
-      uint32_t w = 0;
+// one thread per eight channels of one output, padding included
+__global__ void ql_pack_kernel(const int8_t* __restrict__ codes, const bf16* __restrict__ scales, unsigned char* __restrict__ packed, QlShape s) {
+  const int per = s.units * s.channels / 8, groups = s.d_in / s.group;
+  const long long total = (long long)s.pairs * 32 * per;
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+    const int n = (int)(i / per), k = (int)(i - (long long)n * per) * 8, grp = k / s.group;
+    uint32_t w = 0;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        const int code = n < s.d_out && c0 + c < s.d_in ? codes[(long long)n * s.d_in + c0 + c] : 0;
-        w |= ((uint32_t)(code + 8) & 15u) << (4 * ql_nibble(c));
-      }
-      words[i] = w;
-    } else {
-      const long long j = i - words_total;
-      const int slot = (int)(j & 15), gid = slot >> 1, hi = slot & 1;
-      const long long at = j >> 4;
-      const int mt = (int)(at / s.sgroups), grp = (int)(at - (long long)mt * s.sgroups), n = mt * 16 + gid + 8 * hi;
-      packed_scales[j] = n < s.d_out && grp < groups ? scales[(long long)n * groups + grp] : __float2bfloat16_rn(0.f);
+    for (int c = 0; c < 8; ++c) {
+      const int code = n < s.d_out && k + c < s.d_in ? codes[(long long)n * s.d_in + k + c] : 0;
+      w |= ((uint32_t)(code + 8) & 15u) << (4 * ql_nibble(c));
     }
+    *reinterpret_cast<uint32_t*>(packed + ql_word_at(s, n, k)) = w;
+    if (k % s.group == 0)
+      *reinterpret_cast<bf16*>(packed + ql_scale_at(s, n, k)) = n < s.d_out && grp < groups ? scales[(long long)n * groups + grp] : __float2bfloat16_rn(0.f);
   }
 }
 
 // one thread per (output, group), padding included
-__global__ void ql_quantize_kernel(const float* __restrict__ weights, uint32_t* __restrict__ words, bf16* __restrict__ packed_scales, QlShape s) {
-  const long long total = (long long)s.mtiles * 16 * s.sgroups;
-  const int groups = s.d_in / s.group;
+__global__ void ql_quantize_kernel(const float* __restrict__ weights, unsigned char* __restrict__ packed, QlShape s) {
+  const int per = s.units * s.channels / s.group, groups = s.d_in / s.group;
+  const long long total = (long long)s.pairs * 32 * per;
   for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
-    const int n = (int)(i / s.sgroups), grp = (int)(i - (long long)n * s.sgroups), mt = n >> 4, nl = n & 15;
+    const int n = (int)(i / per), grp = (int)(i - (long long)n * per);
     const bool live = n < s.d_out && grp < groups;
     const float* w = weights + (long long)n * s.d_in + (long long)grp * s.group;
     float top = 0.f;
@@ -100,7 +119,6 @@ __global__ void ql_quantize_kernel(const float* __restrict__ weights, uint32_t* 
     const bf16 scale = __float2bfloat16_rn(bad ? __uint_as_float(0x7fc00000u) : __fdiv_rn(top, 7.f));
     const float f = __bfloat162float(scale);
     for (int c0 = 0; c0 < s.group; c0 += 8) {
-      const int k = grp * s.group + c0, kb = k >> 6, g = (k >> 5) & 1, tig = (k >> 3) & 3;
       uint32_t word = 0;
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
@@ -108,197 +126,386 @@ __global__ void ql_quantize_kernel(const float* __restrict__ weights, uint32_t* 
         if (live && f > 0.f) code = (int)fminf(fmaxf(rintf(__fdiv_rn(w[c0 + c], f)), -8.f), 7.f);
         word |= ((uint32_t)(code + 8) & 15u) << (4 * ql_nibble(c));
       }
-      words[((long long)mt * s.kblocks + kb) * 128 + ql_word(nl, g, tig)] = word;
+      *reinterpret_cast<uint32_t*>(packed + ql_word_at(s, n, grp * s.group + c0)) = word;
     }
-    packed_scales[((long long)mt * s.sgroups + grp) * 16 + (nl & 7) * 2 + (nl >> 3)] = scale;
+    *reinterpret_cast<bf16*>(packed + ql_scale_at(s, n, grp * s.group)) = scale;
   }
 }
 
-__global__ void ql_dequantize_kernel(const uint32_t* __restrict__ words, const bf16* __restrict__ packed_scales, float* __restrict__ weights, QlShape s) {
+__device__ __forceinline__ float ql_weight(const unsigned char* packed, const QlShape& s, int n, int k) {
+  const uint32_t w = *reinterpret_cast<const uint32_t*>(packed + ql_word_at(s, n, k & ~7));
+  return (float)((int)((w >> (4 * ql_nibble(k))) & 15u) - 8) * __bfloat162float(*reinterpret_cast<const bf16*>(packed + ql_scale_at(s, n, k)));
+}
+__global__ void ql_dequantize_kernel(const unsigned char* __restrict__ packed, float* __restrict__ weights, QlShape s) {
   const long long total = (long long)s.d_out * s.d_in;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
-    const int n = (int)(i / s.d_in), k = (int)(i - (long long)n * s.d_in), mt = n >> 4, nl = n & 15;
-    const uint32_t w = words[((long long)mt * s.kblocks + (k >> 6)) * 128 + ql_word(nl, (k >> 5) & 1, (k >> 3) & 3)];
-    const float code = (float)((int)((w >> (4 * ql_nibble(k))) & 15u) - 8);
-    weights[i] = code * __bfloat162float(packed_scales[((long long)mt * s.sgroups + k / s.group) * 16 + (nl & 7) * 2 + (nl >> 3)]);
-  }
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x)
+    weights[i] = ql_weight(packed, s, (int)(i / s.d_in), (int)(i % s.d_in));
 }
 
 // ---- the product ----
-__device__ __forceinline__ void ql_mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+__device__ __forceinline__ void ql_mma_bf16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// codes i and i + 4 of a word as two bf16 numbers, -8 .. 7
+__device__ __forceinline__ void ql_mma_e4m3(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ql_copy16(uint32_t smem, const void* gmem) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
+}
+// codes i and i + 4 of a word as raw bf16 numbers, of weight 16 where i is odd
 template <int I>
-__device__ __forceinline__ uint32_t ql_pair(uint32_t w) {
-  const uint32_t v = ((w >> (4 * I)) & 0x000f000fu) | 0x43004300u;
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), __float2bfloat162_rn(136.f));
+__device__ __forceinline__ uint32_t ql_raw(uint32_t w) { return (I < 2 ? w : w >> 8) & (I & 1 ? 0x00f000f0u : 0x000f000fu); }
+
+// ... less 8 (or 128): the codes themselves
+template <int I>
+__device__ __forceinline__ uint32_t ql_signed(uint32_t w) {
+  const uint32_t v = ql_raw<I>(w), eight = I & 1 ? 0x00800080u : 0x00080008u;
+  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&eight));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-template <typename T> struct QlPieces { static constexpr int N = 1; };
-template <> struct QlPieces<float> { static constexpr int N = 3; };
 
+__device__ __forceinline__ bool ql_finite(float x) { return fabsf(x) <= 3.4028234663852886e38f; }
 // An f32 number as three bf16 numbers that add up to it, each the leading 8 bits of what is left.
-__device__ __forceinline__ void ql_split(float x, uint16_t* p) {
-  if (!(fabsf(x) <= 3.4028234663852886e38f)) {
-    p[0] = x != x ? 0x7fc0 : (uint16_t)(__float_as_uint(x) >> 16);
+__device__ __forceinline__ void ql_split(float x, uint32_t* p) {
+  if (!ql_finite(x)) {
+    p[0] = x != x ? 0x7fc0u : __float_as_uint(x) >> 16;
     p[1] = p[2] = 0;
     return;
   }
 #pragma unroll
   for (int i = 0; i < 3; ++i) {
     const uint32_t top = __float_as_uint(x) & 0xffff0000u;
-    p[i] = (uint16_t)(top >> 16);
+    p[i] = top >> 16;
     x -= __uint_as_float(top);
   }
 }
+template <typename T> __device__ __forceinline__ void ql_load8(const T* p, float* f);
+template <> __device__ __forceinline__ void ql_load8<float>(const float* p, float* f) {
+  *reinterpret_cast<float4*>(f) = __ldg(reinterpret_cast<const float4*>(p));
+  *reinterpret_cast<float4*>(f + 4) = __ldg(reinterpret_cast<const float4*>(p) + 1);
+}
+template <> __device__ __forceinline__ void ql_load8<bf16>(const bf16* p, float* f) {
+  const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(w[i] << 16);
+    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+// two f32 numbers as e4m3, the first one in the low byte
+__device__ __forceinline__ uint32_t ql_e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float2 ql_from_e4m3x2(uint32_t v) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)v));
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
 
-// Shared memory: the activations of a chunk of the reduction, [piece][row][chunk * 64 + 32] bf16 (the 64 extra bytes a row keep the 16-byte
-// loads of a warp off each other's banks), then the warps' partial sums in the same place.
-template <typename T, int NT, int SPB>
-__global__ void __launch_bounds__(QL_THREADS, NT <= 2 ? 2 : 1)
-q4_linear_kernel(const T* __restrict__ x, long long ld_x, const uint4* __restrict__ codes, const uint32_t* __restrict__ scales, T* __restrict__ y,
-                 long long ld_y, int rows_total, QlShape s, int wk_count, int cluster, int chunk) {
-  constexpr int P = QlPieces<T>::N, MT = QL_MT, U = QL_AHEAD;
-  extern __shared__ __align__(16) unsigned char ql_sm[];
+enum { QL_BF16 = 0, QL_E4M3 = 1 };
+template <typename T> struct QlPieces { static constexpr int N = 1; };
+template <> struct QlPieces<float> { static constexpr int N = 3; };
+
+// How a launch cuts the product, and where things lie in shared memory: factors, marks and flags of the rows first; then the starts of the
+// group sums [group][NT * 8] f32; the activations [piece][row][2 bytes a channel, and 64 that keep the 16-byte loads of a warp off each
+// other's banks]; the warps' rings; the partial sums [buffer][wk][row][outputs of the tile] f32.
+struct QlPlan {
+  int warps, wk, cluster;              // warps of a CTA, those of them along the reduction; CTAs along it
+  int tiles, passes, clusters;         // tiles of outputs; passes over the rows; clusters that share the tiles of a pass
+  int slice, per_pass, stages, buffers;   // units of the reduction per CTA, at most; rows per pass; units in a ring; buffers of partial sums
+  int starts, acts, rings, sums, bytes;
+};
+constexpr int QL_FRONT = 3 * QL_ROWS * 4;
+
+// grid: (clusters * passes) * cluster, the passes over the same tiles next to each other
+template <typename T, int MODE, int NT, int GROUP>
+__global__ void __launch_bounds__(QL_MAX_WARPS * 32)
+q4_linear_kernel(const T* __restrict__ x, long long ld_x, const unsigned char* __restrict__ packed, T* __restrict__ y, long long ld_y, int rows_total,
+                 QlShape s, QlPlan plan) {
+  using U = QlUnit<GROUP>;
+  constexpr int P = MODE == QL_E4M3 ? 1 : QlPieces<T>::N, SUBS = GROUP / 32, PER_UNIT = U::CHANNELS / GROUP;
+  extern __shared__ __align__(128) unsigned char ql_sm[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
-  const int wn_count = QL_WARPS / wk_count, wk = warp % wk_count, wn = warp / wk_count;
-  const int tile = blockIdx.x / cluster, rank = blockIdx.x - tile * cluster;
-  const int mt0 = (tile * wn_count + wn) * MT;
-  const bool live = mt0 < s.mtiles;                  // mtiles is a multiple of MT
-  const int row0 = blockIdx.y * QL_ROWS, rows = min(rows_total - row0, NT * 8);
-  const int kbeg = (int)((long long)s.kblocks * rank / cluster), kend = (int)((long long)s.kblocks * (rank + 1) / cluster);
-  const int pitch = chunk * 128 + 64, plane = NT * 8 * pitch;        // bytes
-  const uint4* cw = codes + (long long)mt0 * s.kblocks * 32 + lane;
-  const uint32_t* sw = scales + (long long)mt0 * s.sgroups * 8 + gid;
-  const int per_group = s.group == 128 ? 1 : 0;      // shift from a 64-channel block to its scale (SPB == 1)
+  const int threads = blockDim.x, wk_count = plan.wk, wn_count = plan.warps / wk_count, wk = warp % wk_count, wn = warp / wk_count;
+  const int cluster = plan.cluster, rank = blockIdx.x % cluster, pass = blockIdx.x / cluster % plan.passes, tile0 = blockIdx.x / cluster / plan.passes;
+  const int row0 = pass * plan.per_pass, rows = min(rows_total - row0, plan.per_pass);
+  const int ubeg = (int)((long long)s.units * rank / cluster), uend = (int)((long long)s.units * (rank + 1) / cluster);
+  const int k0 = ubeg * U::CHANNELS, channels = (uend - ubeg) * U::CHANNELS;
+  const int pitch = plan.slice * U::CHANNELS * 2 + 64, plane = rows * pitch;
+  float* factor = reinterpret_cast<float*>(ql_sm);                // what a row's sums are multiplied with in the end
+  int* mark = reinterpret_cast<int*>(ql_sm) + QL_ROWS;            // e4m3: bits of the largest finite magnitude; bf16: one above QL_LARGE is there
+  int* odd = mark + QL_ROWS;                                      // something infinite or NaN is there
+  float* start = reinterpret_cast<float*>(ql_sm + plan.starts);
+  unsigned char* acts = ql_sm + plan.acts;
 
-  float acc[MT][NT][4];
+  // ---- the warp's units: of the tiles tile0, tile0 + clusters, .. those from ubeg + wk on in steps of wk_count ----
+  const int first = ubeg + wk;
+  unsigned char* ring = ql_sm + plan.rings + warp * (plan.stages * U::BYTES);
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
+  int next_tile = first < uend ? tile0 : plan.tiles, next_unit = first, next_stage = 0, stage = 0;
+  auto issue = [&] {
+    const int pair = next_tile * wn_count + wn;
+    if (next_tile < plan.tiles && pair < s.pairs) {
+      const unsigned char* src = packed + ((long long)pair * s.units + next_unit) * U::BYTES + lane * 16;
+      const uint32_t dst = ring_at + next_stage * U::BYTES;
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int n = 0; n < NT; ++n) acc[m][n][0] = acc[m][n][1] = acc[m][n][2] = acc[m][n][3] = 0.f;
-
-  uint4 w[U][MT];
-  uint32_t sc[U][MT][SPB];
-  auto fetch = [&](int u, int kb) {
-    if (live && kb < kend) {
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        w[u][m] = __ldg(cw + ((long long)m * s.kblocks + kb) * 32);
-#pragma unroll
-        for (int g = 0; g < SPB; ++g)
-          sc[u][m][g] = __ldg(sw + ((long long)m * s.sgroups + (SPB == 2 ? 2 * kb + g : kb >> per_group)) * 8);
-      }
+      for (int i = 0; i < U::CODES; i += 512) ql_copy16(dst + i, src + i);
+      if (lane < U::SCALES * 4) ql_copy16(dst + U::CODES, src + U::CODES);
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    next_unit += wk_count;
+    if (next_unit >= uend) { next_unit = first; next_tile += plan.clusters; }
+    next_stage = next_stage + 1 == plan.stages ? 0 : next_stage + 1;
   };
-#pragma unroll
-  for (int u = 0; u < U; ++u) fetch(u, kbeg + wk + u * wk_count);
+  for (int i = 0; i < plan.stages - 1; ++i) issue();
 
-  for (int c0 = kbeg; c0 < kend; c0 += chunk) {      // chunk is a multiple of U * wk_count
-    __syncthreads();                                 // the chunk before has been used
-    {
-      const int blocks = min(chunk, kend - c0), parts = blocks * 8;            // 8 channels at a time
-      for (int i = threadIdx.x; i < rows * parts; i += QL_THREADS) {
-        const int r = i / parts, c = i - r * parts, k = c0 * 64 + c * 8;
-        const T* src = x + (row0 + r) * ld_x + k;
-        unsigned char* dst = ql_sm + r * pitch + c * 16;
-        if constexpr (P == 1) {
-          *reinterpret_cast<uint4*>(dst) = k < s.d_in ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
-        } else {
-          float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-          if (k < s.d_in) {
-            *reinterpret_cast<float4*>(f) = __ldg(reinterpret_cast<const float4*>(src));
-            *reinterpret_cast<float4*>(f + 4) = __ldg(reinterpret_cast<const float4*>(src) + 1);
-          }
-          uint16_t p[8][3];
+  // ---- the activations of the slice, eight channels of a row at a time ----
+  const int parts = channels / 8, work = rows * parts;
+  for (int i = threadIdx.x; i < 2 * QL_ROWS; i += threads) mark[i] = 0;
+  __syncthreads();
+  if constexpr (MODE == QL_E4M3) {
+    for (int i = threadIdx.x; i < work; i += threads) {
+      const int r = i / parts, k = k0 + (i - r * parts) * 8;
+      if (k >= s.d_in) continue;
+      float f[8];
+      ql_load8<T>(x + (row0 + r) * ld_x + k, f);
+      uint32_t top = 0;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) ql_split(f[j], p[j]);
-#pragma unroll
-          for (int q = 0; q < 3; ++q)
-            *reinterpret_cast<uint4*>(dst + q * plane) =
-                make_uint4(p[0][q] | (uint32_t)p[1][q] << 16, p[2][q] | (uint32_t)p[3][q] << 16, p[4][q] | (uint32_t)p[5][q] << 16,
-                           p[6][q] | (uint32_t)p[7][q] << 16);
-        }
-      }
+      for (int j = 0; j < 8; ++j) top = max(top, ql_finite(f[j]) ? __float_as_uint(f[j]) & 0x7fffffffu : 0u);
+      atomicMax(mark + r, (int)top);
     }
     __syncthreads();
-    if (!live) continue;
-    const int end = min(kend, c0 + chunk);
-    for (int kb0 = c0 + wk; kb0 < end; kb0 += U * wk_count) {
+  }
+  for (int again = 0;; ++again) {
+    bool large = false;
+    for (int i0 = warp * 32; i0 < work; i0 += threads) {
+      const int i = i0 + lane, r = min(i / parts, rows - 1), c = (i - r * parts) * 8, k = k0 + c;
+      float f[8], sum = 0.f;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int kb = kb0 + u * wk_count;
-        if (kb < end) {
-          const unsigned char* xs = ql_sm + gid * pitch + (kb - c0) * 128 + tig * 16;
+      for (int j = 0; j < 8; ++j) f[j] = 0.f;
+      if (i < work && k < s.d_in) ql_load8<T>(x + (row0 + r) * ld_x + k, f);
+      int up = QL_UP;
+      if constexpr (MODE == QL_E4M3) up = min(134 - (mark[r] >> 23), 120);         // the row's largest to 128 .. 256
+      else if (again && mark[r]) up = QL_UP - QL_DOWN;
+      const float by = __uint_as_float((uint32_t)(up + 127) << 23);
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            uint32_t a[MT][2][4];
+      for (int j = 0; j < 8; ++j) {
+        if (!ql_finite(f[j])) { odd[r] = 1; f[j] = 0.f; }
+        if (MODE == QL_BF16 && !again && fabsf(f[j]) > QL_LARGE) { mark[r] = 1; large = true; }
+        f[j] *= by;
+        sum += f[j] * ql_pow2(MODE == QL_E4M3 ? 0 : -64);         // a sum of numbers up to 2^127
+      }
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-              const uint32_t lo = g ? w[u][m].z : w[u][m].x, hi = g ? w[u][m].w : w[u][m].y;
-              a[m][0][0] = ql_pair<0>(lo); a[m][0][1] = ql_pair<0>(hi); a[m][0][2] = ql_pair<1>(lo); a[m][0][3] = ql_pair<1>(hi);
-              a[m][1][0] = ql_pair<2>(lo); a[m][1][1] = ql_pair<2>(hi); a[m][1][2] = ql_pair<3>(lo); a[m][1][3] = ql_pair<3>(hi);
-            }
+      for (int o = 1; o < GROUP / 8; o *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (i >= work) continue;
+      if (P == 1 && (c & (GROUP - 1)) == 0) start[(c / GROUP) * (NT * 8) + r] = sum * ql_pow2(MODE == QL_E4M3 ? -9 : 64 - QL_RAW) * -8.f;
+      unsigned char* dst = acts + r * pitch + c * 2;
+      if constexpr (MODE == QL_E4M3) {
+        // channels in the order of a word's low nibbles, then of its high ones; what the first e4m3 number leaves is the second
+        uint32_t hi[4], lo[4];
+        const int at[8] = {0, 4, 1, 5, 2, 6, 3, 7};
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              float part[MT][4];
-#pragma unroll
-              for (int m = 0; m < MT; ++m) part[m][0] = part[m][1] = part[m][2] = part[m][3] = 0.f;
-#pragma unroll
-              for (int q = 0; q < P; ++q) {
-                const uint4 b = *reinterpret_cast<const uint4*>(xs + q * plane + n * 8 * pitch + g * 64);
-#pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                  ql_mma(part[m], a[m][0], b.x, b.y);
-                  ql_mma(part[m], a[m][1], b.z, b.w);
-                }
-              }
-#pragma unroll
-              for (int m = 0; m < MT; ++m) {
-                const uint32_t v = sc[u][m][SPB == 2 ? g : 0];
-                const float s0 = __uint_as_float(v << 16), s1 = __uint_as_float(v & 0xffff0000u);
-                acc[m][n][0] = fmaf(s0, part[m][0], acc[m][n][0]);
-                acc[m][n][1] = fmaf(s0, part[m][1], acc[m][n][1]);
-                acc[m][n][2] = fmaf(s1, part[m][2], acc[m][n][2]);
-                acc[m][n][3] = fmaf(s1, part[m][3], acc[m][n][3]);
-              }
-            }
-          }
+        for (int j = 0; j < 4; ++j) {
+          const float a = f[at[2 * j]], b = f[at[2 * j + 1]];
+          hi[j] = ql_e4m3x2(a, b);
+          const float2 h = ql_from_e4m3x2(hi[j]);
+          lo[j] = ql_e4m3x2(a - h.x, b - h.y);
         }
-        fetch(u, kb + U * wk_count);
+        *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0] | hi[1] << 16, hi[2] | hi[3] << 16, lo[0] | lo[1] << 16, lo[2] | lo[3] << 16);
+      } else {
+        uint32_t p[8][3];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (j & 2) f[j] *= 0.0625f;                             // its code weighs 16
+          if constexpr (P == 1) p[j][0] = __float_as_uint(f[j]) >> 16;
+          else ql_split(f[j], p[j]);
+        }
+#pragma unroll
+        for (int q = 0; q < P; ++q)
+          *reinterpret_cast<uint4*>(dst + q * plane) = make_uint4(p[0][q] | p[1][q] << 16, p[2][q] | p[3][q] << 16, p[4][q] | p[5][q] << 16, p[6][q] | p[7][q] << 16);
       }
     }
+    if (MODE == QL_E4M3 || again || !__syncthreads_or(large)) break;
   }
-
-  // ---- add the partial sums of the warps and of the cluster's CTAs ----
-  constexpr int TN = MT * 16;
-  float* red = reinterpret_cast<float*>(ql_sm);      // [wk][row][wn * TN + output]
-  const int width = wn_count * TN;
   __syncthreads();
+  if (threadIdx.x < rows) {
+    const int m = mark[threadIdx.x];
+    factor[threadIdx.x] = MODE == QL_E4M3 ? __uint_as_float((uint32_t)(127 - min(134 - (m >> 23), 120)) << 23) : m ? ql_pow2(QL_DOWN) : 1.f;
+  }
+  bool any_odd = false;
+  for (int r = 0; r < rows; ++r) any_odd |= odd[r] != 0;
+  __syncthreads();
+
+  const unsigned char* mine[NT];                                  // rows past the last one repeat it; nobody looks at their sums
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+  for (int n = 0; n < NT; ++n) mine[n] = acts + min(n * 8 + gid, rows - 1) * pitch + tig * 16;
+  const int width = wn_count * 32;
+  float* red = reinterpret_cast<float*>(ql_sm + plan.sums);
+  const int other = plan.buffers == 2 ? wk_count * rows * width : 0;
+  int turn = 0;
+  cg::cluster_group cl = cg::this_cluster();
+
+  for (int tile = tile0; tile < plan.tiles; tile += plan.clusters) {
+    const bool live = tile * wn_count + wn < s.pairs;
+    float acc[2][NT][4];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) acc[m][n][0] = acc[m][n][1] = acc[m][n][2] = acc[m][n][3] = 0.f;
+    for (int unit = first; unit < uend; unit += wk_count) {
+      if (plan.stages == 3) asm volatile("cp.async.wait_group 1;" ::: "memory");
+      else if (plan.stages == 4) asm volatile("cp.async.wait_group 2;" ::: "memory");
+      else asm volatile("cp.async.wait_group 4;" ::: "memory");
+      __syncwarp();                                               // the unit has landed for every lane, and the one before is used up
+      issue();
+      const unsigned char* at = ring + stage * U::BYTES;
+      stage = stage + 1 == plan.stages ? 0 : stage + 1;
+      if (!live) continue;
+      const int c0 = (unit - ubeg) * U::CHANNELS;
+#pragma unroll
+      for (int grp = 0; grp < PER_UNIT; ++grp) {
+        float part[2][NT][4];
+        auto scaled = [&](int grp) {
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            const uint32_t v = *reinterpret_cast<const uint32_t*>(at + U::CODES + (m * U::SCALES + grp) * 32 + gid * 4);
+            const float s0 = __uint_as_float(v << 16), s1 = __uint_as_float(v & 0xffff0000u);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              acc[m][n][0] = fmaf(s0, part[m][n][0], acc[m][n][0]);
+              acc[m][n][1] = fmaf(s0, part[m][n][1], acc[m][n][1]);
+              acc[m][n][2] = fmaf(s1, part[m][n][2], acc[m][n][2]);
+              acc[m][n][3] = fmaf(s1, part[m][n][3], acc[m][n][3]);
+            }
+          }
+        };
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float2 v = make_float2(0.f, 0.f);
+          if constexpr (P == 1) v = *reinterpret_cast<const float2*>(start + (c0 / GROUP + grp) * (NT * 8) + n * 8 + 2 * tig);
+#pragma unroll
+          for (int m = 0; m < 2; ++m) { part[m][n][0] = part[m][n][2] = v.x; part[m][n][1] = part[m][n][3] = v.y; }
+        }
+#pragma unroll
+        for (int sub = 0; sub < SUBS; ++sub) {
+          const int g32 = grp * SUBS + sub, block = g32 >> 1, g = g32 & 1;
+          uint32_t lo[2], hi[2];
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            const uint2 w = *reinterpret_cast<const uint2*>(at + (m * U::BLOCKS + block) * 512 + lane * 16 + g * 8);
+            lo[m] = w.x; hi[m] = w.y;
+          }
+          const int off = (c0 + g32 * 32) * 2;
+          if constexpr (MODE == QL_E4M3) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const uint4 b = *reinterpret_cast<const uint4*>(mine[n] + off);
+#pragma unroll
+              for (int m = 0; m < 2; ++m) {
+                const uint32_t a0 = lo[m] & 0x0f0f0f0fu, a1 = hi[m] & 0x0f0f0f0fu, a2 = (lo[m] >> 4) & 0x0f0f0f0fu, a3 = (hi[m] >> 4) & 0x0f0f0f0fu;
+                ql_mma_e4m3(part[m][n], a0, a1, a2, a3, b.x, b.y);
+                ql_mma_e4m3(part[m][n], a0, a1, a2, a3, b.z, b.w);
+              }
+            }
+          } else {
+            uint32_t a[2][8];
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+              if constexpr (P == 1) {
+                a[m][0] = ql_raw<0>(lo[m]); a[m][1] = ql_raw<0>(hi[m]); a[m][2] = ql_raw<1>(lo[m]); a[m][3] = ql_raw<1>(hi[m]);
+                a[m][4] = ql_raw<2>(lo[m]); a[m][5] = ql_raw<2>(hi[m]); a[m][6] = ql_raw<3>(lo[m]); a[m][7] = ql_raw<3>(hi[m]);
+              } else {
+                a[m][0] = ql_signed<0>(lo[m]); a[m][1] = ql_signed<0>(hi[m]); a[m][2] = ql_signed<1>(lo[m]); a[m][3] = ql_signed<1>(hi[m]);
+                a[m][4] = ql_signed<2>(lo[m]); a[m][5] = ql_signed<2>(hi[m]); a[m][6] = ql_signed<3>(lo[m]); a[m][7] = ql_signed<3>(hi[m]);
+              }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int q = 0; q < P; ++q) {
+                const uint4 b = *reinterpret_cast<const uint4*>(mine[n] + q * plane + off);
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                  ql_mma_bf16(part[m][n], a[m][0], a[m][1], a[m][2], a[m][3], b.x, b.y);
+                  ql_mma_bf16(part[m][n], a[m][4], a[m][5], a[m][6], a[m][7], b.z, b.w);
+                }
+              }
+          }
+          if constexpr (P > 1) {
+            // the tensor cores cut sums off where f32 arithmetic rounds them: short chains only
+            scaled(grp);
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+              for (int n = 0; n < NT; ++n) part[m][n][0] = part[m][n][1] = part[m][n][2] = part[m][n][3] = 0.f;
+          }
+        }
+        if constexpr (P == 1) scaled(grp);
+      }
+    }
+
+    // ---- add up the warps and the cluster, always in the same order ----
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        red[(wk * NT * 8 + n * 8 + 2 * tig + (e & 1)) * width + wn * TN + m * 16 + gid + 8 * (e >> 1)] = acc[m][n][e];
-  cg::cluster_group cl = cg::this_cluster();
-  if (cluster > 1) cl.sync(); else __syncthreads();
-  const int n0 = tile * width;
-  for (int i = rank * QL_THREADS + threadIdx.x; i < rows * width; i += cluster * QL_THREADS) {
-    const int r = i / width, n = i - r * width;
-    if (n0 + n >= s.d_out) continue;
-    float v = 0.f;
-    for (int c = 0; c < cluster; ++c) {
-      const float* part = cluster > 1 ? cl.map_shared_rank(red, c) : red;
-      for (int k = 0; k < wk_count; ++k) v += part[(k * NT * 8 + r) * width + n];
+      for (int e = 0; e < 2; ++e) {
+        const int r = n * 8 + 2 * tig + e;
+        if (r >= rows) continue;
+        const float by = factor[r];
+        float* dst = red + (wk * rows + r) * width + wn * 32 + gid;
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          dst[16 * m] = acc[m][n][e] * ql_pow2(MODE == QL_E4M3 ? 9 : QL_RAW - QL_UP) * by;
+          dst[16 * m + 8] = acc[m][n][2 + e] * ql_pow2(MODE == QL_E4M3 ? 9 : QL_RAW - QL_UP) * by;
+        }
+      }
+    const int n0 = tile * width;
+    if (any_odd) {
+      // infinities and NaN took part as 0 above (an infinity against a sum's start would be NaN): add what they really give
+      __syncthreads();
+      for (int i = threadIdx.x; i < rows * width; i += threads) {
+        const int r = i / width, n = n0 + i % width;
+        if (!odd[r] || n >= s.d_out) continue;
+        float v = 0.f;
+        for (int k = k0; k < min(k0 + channels, s.d_in); ++k) {
+          const float f = to_f32<T>(x[(row0 + r) * ld_x + k]);
+          if (!ql_finite(f)) v += f * ql_weight(packed, s, n, k);
+        }
+        red[i] += v;
+      }
     }
-    y[(row0 + r) * ld_y + n0 + n] = from_f32<T>(v);
+    if (cluster > 1) cl.sync(); else __syncthreads();
+    const int count = cluster * wk_count;
+    for (int i = rank * threads + threadIdx.x; i < rows * width / 4; i += cluster * threads) {
+      const int r = i * 4 / width, n = i * 4 % width;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+      for (int j = 0; j < count; ++j) {
+        const int from = j / wk_count, w = j - from * wk_count;
+        const float* src = (cluster > 1 ? cl.map_shared_rank(red, from) : red) + w * rows * width + i * 4;
+        const float4 p = *reinterpret_cast<const float4*>(src);
+        v.x += p.x; v.y += p.y; v.z += p.z; v.w += p.w;
+      }
+      const float out[4] = {v.x, v.y, v.z, v.w};
+      T* dst = y + (row0 + r) * ld_y + n0 + n;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (n0 + n + j < s.d_out) dst[j] = from_f32<T>(out[j]);
+    }
+    // with two buffers the next tile writes to the other one, and its barrier comes before this one is written again
+    if (plan.buffers == 1) { if (cluster > 1) cl.sync(); else __syncthreads(); }
+    red += turn ? -other : other;
+    turn ^= 1;
   }
-  if (cluster > 1) cl.sync();                        // nobody leaves while its sums are being read
+  if (cluster > 1) cl.sync();                                     // nobody leaves while its sums are being read
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 int ql_fail(char* msg, int len, int code, const char* text) {
@@ -307,60 +514,107 @@ int ql_fail(char* msg, int len, int code, const char* text) {
 }
 
 bool ql_sizes_ok(int d_out, int d_in, int group) {
-  return d_out > 0 && d_in > 0 && (group == 32 || group == 64 || group == 128) && d_in % group == 0 && d_in <= (1 << 24) && d_out <= (1 << 28);
+  return d_out > 0 && d_in > 0 && (group == 32 || group == 64 || group == 128) && d_in % group == 0 && d_in <= QL_MAX_IN && d_out <= (1 << 28);
 }
 
-template <typename T, int NT, int SPB>
+// How to cut a product with `live` <= NT * 8 rows a pass.  False: the activations of a pass do not fit.
+template <typename T, int MODE, int NT, int GROUP>
+bool ql_plan(const QlShape& s, int rows, int live, QlPlan* out) {
+  using U = QlUnit<GROUP>;
+  constexpr int P = MODE == QL_E4M3 ? 1 : QlPieces<T>::N;
+  QlPlan p{};
+  p.per_pass = live;
+  p.passes = (rows + live - 1) / live;
+  auto up = [](int v) { return (v + 127) / 128 * 128; };
+  // where things lie, with as many units in flight and as many buffers as fit
+  auto fits = [&](int limit) {
+    p.starts = QL_FRONT;
+    p.acts = p.starts + up(p.slice * U::CHANNELS / GROUP * NT * 8 * 4);
+    p.rings = p.acts + up(P * live * (p.slice * U::CHANNELS * 2 + 64));
+    const int sums = live * 32 * p.warps * 4;
+    for (p.buffers = 2; p.buffers >= 1; --p.buffers)
+      for (p.stages = 6; p.stages >= 3; p.stages -= p.stages == 6 ? 2 : 1) {
+        p.sums = p.rings + up(p.warps * p.stages * U::BYTES);
+        p.bytes = p.sums + p.buffers * sums;
+        if (p.bytes <= limit) return true;
+      }
+    return false;
+  };
+  // Two CTAs of 8 warps on an SM, or one of 16 where the activations take more than a half.  Warps along the reduction: each should have
+  // several units of a tile (joining a tile costs about 2.5 units' time), and the tiles should come out even.
+  auto shape = [&](int warps, int limit, int ctas) {
+    double best = -1;
+    QlPlan keep{};
+    for (int cluster = 1; cluster <= QL_MAX_CLUSTER; cluster *= 2) {
+      p.warps = warps;
+      p.cluster = cluster;
+      p.slice = (s.units + cluster - 1) / cluster;
+      if (cluster > 1 && p.slice * cluster > s.units + cluster - 1) break;
+      if (cluster > 1 && p.slice < 2) break;
+      for (p.wk = 1; p.wk <= warps && p.wk <= p.slice; p.wk *= 2) {
+        p.tiles = (s.pairs + warps / p.wk - 1) / (warps / p.wk);
+        p.clusters = std::min(p.tiles, std::max(1, ctas / (cluster * p.passes)));
+        const int rounds = (p.tiles + p.clusters - 1) / p.clusters, each = (p.slice + p.wk - 1) / p.wk;
+        // units' time from start to end: filling the activations, the tiles, joining them (a cluster's join takes longer)
+        const double busy = std::min(1.0, (double)p.clusters * cluster * p.passes * warps / (148.0 * 16));
+        const double time = rounds * (each * std::max(busy, 0.35) + (cluster > 1 ? 6.0 : 2.5) * std::max(busy, 0.5));
+        if ((best < 0 || time < best) && fits(limit)) { best = time; keep = p; }
+      }
+    }
+    if (best < 0) return false;
+    *out = keep;
+    fits(limit);
+    return true;
+  };
+  return shape(8, 113 * 1024, 2 * 148) || shape(16, 227 * 1024, 148);
+}
+
+template <typename T, int MODE, int NT, int GROUP>
 cudaError_t ql_launch(const T* x, long long ld_x, const void* packed, T* y, long long ld_y, int rows, const QlShape& s, cudaStream_t st) {
-  constexpr int P = QlPieces<T>::N;
-  // Warps along the reduction: many for few rows (less to join), few for many rows (their activations fill shared memory).
-  int wk = NT == 1 ? 4 : NT == 2 ? 2 : 1;
-  while (wk > 1 && s.kblocks < wk) wk /= 2;
-  const int tiles = (s.mtiles / QL_MT + QL_WARPS / wk - 1) / (QL_WARPS / wk);
-  int cluster = 1;
-  while (cluster < QL_MAX_CLUSTER && tiles * cluster < 2 * 148 && s.kblocks >= cluster * 2 * wk * 2) cluster *= 2;
-  const int slice = (s.kblocks + cluster - 1) / cluster, unit = QL_AHEAD * wk;
-  // the chunk of the reduction whose activations are in shared memory at a time
-  int chunk = (slice + unit - 1) / unit * unit;
-  while (chunk > unit && P * NT * 8 * (chunk * 128 + 64) > QL_SMEM) chunk -= unit;
-  const int smem = std::max(P * NT * 8 * (chunk * 128 + 64), QL_WARPS * QL_MT * 16 * NT * 8 * 4);
-  auto kernel = q4_linear_kernel<T, NT, SPB>;
+  QlPlan plan;
+  int live = std::min(rows, NT * 8);
+  while (!ql_plan<T, MODE, NT, GROUP>(s, rows, live, &plan)) {
+    if (live == 1) return cudaErrorInvalidConfiguration;   // not reached: d_in is at most QL_MAX_IN
+    live = (live + 1) / 2;
+  }
+  auto kernel = q4_linear_kernel<T, MODE, NT, GROUP>;
   static std::atomic<unsigned long long> raised{0};   // devices on which the kernel's shared-memory limit has been raised
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
   if (e != cudaSuccess) return e;
   const unsigned long long bit = 1ull << (device & 63);
   if (!(raised.load(std::memory_order_relaxed) & bit)) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, QL_SMEM_MAX);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
     if (e != cudaSuccess) return e;
     raised.fetch_or(bit, std::memory_order_relaxed);
   }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(tiles * cluster), (unsigned)((rows + QL_ROWS - 1) / QL_ROWS));
-  cfg.blockDim = dim3(QL_THREADS);
-  cfg.dynamicSmemBytes = smem;
+  cfg.gridDim = dim3((unsigned)(plan.clusters * plan.passes * plan.cluster));
+  cfg.blockDim = dim3(plan.warps * 32);
+  cfg.dynamicSmemBytes = plan.bytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const uint4* codes = (const uint4*)packed;
-  const uint32_t* scales = (const uint32_t*)((const char*)packed + ql_code_bytes(s));
+  attr[0].val.clusterDim.x = plan.cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  if (plan.cluster > 1) { cfg.attrs = attr; cfg.numAttrs = 1; }
   count_launch();
-  return cudaLaunchKernelEx(&cfg, kernel, x, ld_x, codes, scales, y, ld_y, rows, s, wk, cluster, chunk);
+  return cudaLaunchKernelEx(&cfg, kernel, x, ld_x, (const unsigned char*)packed, y, ld_y, rows, s, plan);
 }
 
-template <typename T>
+template <typename T, int GROUP>
 cudaError_t ql_dispatch(const void* x, long long ld_x, const void* packed, void* y, long long ld_y, int rows, const QlShape& s, cudaStream_t st) {
   const T* xt = (const T*)x;
   T* yt = (T*)y;
-#define QL_GO(NT) (s.group == 32 ? ql_launch<T, NT, 2>(xt, ld_x, packed, yt, ld_y, rows, s, st) : ql_launch<T, NT, 1>(xt, ld_x, packed, yt, ld_y, rows, s, st))
-  if (rows <= 8) return QL_GO(1);
-  if (rows <= 16) return QL_GO(2);
-  if (rows <= 32) return QL_GO(4);
-  return QL_GO(8);
-#undef QL_GO
+  if (rows <= 8) return ql_launch<T, QL_BF16, 1, GROUP>(xt, ld_x, packed, yt, ld_y, rows, s, st);
+  if constexpr (sizeof(T) == 2)
+    if (rows > 16) return ql_launch<T, QL_E4M3, 2, GROUP>(xt, ld_x, packed, yt, ld_y, rows, s, st);
+  return ql_launch<T, QL_BF16, 2, GROUP>(xt, ld_x, packed, yt, ld_y, rows, s, st);
+}
+template <typename T>
+cudaError_t ql_dispatch(const void* x, long long ld_x, const void* packed, void* y, long long ld_y, int rows, const QlShape& s, cudaStream_t st) {
+  return s.group == 32   ? ql_dispatch<T, 32>(x, ld_x, packed, y, ld_y, rows, s, st)
+         : s.group == 64 ? ql_dispatch<T, 64>(x, ld_x, packed, y, ld_y, rows, s, st)
+                         : ql_dispatch<T, 128>(x, ld_x, packed, y, ld_y, rows, s, st);
 }
 
 int ql_blocks(long long work) { return (int)std::min<long long>((work + 255) / 256, 148 * 16); }
@@ -375,7 +629,7 @@ extern "C" {
 int64_t q4_linear_packed_bytes(int32_t d_out, int32_t d_in, int32_t group) {
   if (!ql_sizes_ok(d_out, d_in, group)) return 0;
   const QlShape s = ql_shape(d_out, d_in, group);
-  return ql_code_bytes(s) + ql_scale_bytes(s);
+  return ql_bytes(s);
 }
 
 #define QL_CHECK(packed)                                                                                                                  \
@@ -391,8 +645,8 @@ int32_t q4_linear_pack(const int8_t* codes, const void* scales, void* packed, in
   QL_CHECK(packed);
   if (!codes || !scales) return ql_fail(message, message_len, MOE_INVALID_INPUT, "InvalidInput: null buffer");
   const QlShape s = ql_shape(d_out, d_in, group);
-  ql_pack_kernel<<<ql_blocks((long long)s.mtiles * (s.kblocks * 128ll + s.sgroups * 16ll)), 256, 0, (cudaStream_t)stream>>>(
-      codes, (const bf16*)scales, (uint32_t*)packed, (bf16*)((char*)packed + ql_code_bytes(s)), s);
+  ql_pack_kernel<<<ql_blocks((long long)s.pairs * 32 * s.units * s.channels / 8), 256, 0, (cudaStream_t)stream>>>(codes, (const bf16*)scales,
+                                                                                                                (unsigned char*)packed, s);
   count_launch();
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? MOE_OK : ql_fail(message, message_len, MOE_CUDA_ERROR, cudaGetErrorString(e));
@@ -403,8 +657,7 @@ int32_t q4_linear_quantize(const float* weights, void* packed, int32_t d_out, in
   QL_CHECK(packed);
   if (!weights) return ql_fail(message, message_len, MOE_INVALID_INPUT, "InvalidInput: null buffer");
   const QlShape s = ql_shape(d_out, d_in, group);
-  ql_quantize_kernel<<<ql_blocks((long long)s.mtiles * 16 * s.sgroups), 256, 0, (cudaStream_t)stream>>>(
-      weights, (uint32_t*)packed, (bf16*)((char*)packed + ql_code_bytes(s)), s);
+  ql_quantize_kernel<<<ql_blocks((long long)s.pairs * 32 * s.units * s.channels / group), 256, 0, (cudaStream_t)stream>>>(weights, (unsigned char*)packed, s);
   count_launch();
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? MOE_OK : ql_fail(message, message_len, MOE_CUDA_ERROR, cudaGetErrorString(e));
@@ -415,8 +668,7 @@ int32_t q4_linear_dequantize(const void* packed, float* weights, int32_t d_out, 
   QL_CHECK(packed);
   if (!weights) return ql_fail(message, message_len, MOE_INVALID_INPUT, "InvalidInput: null buffer");
   const QlShape s = ql_shape(d_out, d_in, group);
-  ql_dequantize_kernel<<<ql_blocks((long long)d_out * d_in), 256, 0, (cudaStream_t)stream>>>(
-      (const uint32_t*)packed, (const bf16*)((const char*)packed + ql_code_bytes(s)), weights, s);
+  ql_dequantize_kernel<<<ql_blocks((long long)d_out * d_in), 256, 0, (cudaStream_t)stream>>>((const unsigned char*)packed, weights, s);
   count_launch();
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? MOE_OK : ql_fail(message, message_len, MOE_CUDA_ERROR, cudaGetErrorString(e));
@@ -428,7 +680,7 @@ int32_t q4_linear_forward(const void* x, int64_t ld_x, const void* packed, void*
     return ql_fail(message, message_len, MOE_INVALID_CONFIG, "InvalidConfig: activations are f32 or bf16");
   QL_CHECK(packed);
   const int elem = precision == MOE_PRECISION_BF16 ? 2 : 4;
-  if (rows < 0 || rows > QL_ROWS * 65535 || ld_x < d_in || ld_y < d_out)
+  if (rows < 0 || rows > 65535 || ld_x < d_in || ld_y < d_out)
     return ql_fail(message, message_len, MOE_INVALID_INPUT, "InvalidInput: rows >= 0, ld_x >= d_in and ld_y >= d_out");
   if (rows == 0) return MOE_OK;
   if (!x || !y) return ql_fail(message, message_len, MOE_INVALID_INPUT, "InvalidInput: null buffer");
