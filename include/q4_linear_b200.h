@@ -5,12 +5,11 @@
  *   y[r, n] = sum_k x[r, k] * w[n, k],    w[n, k] = scale[n, k / group] * code[n, k]
  *
  * code is -8 .. 7, scale a bf16 number, group 32, 64 or 128 input channels; d_in is a multiple of the group and at most 65536, d_out anything.
- * x and y are both f32 (MOE_PRECISION_F32) or both bf16 (MOE_PRECISION_BF16).  Products of codes and activations are exact (in bf16
- * batches of more than 16 rows an activation is kept to 2^-17 of the largest of its row), sums are f32, y is rounded once; the order of the
- * sums depends on the sizes only, so results do not depend on the run.  An infinity or a NaN of x or of a scale appears in the outputs it
- * takes part in.
+ * x and y are both f32 (MOE_PRECISION_F32) or both bf16 (MOE_PRECISION_BF16).  Products of codes and activations are exact, sums are f32,
+ * y is rounded once; the order of the sums depends on the sizes only, so results do not depend on the run.  An infinity or a NaN of x
+ * or of a scale appears in the outputs it takes part in.
  *
- * Meant for decode batches: up to 64 rows (fewer where d_in is very large) read the weights once, more rows read them once for every 64.
+ * Meant for decode batches: 16 rows at a time (fewer where d_in is very large), more rows are passes side by side over the same weights.
  *
  * Stateless: all pointers are device pointers of the current device, owned by the caller; nothing is allocated, no scratch is kept, every
  * call can be captured into a CUDA graph, and calls on different streams do not meet.  Status codes are the moe_status values of

@@ -6,15 +6,14 @@
 // channels of a product may come in any order, the activations' 8 channels are one 16-byte shared load of the B operand.  Two such blocks
 // (32 outputs) and their scales are a unit, which a warp brings into its own ring in shared memory, several units ahead.
 //
-// A code plus 8 needs no conversion.  Bits 0 .. 7 of a bf16 are a number linear in them, bits * 2^-133 (below 128 it is subnormal, and the
-// next binade goes on in the same steps), and bits 0 .. 3 of an e4m3 likewise, bits * 2^-9.  So a code is cut out of its word and is an
-// operand, at weight 1 or, where it comes out four bits further up, 16.  The activations make up for the powers of two, and the 8 that
-// the codes have too much is where the sum of a group starts: -8 times the sum of its activations.
-//   up to 16 rows, or f32:  activations as bf16 numbers, five instructions for eight codes.  Products are exact, and the group's scale is
-//                           applied to its f32 sum.  An f32 activation is three bf16 numbers that add up to it; there the 8 is taken off the
-//                           codes, whose sums then stay small enough for the accuracy of f32.
-//   more bf16 rows:         the tensor cores' time counts, and e4m3 products take a quarter of it: a bf16 activation, scaled so that its row's
-//                           largest is in 128 .. 256, is the sum of two e4m3 numbers (to 2^-17 of the largest), three instructions for eight codes.
+// A code plus 8 needs no conversion: bits 0 .. 7 of a bf16 are a number linear in them, bits * 2^-133 (below 128 it is subnormal, and the
+// next binade goes on in the same steps).  So a code is cut out of its word and is an operand, at weight 1 or, where it comes out four
+// bits further up, 16: five instructions for eight codes.  The activations make up for the powers of two, and the 8 that the codes have
+// too much is where the sum of a group starts: -8 times the sum of its activations.  Products are exact, and the group's scale is applied
+// to its f32 sum.  An f32 activation is three bf16 numbers that add up to it; there the 8 is taken off the codes, whose sums then
+// stay small enough for the accuracy of f32.
+// (e4m3 operands would take three instructions for eight codes, but mma.sync has no e4m3 product of its own here: it costs two bf16 ones
+// and the conversions.)
 //
 // A CTA keeps the activations of up to 16 rows in shared memory and goes through tiles of outputs, weights arriving without a pause from
 // tile to tile; its warps split the reduction of a tile.  More rows are passes side by side, which find the weights in L2.  Where there
@@ -22,7 +21,6 @@
 // the same order: one launch, no workspace.
 
 #include <cooperative_groups.h>
-#include <cuda_fp16.h>
 #include <algorithm>
 #include <atomic>
 #include <cstdio>
@@ -38,7 +36,7 @@ namespace {
 
 constexpr int QL_MAX_WARPS = 16;
 constexpr int QL_ROWS = 16;              // batch rows per pass
-constexpr int QL_MAX_CLUSTER = 8;
+
 constexpr int QL_MAX_IN = 1 << 16;       // a row of f32 activations, cut over a cluster, fits shared memory
 constexpr int QL_RAW = 133;              // bits 0 .. 7 of a bf16 are worth bits * 2^-QL_RAW
 constexpr int QL_UP = 88, QL_DOWN = 96;  // activations times 2^QL_UP, those of a row with one above 2^38 times 2^(QL_UP - QL_DOWN)
@@ -50,41 +48,32 @@ __host__ __device__ constexpr float ql_pow2(int e) {
   return v;
 }
 
-// A unit: 32 outputs and 64 (group 128: 128) channels, codes [2 output blocks][blocks][512 bytes], then scales [2][scales][8][2] bf16.
-template <int GROUP> struct QlUnit {
-  static constexpr int BLOCKS = GROUP == 128 ? 2 : 1, SCALES = GROUP == 32 ? 2 : 1, CODES = 2 * BLOCKS * 512, BYTES = CODES + 2 * SCALES * 32;
-  static constexpr int CHANNELS = 64 * BLOCKS;
-};
+// A unit: 32 outputs and 128 channels, codes [2 output blocks][2 channel blocks][512 bytes], then scales [2][128 / group][8][2] bf16.
+constexpr int QL_CHANNELS = 128, QL_CODES = 2048;
+__host__ __device__ constexpr int ql_unit_bytes(int group) { return QL_CODES + 2 * (QL_CHANNELS / group) * 32; }
 struct QlShape {
-  int d_in, d_out, group, pairs, units, unit_bytes, channels;   // pairs of 16 outputs; units along the reduction
+  int d_in, d_out, group, pairs, units;   // pairs of 16 outputs; units along the reduction
 };
 inline QlShape ql_shape(int d_out, int d_in, int group) {
-  QlShape s;
-  s.d_in = d_in; s.d_out = d_out; s.group = group;
-  s.channels = group == 128 ? 128 : 64;
-  s.unit_bytes = group == 128 ? QlUnit<128>::BYTES : group == 64 ? QlUnit<64>::BYTES : QlUnit<32>::BYTES;
-  s.pairs = (d_out + 31) / 32;
-  s.units = (d_in + s.channels - 1) / s.channels;
-  return s;
+  return QlShape{d_in, d_out, group, (d_out + 31) / 32, (d_in + QL_CHANNELS - 1) / QL_CHANNELS};
 }
-inline long long ql_bytes(const QlShape& s) { return (long long)s.pairs * s.units * s.unit_bytes; }
+inline long long ql_bytes(const QlShape& s) { return (long long)s.pairs * s.units * ql_unit_bytes(s.group); }
 
 // Byte offsets of output n's word for channels k .. k + 7 (k a multiple of 8), and of its scale; inside a word channel 2 i + e is nibble
 // i + 4 e.
+__device__ inline long long ql_unit_at(const QlShape& s, int n, int k) { return ((long long)(n >> 5) * s.units + k / QL_CHANNELS) * ql_unit_bytes(s.group); }
 __device__ inline long long ql_word_at(const QlShape& s, int n, int k) {
-  const int unit = k / s.channels, blocks = s.channels / 64, block = (k % s.channels) / 64, g = (k >> 5) & 1, tig = (k >> 3) & 3;
-  return ((long long)(n >> 5) * s.units + unit) * s.unit_bytes + (((n >> 4) & 1) * blocks + block) * 512 + (((n & 7) * 4 + tig) * 4 + 2 * g + ((n >> 3) & 1)) * 4;
+  return ql_unit_at(s, n, k) + (((n >> 4) & 1) * 2 + ((k >> 6) & 1)) * 512 + (((n & 7) * 4 + ((k >> 3) & 3)) * 4 + 2 * ((k >> 5) & 1) + ((n >> 3) & 1)) * 4;
 }
 __device__ inline long long ql_scale_at(const QlShape& s, int n, int k) {
-  const int unit = k / s.channels, blocks = s.channels / 64, scales = s.group == 32 ? 2 : 1, g = s.group == 32 ? (k >> 5) & 1 : 0;
-  return ((long long)(n >> 5) * s.units + unit) * s.unit_bytes + 2 * blocks * 512 + (((n >> 4) & 1) * scales + g) * 32 + (n & 7) * 4 + ((n >> 3) & 1) * 2;
+  return ql_unit_at(s, n, k) + QL_CODES + (((n >> 4) & 1) * (QL_CHANNELS / s.group) + k % QL_CHANNELS / s.group) * 32 + (n & 7) * 4 + ((n >> 3) & 1) * 2;
 }
 __host__ __device__ inline int ql_nibble(int c) { return ((c & 7) >> 1) + 4 * (c & 1); }
 
 // ---- packing (once per matrix) ----
 // one thread per eight channels of one output, padding included
 __global__ void ql_pack_kernel(const int8_t* __restrict__ codes, const bf16* __restrict__ scales, unsigned char* __restrict__ packed, QlShape s) {
-  const int per = s.units * s.channels / 8, groups = s.d_in / s.group;
+  const int per = s.units * QL_CHANNELS / 8, groups = s.d_in / s.group;
   const long long total = (long long)s.pairs * 32 * per;
   for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
     const int n = (int)(i / per), k = (int)(i - (long long)n * per) * 8, grp = k / s.group;
@@ -102,7 +91,7 @@ __global__ void ql_pack_kernel(const int8_t* __restrict__ codes, const bf16* __r
 
 // one thread per (output, group), padding included
 __global__ void ql_quantize_kernel(const float* __restrict__ weights, unsigned char* __restrict__ packed, QlShape s) {
-  const int per = s.units * s.channels / s.group, groups = s.d_in / s.group;
+  const int per = s.units * QL_CHANNELS / s.group, groups = s.d_in / s.group;
   const long long total = (long long)s.pairs * 32 * per;
   for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
     const int n = (int)(i / per), grp = (int)(i - (long long)n * per);
@@ -148,10 +137,11 @@ __device__ __forceinline__ void ql_mma_bf16(float* c, uint32_t a0, uint32_t a1, 
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void ql_mma_e4m3(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// the same with a start of its own
+__device__ __forceinline__ void ql_mma_bf16(float* d, const float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 __device__ __forceinline__ void ql_copy16(uint32_t smem, const void* gmem) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
@@ -197,19 +187,6 @@ template <> __device__ __forceinline__ void ql_load8<bf16>(const bf16* p, float*
     f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
   }
 }
-// two f32 numbers as e4m3, the first one in the low byte
-__device__ __forceinline__ uint32_t ql_e4m3x2(float lo, float hi) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ float2 ql_from_e4m3x2(uint32_t v) {
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)v));
-  return __half22float2(*reinterpret_cast<const __half2*>(&h));
-}
-
-enum { QL_BF16 = 0, QL_E4M3 = 1 };
 template <typename T> struct QlPieces { static constexpr int N = 1; };
 template <> struct QlPieces<float> { static constexpr int N = 3; };
 
@@ -225,44 +202,50 @@ struct QlPlan {
 constexpr int QL_FRONT = 3 * QL_ROWS * 4;
 
 // grid: (clusters * passes) * cluster, the passes over the same tiles next to each other
-template <typename T, int MODE, int NT, int GROUP>
+template <typename T, int NT, int GROUP>
 __global__ void __launch_bounds__(QL_MAX_WARPS * 32)
 q4_linear_kernel(const T* __restrict__ x, long long ld_x, const unsigned char* __restrict__ packed, T* __restrict__ y, long long ld_y, int rows_total,
                  QlShape s, QlPlan plan) {
-  using U = QlUnit<GROUP>;
-  constexpr int P = MODE == QL_E4M3 ? 1 : QlPieces<T>::N, SUBS = GROUP / 32, PER_UNIT = U::CHANNELS / GROUP;
+  constexpr int P = QlPieces<T>::N, SUBS = GROUP / 32, PER_UNIT = QL_CHANNELS / GROUP, BYTES = ql_unit_bytes(GROUP);
   extern __shared__ __align__(128) unsigned char ql_sm[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
   const int threads = blockDim.x, wk_count = plan.wk, wn_count = plan.warps / wk_count, wk = warp % wk_count, wn = warp / wk_count;
   const int cluster = plan.cluster, rank = blockIdx.x % cluster, pass = blockIdx.x / cluster % plan.passes, tile0 = blockIdx.x / cluster / plan.passes;
   const int row0 = pass * plan.per_pass, rows = min(rows_total - row0, plan.per_pass);
   const int ubeg = (int)((long long)s.units * rank / cluster), uend = (int)((long long)s.units * (rank + 1) / cluster);
-  const int k0 = ubeg * U::CHANNELS, channels = (uend - ubeg) * U::CHANNELS;
-  const int pitch = plan.slice * U::CHANNELS * 2 + 64, plane = rows * pitch;
+  const int k0 = ubeg * QL_CHANNELS, channels = (uend - ubeg) * QL_CHANNELS;
+  const int pitch = plan.slice * QL_CHANNELS * 2 + 64, plane = rows * pitch;
   float* factor = reinterpret_cast<float*>(ql_sm);                // what a row's sums are multiplied with in the end
-  int* mark = reinterpret_cast<int*>(ql_sm) + QL_ROWS;            // e4m3: bits of the largest finite magnitude; bf16: one above QL_LARGE is there
+  int* mark = reinterpret_cast<int*>(ql_sm) + QL_ROWS;            // one above QL_LARGE is there
   int* odd = mark + QL_ROWS;                                      // something infinite or NaN is there
   float* start = reinterpret_cast<float*>(ql_sm + plan.starts);
   unsigned char* acts = ql_sm + plan.acts;
 
   // ---- the warp's units: of the tiles tile0, tile0 + clusters, .. those from ubeg + wk on in steps of wk_count ----
   const int first = ubeg + wk;
-  unsigned char* ring = ql_sm + plan.rings + warp * (plan.stages * U::BYTES);
+  int stage = 0;
+  unsigned char* ring = ql_sm + plan.rings + warp * (plan.stages * BYTES);
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
-  int next_tile = first < uend ? tile0 : plan.tiles, next_unit = first, next_stage = 0, stage = 0;
+  const int pairs_per_tile = wn_count * plan.clusters;
+  int next_pair = first < uend ? tile0 * wn_count + wn : s.pairs, next_unit = first;
+  const unsigned char* next_src = packed + ((long long)next_pair * s.units + first) * BYTES + lane * 16;
+  uint32_t next_dst = ring_at;
+  const uint32_t ring_end = ring_at + plan.stages * BYTES;
   auto issue = [&] {
-    const int pair = next_tile * wn_count + wn;
-    if (next_tile < plan.tiles && pair < s.pairs) {
-      const unsigned char* src = packed + ((long long)pair * s.units + next_unit) * U::BYTES + lane * 16;
-      const uint32_t dst = ring_at + next_stage * U::BYTES;
+    if (next_pair < s.pairs) {
 #pragma unroll
-      for (int i = 0; i < U::CODES; i += 512) ql_copy16(dst + i, src + i);
-      if (lane < U::SCALES * 4) ql_copy16(dst + U::CODES, src + U::CODES);
+      for (int i = 0; i < QL_CODES; i += 512) ql_copy16(next_dst + i, next_src + i);
+      if (lane < (BYTES - QL_CODES) / 16) ql_copy16(next_dst + QL_CODES, next_src + QL_CODES);
+      next_unit += wk_count;
+      next_src += wk_count * BYTES;
+      if (next_unit >= uend) {
+        next_src += ((long long)pairs_per_tile * s.units + first - next_unit) * BYTES;
+        next_unit = first;
+        next_pair += pairs_per_tile;
+      }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
-    next_unit += wk_count;
-    if (next_unit >= uend) { next_unit = first; next_tile += plan.clusters; }
-    next_stage = next_stage + 1 == plan.stages ? 0 : next_stage + 1;
+    next_dst = next_dst + BYTES == ring_end ? ring_at : next_dst + BYTES;
   };
   for (int i = 0; i < plan.stages - 1; ++i) issue();
 
@@ -270,19 +253,6 @@ q4_linear_kernel(const T* __restrict__ x, long long ld_x, const unsigned char* _
   const int parts = channels / 8, work = rows * parts;
   for (int i = threadIdx.x; i < 2 * QL_ROWS; i += threads) mark[i] = 0;
   __syncthreads();
-  if constexpr (MODE == QL_E4M3) {
-    for (int i = threadIdx.x; i < work; i += threads) {
-      const int r = i / parts, k = k0 + (i - r * parts) * 8;
-      if (k >= s.d_in) continue;
-      float f[8];
-      ql_load8<T>(x + (row0 + r) * ld_x + k, f);
-      uint32_t top = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, ql_finite(f[j]) ? __float_as_uint(f[j]) & 0x7fffffffu : 0u);
-      atomicMax(mark + r, (int)top);
-    }
-    __syncthreads();
-  }
   for (int again = 0;; ++again) {
     bool large = false;
     for (int i0 = warp * 32; i0 < work; i0 += threads) {
@@ -291,35 +261,20 @@ q4_linear_kernel(const T* __restrict__ x, long long ld_x, const unsigned char* _
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[j] = 0.f;
       if (i < work && k < s.d_in) ql_load8<T>(x + (row0 + r) * ld_x + k, f);
-      int up = QL_UP;
-      if constexpr (MODE == QL_E4M3) up = min(134 - (mark[r] >> 23), 120);         // the row's largest to 128 .. 256
-      else if (again && mark[r]) up = QL_UP - QL_DOWN;
-      const float by = __uint_as_float((uint32_t)(up + 127) << 23);
+      const float by = again && mark[r] ? ql_pow2(QL_UP - QL_DOWN) : ql_pow2(QL_UP);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         if (!ql_finite(f[j])) { odd[r] = 1; f[j] = 0.f; }
-        if (MODE == QL_BF16 && !again && fabsf(f[j]) > QL_LARGE) { mark[r] = 1; large = true; }
+        if (!again && fabsf(f[j]) > QL_LARGE) { mark[r] = 1; large = true; }
         f[j] *= by;
-        sum += f[j] * ql_pow2(MODE == QL_E4M3 ? 0 : -64);         // a sum of numbers up to 2^127
+        sum += f[j] * ql_pow2(-64);         // a sum of numbers up to 2^127
       }
 #pragma unroll
       for (int o = 1; o < GROUP / 8; o *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       if (i >= work) continue;
-      if (P == 1 && (c & (GROUP - 1)) == 0) start[(c / GROUP) * (NT * 8) + r] = sum * ql_pow2(MODE == QL_E4M3 ? -9 : 64 - QL_RAW) * -8.f;
+      if (P == 1 && (c & (GROUP - 1)) == 0) start[(c / GROUP) * (NT * 8) + r] = sum * ql_pow2(64 - QL_RAW) * -8.f;
       unsigned char* dst = acts + r * pitch + c * 2;
-      if constexpr (MODE == QL_E4M3) {
-        // channels in the order of a word's low nibbles, then of its high ones; what the first e4m3 number leaves is the second
-        uint32_t hi[4], lo[4];
-        const int at[8] = {0, 4, 1, 5, 2, 6, 3, 7};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float a = f[at[2 * j]], b = f[at[2 * j + 1]];
-          hi[j] = ql_e4m3x2(a, b);
-          const float2 h = ql_from_e4m3x2(hi[j]);
-          lo[j] = ql_e4m3x2(a - h.x, b - h.y);
-        }
-        *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0] | hi[1] << 16, hi[2] | hi[3] << 16, lo[0] | lo[1] << 16, lo[2] | lo[3] << 16);
-      } else {
+      {
         uint32_t p[8][3];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -332,12 +287,11 @@ q4_linear_kernel(const T* __restrict__ x, long long ld_x, const unsigned char* _
           *reinterpret_cast<uint4*>(dst + q * plane) = make_uint4(p[0][q] | p[1][q] << 16, p[2][q] | p[3][q] << 16, p[4][q] | p[5][q] << 16, p[6][q] | p[7][q] << 16);
       }
     }
-    if (MODE == QL_E4M3 || again || !__syncthreads_or(large)) break;
+    if (again || !__syncthreads_or(large)) break;
   }
   __syncthreads();
   if (threadIdx.x < rows) {
-    const int m = mark[threadIdx.x];
-    factor[threadIdx.x] = MODE == QL_E4M3 ? __uint_as_float((uint32_t)(127 - min(134 - (m >> 23), 120)) << 23) : m ? ql_pow2(QL_DOWN) : 1.f;
+    factor[threadIdx.x] = mark[threadIdx.x] ? ql_pow2(QL_DOWN) : 1.f;
   }
   bool any_odd = false;
   for (int r = 0; r < rows; ++r) any_odd |= odd[r] != 0;
@@ -359,95 +313,76 @@ q4_linear_kernel(const T* __restrict__ x, long long ld_x, const unsigned char* _
     for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int n = 0; n < NT; ++n) acc[m][n][0] = acc[m][n][1] = acc[m][n][2] = acc[m][n][3] = 0.f;
-    for (int unit = first; unit < uend; unit += wk_count) {
-      if (plan.stages == 3) asm volatile("cp.async.wait_group 1;" ::: "memory");
-      else if (plan.stages == 4) asm volatile("cp.async.wait_group 2;" ::: "memory");
-      else asm volatile("cp.async.wait_group 4;" ::: "memory");
+    // a pair that does not exist has no units in the ring: the warp only takes part in the joining
+    for (int unit = first; live && unit < uend; unit += wk_count) {
+      if (plan.stages == 2) asm volatile("cp.async.wait_group 0;" ::: "memory");
+      else if (plan.stages == 3) asm volatile("cp.async.wait_group 1;" ::: "memory");
+      else asm volatile("cp.async.wait_group 2;" ::: "memory");
       __syncwarp();                                               // the unit has landed for every lane, and the one before is used up
       issue();
-      const unsigned char* at = ring + stage * U::BYTES;
-      stage = stage + 1 == plan.stages ? 0 : stage + 1;
-      if (!live) continue;
-      const int c0 = (unit - ubeg) * U::CHANNELS;
+      const unsigned char* at = ring + stage;
+      stage = stage + BYTES == plan.stages * BYTES ? 0 : stage + BYTES;
+      const int c0 = (unit - ubeg) * QL_CHANNELS;
+      float part[2][NT][4];
+      auto scaled = [&](int grp) {
 #pragma unroll
-      for (int grp = 0; grp < PER_UNIT; ++grp) {
-        float part[2][NT][4];
-        auto scaled = [&](int grp) {
+        for (int m = 0; m < 2; ++m) {
+          const uint32_t v = *reinterpret_cast<const uint32_t*>(at + QL_CODES + (m * PER_UNIT + grp) * 32 + gid * 4);
+          const float s0 = __uint_as_float(v << 16), s1 = __uint_as_float(v & 0xffff0000u);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            acc[m][n][0] = fmaf(s0, part[m][n][0], acc[m][n][0]);
+            acc[m][n][1] = fmaf(s0, part[m][n][1], acc[m][n][1]);
+            acc[m][n][2] = fmaf(s1, part[m][n][2], acc[m][n][2]);
+            acc[m][n][3] = fmaf(s1, part[m][n][3], acc[m][n][3]);
+          }
+        }
+      };
+#pragma unroll
+      for (int block = 0; block < 2; ++block) {
+        uint4 w[2];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) w[m] = *reinterpret_cast<const uint4*>(at + (m * 2 + block) * 512 + lane * 16);
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const int g32 = block * 2 + g, grp = g32 / SUBS, off = (c0 + g32 * 32) * 2;
+          const bool opens = P > 1 || g32 % SUBS == 0, closes = P > 1 || g32 % SUBS == SUBS - 1;
+          uint32_t a[2][8];
 #pragma unroll
           for (int m = 0; m < 2; ++m) {
-            const uint32_t v = *reinterpret_cast<const uint32_t*>(at + U::CODES + (m * U::SCALES + grp) * 32 + gid * 4);
-            const float s0 = __uint_as_float(v << 16), s1 = __uint_as_float(v & 0xffff0000u);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              acc[m][n][0] = fmaf(s0, part[m][n][0], acc[m][n][0]);
-              acc[m][n][1] = fmaf(s0, part[m][n][1], acc[m][n][1]);
-              acc[m][n][2] = fmaf(s1, part[m][n][2], acc[m][n][2]);
-              acc[m][n][3] = fmaf(s1, part[m][n][3], acc[m][n][3]);
+            const uint32_t lo = g ? w[m].z : w[m].x, hi = g ? w[m].w : w[m].y;
+            if constexpr (P == 1) {
+              a[m][0] = ql_raw<0>(lo); a[m][1] = ql_raw<0>(hi); a[m][2] = ql_raw<1>(lo); a[m][3] = ql_raw<1>(hi);
+              a[m][4] = ql_raw<2>(lo); a[m][5] = ql_raw<2>(hi); a[m][6] = ql_raw<3>(lo); a[m][7] = ql_raw<3>(hi);
+            } else {
+              a[m][0] = ql_signed<0>(lo); a[m][1] = ql_signed<0>(hi); a[m][2] = ql_signed<1>(lo); a[m][3] = ql_signed<1>(hi);
+              a[m][4] = ql_signed<2>(lo); a[m][5] = ql_signed<2>(hi); a[m][6] = ql_signed<3>(lo); a[m][7] = ql_signed<3>(hi);
             }
           }
-        };
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float2 v = make_float2(0.f, 0.f);
-          if constexpr (P == 1) v = *reinterpret_cast<const float2*>(start + (c0 / GROUP + grp) * (NT * 8) + n * 8 + 2 * tig);
+          for (int n = 0; n < NT; ++n) {
+            float from[4] = {0.f, 0.f, 0.f, 0.f};
+            if (P == 1 && opens) {
+              const float2 v = *reinterpret_cast<const float2*>(start + (c0 / GROUP + grp) * (NT * 8) + n * 8 + 2 * tig);
+              from[0] = from[2] = v.x;
+              from[1] = from[3] = v.y;
+            }
 #pragma unroll
-          for (int m = 0; m < 2; ++m) { part[m][n][0] = part[m][n][2] = v.x; part[m][n][1] = part[m][n][3] = v.y; }
-        }
-#pragma unroll
-        for (int sub = 0; sub < SUBS; ++sub) {
-          const int g32 = grp * SUBS + sub, block = g32 >> 1, g = g32 & 1;
-          uint32_t lo[2], hi[2];
-#pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            const uint2 w = *reinterpret_cast<const uint2*>(at + (m * U::BLOCKS + block) * 512 + lane * 16 + g * 8);
-            lo[m] = w.x; hi[m] = w.y;
-          }
-          const int off = (c0 + g32 * 32) * 2;
-          if constexpr (MODE == QL_E4M3) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              const uint4 b = *reinterpret_cast<const uint4*>(mine[n] + off);
+            for (int q = 0; q < P; ++q) {
+              const uint4 b = *reinterpret_cast<const uint4*>(mine[n] + q * plane + off);
 #pragma unroll
               for (int m = 0; m < 2; ++m) {
-                const uint32_t a0 = lo[m] & 0x0f0f0f0fu, a1 = hi[m] & 0x0f0f0f0fu, a2 = (lo[m] >> 4) & 0x0f0f0f0fu, a3 = (hi[m] >> 4) & 0x0f0f0f0fu;
-                ql_mma_e4m3(part[m][n], a0, a1, a2, a3, b.x, b.y);
-                ql_mma_e4m3(part[m][n], a0, a1, a2, a3, b.z, b.w);
-              }
-            }
-          } else {
-            uint32_t a[2][8];
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-              if constexpr (P == 1) {
-                a[m][0] = ql_raw<0>(lo[m]); a[m][1] = ql_raw<0>(hi[m]); a[m][2] = ql_raw<1>(lo[m]); a[m][3] = ql_raw<1>(hi[m]);
-                a[m][4] = ql_raw<2>(lo[m]); a[m][5] = ql_raw<2>(hi[m]); a[m][6] = ql_raw<3>(lo[m]); a[m][7] = ql_raw<3>(hi[m]);
-              } else {
-                a[m][0] = ql_signed<0>(lo[m]); a[m][1] = ql_signed<0>(hi[m]); a[m][2] = ql_signed<1>(lo[m]); a[m][3] = ql_signed<1>(hi[m]);
-                a[m][4] = ql_signed<2>(lo[m]); a[m][5] = ql_signed<2>(hi[m]); a[m][6] = ql_signed<3>(lo[m]); a[m][7] = ql_signed<3>(hi[m]);
-              }
-            }
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int q = 0; q < P; ++q) {
-                const uint4 b = *reinterpret_cast<const uint4*>(mine[n] + q * plane + off);
-#pragma unroll
-                for (int m = 0; m < 2; ++m) {
-                  ql_mma_bf16(part[m][n], a[m][0], a[m][1], a[m][2], a[m][3], b.x, b.y);
+                {
+                  if (opens && q == 0) ql_mma_bf16(part[m][n], from, a[m][0], a[m][1], a[m][2], a[m][3], b.x, b.y);
+                  else ql_mma_bf16(part[m][n], a[m][0], a[m][1], a[m][2], a[m][3], b.x, b.y);
                   ql_mma_bf16(part[m][n], a[m][4], a[m][5], a[m][6], a[m][7], b.z, b.w);
                 }
               }
+            }
           }
-          if constexpr (P > 1) {
-            // the tensor cores cut sums off where f32 arithmetic rounds them: short chains only
-            scaled(grp);
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-              for (int n = 0; n < NT; ++n) part[m][n][0] = part[m][n][1] = part[m][n][2] = part[m][n][3] = 0.f;
-          }
+          // f32: the tensor cores cut sums off where f32 arithmetic rounds them, so chains are short
+          if (closes) scaled(grp);
         }
-        if constexpr (P == 1) scaled(grp);
       }
     }
 
@@ -462,8 +397,8 @@ q4_linear_kernel(const T* __restrict__ x, long long ld_x, const unsigned char* _
         float* dst = red + (wk * rows + r) * width + wn * 32 + gid;
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-          dst[16 * m] = acc[m][n][e] * ql_pow2(MODE == QL_E4M3 ? 9 : QL_RAW - QL_UP) * by;
-          dst[16 * m + 8] = acc[m][n][2 + e] * ql_pow2(MODE == QL_E4M3 ? 9 : QL_RAW - QL_UP) * by;
+          dst[16 * m] = acc[m][n][e] * ql_pow2(QL_RAW - QL_UP) * by;
+          dst[16 * m + 8] = acc[m][n][2 + e] * ql_pow2(QL_RAW - QL_UP) * by;
         }
       }
     const int n0 = tile * width;
@@ -517,67 +452,74 @@ bool ql_sizes_ok(int d_out, int d_in, int group) {
   return d_out > 0 && d_in > 0 && (group == 32 || group == 64 || group == 128) && d_in % group == 0 && d_in <= QL_MAX_IN && d_out <= (1 << 28);
 }
 
-// How to cut a product with `live` <= NT * 8 rows a pass.  False: the activations of a pass do not fit.
-template <typename T, int MODE, int NT, int GROUP>
+// How to cut a product with `live` <= NT * 8 rows a pass: of the ways that fit, the one that should be done first.  False: none fits.
+// The estimate is in cycles of an SM and counts what was measured: a unit takes an SM the issue of its instructions (0.17 a cycle for each warp, up to 2.6), its
+// products (2.1 cycles each) or its share of HBM (24 bytes a cycle), whichever is longest, and a warp no less than its latency; joining
+// a tile takes 700 cycles, over a cluster 5000; a thread takes 50 to 110 instructions for eight activations.
+template <typename T, int NT, int GROUP>
 bool ql_plan(const QlShape& s, int rows, int live, QlPlan* out) {
-  using U = QlUnit<GROUP>;
-  constexpr int P = MODE == QL_E4M3 ? 1 : QlPieces<T>::N;
+  constexpr int P = QlPieces<T>::N, BYTES = ql_unit_bytes(GROUP), SM = 148;
+  constexpr double issue = (70 + 4 * (P == 1 ? 28 + 6 * NT : 48 + 18 * NT) + QL_CHANNELS / (P == 1 ? GROUP : 32) * (6 + 18 * NT));
+  constexpr double products = 16 * NT * 2.1 * P;
+  const int most[4] = {8, 8, 12, 16}, limit[4] = {113 * 1024, 227 * 1024, 227 * 1024, 227 * 1024}, resident[4] = {2, 1, 1, 1};
+  const int at_once[4] = {SM, 74, 33, 15};   // clusters of 1, 2, 4 and 8 SMs that the machine holds: they do not cross the borders of a GPC
+  double best = -1;
   QlPlan p{};
   p.per_pass = live;
   p.passes = (rows + live - 1) / live;
   auto up = [](int v) { return (v + 127) / 128 * 128; };
-  // where things lie, with as many units in flight and as many buffers as fit
-  auto fits = [&](int limit) {
-    p.starts = QL_FRONT;
-    p.acts = p.starts + up(p.slice * U::CHANNELS / GROUP * NT * 8 * 4);
-    p.rings = p.acts + up(P * live * (p.slice * U::CHANNELS * 2 + 64));
-    const int sums = live * 32 * p.warps * 4;
-    for (p.buffers = 2; p.buffers >= 1; --p.buffers)
-      for (p.stages = 6; p.stages >= 3; p.stages -= p.stages == 6 ? 2 : 1) {
-        p.sums = p.rings + up(p.warps * p.stages * U::BYTES);
-        p.bytes = p.sums + p.buffers * sums;
-        if (p.bytes <= limit) return true;
-      }
-    return false;
-  };
-  // Two CTAs of 8 warps on an SM, or one of 16 where the activations take more than a half.  Warps along the reduction: each should have
-  // several units of a tile (joining a tile costs about 2.5 units' time), and the tiles should come out even.
-  auto shape = [&](int warps, int limit, int ctas) {
-    double best = -1;
-    QlPlan keep{};
-    for (int cluster = 1; cluster <= QL_MAX_CLUSTER; cluster *= 2) {
-      p.warps = warps;
-      p.cluster = cluster;
-      p.slice = (s.units + cluster - 1) / cluster;
-      if (cluster > 1 && p.slice * cluster > s.units + cluster - 1) break;
-      if (cluster > 1 && p.slice < 2) break;
-      for (p.wk = 1; p.wk <= warps && p.wk <= p.slice; p.wk *= 2) {
-        p.tiles = (s.pairs + warps / p.wk - 1) / (warps / p.wk);
-        p.clusters = std::min(p.tiles, std::max(1, ctas / (cluster * p.passes)));
-        const int rounds = (p.tiles + p.clusters - 1) / p.clusters, each = (p.slice + p.wk - 1) / p.wk;
-        // units' time from start to end: filling the activations, the tiles, joining them (a cluster's join takes longer)
-        const double busy = std::min(1.0, (double)p.clusters * cluster * p.passes * warps / (148.0 * 16));
-        const double time = rounds * (each * std::max(busy, 0.35) + (cluster > 1 ? 6.0 : 2.5) * std::max(busy, 0.5));
-        if ((best < 0 || time < best) && fits(limit)) { best = time; keep = p; }
+  for (int way = 0; way < 4; ++way)
+    for (int log = 0; log < 4; ++log) {
+      p.cluster = 1 << log;
+      p.warps = most[way];
+      p.slice = (s.units + p.cluster - 1) / p.cluster;
+      if (p.cluster > 1 && s.units < 2 * p.cluster) break;
+      p.starts = QL_FRONT;
+      p.acts = p.starts + up(p.slice * QL_CHANNELS / GROUP * NT * 8 * 4);
+      p.rings = p.acts + up(P * live * (p.slice * QL_CHANNELS * 2 + 64));
+      const int sums = live * 32 * p.warps * 4;
+      bool fits = false;
+      for (p.stages = 4; p.stages >= 2 && !fits; p.stages -= !fits)
+        for (p.buffers = 2; p.buffers >= 1 && !fits; p.buffers -= !fits) {
+          p.sums = p.rings + p.warps * p.stages * BYTES;
+          p.bytes = p.sums + p.buffers * sums;
+          fits = p.bytes <= limit[way];
+        }
+      if (!fits) continue;
+      for (p.wk = 1; p.warps % p.wk == 0 && p.wk <= p.slice; p.wk *= 2) {
+        p.tiles = (s.pairs + p.warps / p.wk - 1) / (p.warps / p.wk);
+        p.clusters = std::min(p.tiles, std::max(1, resident[way] * at_once[log] / p.passes));
+        const int rounds = (p.tiles + p.clusters - 1) / p.clusters, each = (p.slice + p.wk - 1) / p.wk, ctas = p.clusters * p.cluster * p.passes;
+        const int room = at_once[log] * p.cluster, on_sm = std::min(resident[way], (ctas + room - 1) / room);
+        const double hbm = BYTES / 24.0 / p.passes * std::min(1.0, (double)ctas / SM / on_sm);
+        const double rate = std::min(2.6, 0.17 * p.warps * on_sm);
+        const double unit = std::max(p.warps * on_sm * std::max(hbm, std::max(issue / rate, products)), std::max(350.0, 1100.0 / (p.stages - 1)));
+        const double fill = 1500 + (double)live * p.slice * 16 / 32 * (P == 1 ? 50 : 110) * on_sm / rate;
+        const double waves = (double)((ctas + on_sm * room - 1) / (on_sm * room));
+        const double time = waves * (fill + rounds * (each * unit + (p.cluster > 1 ? 5000.0 : 700.0)));
+        if (best < 0 || time < best) { best = time; *out = p; }
       }
     }
-    if (best < 0) return false;
-    *out = keep;
-    fits(limit);
-    return true;
-  };
-  return shape(8, 113 * 1024, 2 * 148) || shape(16, 227 * 1024, 148);
+  return best >= 0;
 }
 
-template <typename T, int MODE, int NT, int GROUP>
+template <typename T, int NT, int GROUP>
 cudaError_t ql_launch(const T* x, long long ld_x, const void* packed, T* y, long long ld_y, int rows, const QlShape& s, cudaStream_t st) {
-  QlPlan plan;
-  int live = std::min(rows, NT * 8);
-  while (!ql_plan<T, MODE, NT, GROUP>(s, rows, live, &plan)) {
-    if (live == 1) return cudaErrorInvalidConfiguration;   // not reached: d_in is at most QL_MAX_IN
-    live = (live + 1) / 2;
+  // a plan depends on the sizes alone: a thread keeps the last few
+  struct Known { int d_in, d_out, rows; QlPlan plan; };
+  static thread_local Known known[16] = {};
+  Known& last = known[(unsigned)(s.d_in * 31 + s.d_out * 7 + rows) % 16];
+  if (last.rows != rows || last.d_in != s.d_in || last.d_out != s.d_out) {
+    QlPlan made;
+    int live = std::min(rows, NT * 8);
+    while (!ql_plan<T, NT, GROUP>(s, rows, live, &made)) {
+      if (live == 1) return cudaErrorInvalidConfiguration;   // not reached: d_in is at most QL_MAX_IN
+      live = (live + 1) / 2;
+    }
+    last = Known{s.d_in, s.d_out, rows, made};
   }
-  auto kernel = q4_linear_kernel<T, MODE, NT, GROUP>;
+  const QlPlan plan = last.plan;
+  auto kernel = q4_linear_kernel<T, NT, GROUP>;
   static std::atomic<unsigned long long> raised{0};   // devices on which the kernel's shared-memory limit has been raised
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
@@ -605,10 +547,7 @@ template <typename T, int GROUP>
 cudaError_t ql_dispatch(const void* x, long long ld_x, const void* packed, void* y, long long ld_y, int rows, const QlShape& s, cudaStream_t st) {
   const T* xt = (const T*)x;
   T* yt = (T*)y;
-  if (rows <= 8) return ql_launch<T, QL_BF16, 1, GROUP>(xt, ld_x, packed, yt, ld_y, rows, s, st);
-  if constexpr (sizeof(T) == 2)
-    if (rows > 16) return ql_launch<T, QL_E4M3, 2, GROUP>(xt, ld_x, packed, yt, ld_y, rows, s, st);
-  return ql_launch<T, QL_BF16, 2, GROUP>(xt, ld_x, packed, yt, ld_y, rows, s, st);
+  return rows <= 8 ? ql_launch<T, 1, GROUP>(xt, ld_x, packed, yt, ld_y, rows, s, st) : ql_launch<T, 2, GROUP>(xt, ld_x, packed, yt, ld_y, rows, s, st);
 }
 template <typename T>
 cudaError_t ql_dispatch(const void* x, long long ld_x, const void* packed, void* y, long long ld_y, int rows, const QlShape& s, cudaStream_t st) {
@@ -645,7 +584,7 @@ int32_t q4_linear_pack(const int8_t* codes, const void* scales, void* packed, in
   QL_CHECK(packed);
   if (!codes || !scales) return ql_fail(message, message_len, MOE_INVALID_INPUT, "InvalidInput: null buffer");
   const QlShape s = ql_shape(d_out, d_in, group);
-  ql_pack_kernel<<<ql_blocks((long long)s.pairs * 32 * s.units * s.channels / 8), 256, 0, (cudaStream_t)stream>>>(codes, (const bf16*)scales,
+  ql_pack_kernel<<<ql_blocks((long long)s.pairs * 32 * s.units * QL_CHANNELS / 8), 256, 0, (cudaStream_t)stream>>>(codes, (const bf16*)scales,
                                                                                                                 (unsigned char*)packed, s);
   count_launch();
   const cudaError_t e = cudaGetLastError();
@@ -657,7 +596,7 @@ int32_t q4_linear_quantize(const float* weights, void* packed, int32_t d_out, in
   QL_CHECK(packed);
   if (!weights) return ql_fail(message, message_len, MOE_INVALID_INPUT, "InvalidInput: null buffer");
   const QlShape s = ql_shape(d_out, d_in, group);
-  ql_quantize_kernel<<<ql_blocks((long long)s.pairs * 32 * s.units * s.channels / group), 256, 0, (cudaStream_t)stream>>>(weights, (unsigned char*)packed, s);
+  ql_quantize_kernel<<<ql_blocks((long long)s.pairs * 32 * s.units * QL_CHANNELS / group), 256, 0, (cudaStream_t)stream>>>(weights, (unsigned char*)packed, s);
   count_launch();
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? MOE_OK : ql_fail(message, message_len, MOE_CUDA_ERROR, cudaGetErrorString(e));

@@ -12,10 +12,10 @@ from rustingbrain_b200 import InvalidConfig, InvalidInput, _lib
 def test_arguments_are_checked_before_any_device_work():
     L = _lib.lib()
     size = L.q4_linear_packed_bytes
-    # 16-output blocks in pairs, 64-channel blocks of 512 bytes, 32 bytes of scales per block of outputs and group
-    assert size(1, 32, 32) == 2 * 512 + 2 * 2 * 32
-    assert size(2816, 1024, 32) == 176 * 16 * 512 + 176 * 32 * 32
-    assert size(33, 384, 128) == 4 * 6 * 512 + 4 * 3 * 32
+    # units of 32 outputs and 128 channels: half a byte a code, two bytes a scale
+    assert size(1, 32, 32) == 32 * 64 + 32 * 4 * 2
+    assert size(2816, 1024, 32) == 2816 * 512 + 2816 * 32 * 2
+    assert size(33, 384, 128) == 64 * 192 + 64 * 3 * 2
     for bad in ((0, 32, 32), (4, 0, 32), (4, 33, 32), (4, 64, 16), (4, 64, 128), (4, 96, 64), (-1, 32, 32), (4, 256, 256)):
         assert size(*bad) == 0, bad
     buf = (C.c_float * 256)()
