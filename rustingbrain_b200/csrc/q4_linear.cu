@@ -173,25 +173,77 @@ __device__ __forceinline__ void ql_split(float x, uint32_t* p) {
     x -= __uint_as_float(top);
   }
 }
-template <typename T> __device__ __forceinline__ void ql_load8(const T* p, float* f);
-template <> __device__ __forceinline__ void ql_load8<float>(const float* p, float* f) {
-  *reinterpret_cast<float4*>(f) = __ldg(reinterpret_cast<const float4*>(p));
-  *reinterpret_cast<float4*>(f + 4) = __ldg(reinterpret_cast<const float4*>(p) + 1);
-}
-template <> __device__ __forceinline__ void ql_load8<bf16>(const bf16* p, float* f) {
-  const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+// Eight activations as they were loaded.  `plain` ones (finite, at most QL_LARGE) become operands here: times 2^QL_UP, and 2^-4 less where the
+// code weighs 16; returned is their sum.
+template <typename T> constexpr int QL_BATCH = sizeof(T) == 2 ? 4 : 2;
+template <typename T> struct QlRaw;
+template <> struct QlRaw<bf16> {
+  struct type { uint4 v; };
+  static __device__ __forceinline__ type load(const bf16* p) { return {__ldg(reinterpret_cast<const uint4*>(p))}; }
+  static __device__ __forceinline__ void widen(const type& a, float* f) {
+    const uint32_t w[4] = {a.v.x, a.v.y, a.v.z, a.v.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = __uint_as_float(w[i] << 16);
-    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
   }
-}
+  static __device__ __forceinline__ __nv_bfloat162 pair(uint32_t v) { return *reinterpret_cast<const __nv_bfloat162*>(&v); }
+  static __device__ __forceinline__ uint32_t times(uint32_t v, float by) {
+    const __nv_bfloat162 r = __hmul2(pair(v), __float2bfloat162_rn(by));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  static __device__ __forceinline__ bool plain(const type& a) {
+    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(__habs2(pair(a.v.x)), __habs2(pair(a.v.y))), __hmax2_nan(__habs2(pair(a.v.z)), __habs2(pair(a.v.w))));
+    return __low2float(m) <= QL_LARGE && __high2float(m) <= QL_LARGE;
+  }
+  static __device__ __forceinline__ float plain_pieces(const type& a, uint4* out) {
+    float f[8];
+    widen(a, f);
+    out[0] = make_uint4(times(a.v.x, ql_pow2(QL_UP)), times(a.v.y, ql_pow2(QL_UP - 4)), times(a.v.z, ql_pow2(QL_UP)), times(a.v.w, ql_pow2(QL_UP - 4)));
+    return ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+  }
+};
+template <> struct QlRaw<float> {
+  struct type { float4 a, b; };
+  static __device__ __forceinline__ type load(const float* p) { return {__ldg(reinterpret_cast<const float4*>(p)), __ldg(reinterpret_cast<const float4*>(p) + 1)}; }
+  static __device__ __forceinline__ void widen(const type& t, float* f) {
+    *reinterpret_cast<float4*>(f) = t.a;
+    *reinterpret_cast<float4*>(f + 4) = t.b;
+  }
+  static __device__ __forceinline__ bool plain(const type& t) {
+    float f[8];
+    widen(t, f);
+    bool ok = true;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ok &= fabsf(f[j]) <= QL_LARGE;
+    return ok;
+  }
+  static __device__ __forceinline__ float plain_pieces(const type& t, uint4* out) {
+    float f[8];
+    uint32_t p[8][3];
+    widen(t, f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float v = f[j] * ql_pow2(j & 2 ? QL_UP - 4 : QL_UP);
+#pragma unroll
+      for (int q = 0; q < 3; ++q) {
+        p[j][q] = __float_as_uint(v) & 0xffff0000u;
+        v -= __uint_as_float(p[j][q]);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 3; ++q)
+      out[q] = make_uint4(p[0][q] >> 16 | p[1][q], p[2][q] >> 16 | p[3][q], p[4][q] >> 16 | p[5][q], p[6][q] >> 16 | p[7][q]);
+    return 0.f;                                       // not used: the codes are taken without their 8
+  }
+};
+
 template <typename T> struct QlPieces { static constexpr int N = 1; };
 template <> struct QlPieces<float> { static constexpr int N = 3; };
 
-// How a launch cuts the product, and where things lie in shared memory: factors, marks and flags of the rows first; then the starts of the
-// group sums [group][NT * 8] f32; the activations [piece][row][2 bytes a channel, and 64 that keep the 16-byte loads of a warp off each
+// How a launch cuts the product, and where things lie in shared memory: marks of the rows first; then the starts of the group sums
+// [group][NT * 8] f32; the activations [piece][row][2 bytes a channel, and 64 that keep the 16-byte loads of a warp off each
 // other's banks]; the warps' rings; the partial sums [buffer][wk][row][outputs of the tile] f32.
 struct QlPlan {
   int warps, wk, cluster;              // warps of a CTA, those of them along the reduction; CTAs along it
@@ -199,7 +251,7 @@ struct QlPlan {
   int slice, per_pass, stages, buffers;   // units of the reduction per CTA, at most; rows per pass; units in a ring; buffers of partial sums
   int starts, acts, rings, sums, bytes;
 };
-constexpr int QL_FRONT = 3 * QL_ROWS * 4;
+constexpr int QL_FRONT = 2 * QL_ROWS * 4;
 
 // grid: (clusters * passes) * cluster, the passes over the same tiles next to each other
 template <typename T, int NT, int GROUP>
@@ -215,8 +267,7 @@ q4_linear_kernel(const T* __restrict__ x, long long ld_x, const unsigned char* _
   const int ubeg = (int)((long long)s.units * rank / cluster), uend = (int)((long long)s.units * (rank + 1) / cluster);
   const int k0 = ubeg * QL_CHANNELS, channels = (uend - ubeg) * QL_CHANNELS;
   const int pitch = plan.slice * QL_CHANNELS * 2 + 64, plane = rows * pitch;
-  float* factor = reinterpret_cast<float*>(ql_sm);                // what a row's sums are multiplied with in the end
-  int* mark = reinterpret_cast<int*>(ql_sm) + QL_ROWS;            // one above QL_LARGE is there
+  int* mark = reinterpret_cast<int*>(ql_sm);                      // by row: one above QL_LARGE is there
   int* odd = mark + QL_ROWS;                                      // something infinite or NaN is there
   float* start = reinterpret_cast<float*>(ql_sm + plan.starts);
   unsigned char* acts = ql_sm + plan.acts;
@@ -249,53 +300,65 @@ q4_linear_kernel(const T* __restrict__ x, long long ld_x, const unsigned char* _
   };
   for (int i = 0; i < plan.stages - 1; ++i) issue();
 
-  // ---- the activations of the slice, eight channels of a row at a time ----
-  const int parts = channels / 8, work = rows * parts;
-  for (int i = threadIdx.x; i < 2 * QL_ROWS; i += threads) mark[i] = 0;
+  // ---- the activations of the slice, eight channels of a row at a time, several loads of a thread in flight ----
+  const int parts = channels / 8, work = rows * parts, row_step = threads / parts, part_step = threads - row_step * parts;
+  if (threadIdx.x < 2 * QL_ROWS) mark[threadIdx.x] = 0;
   __syncthreads();
-  for (int again = 0;; ++again) {
-    bool large = false;
-    for (int i0 = warp * 32; i0 < work; i0 += threads) {
-      const int i = i0 + lane, r = min(i / parts, rows - 1), c = (i - r * parts) * 8, k = k0 + c;
-      float f[8], sum = 0.f;
+  int again = 0;
+  for (bool large = true; large; ++again) {
+    large = false;
+    int r = threadIdx.x / parts, c = threadIdx.x - r * parts;
+    for (int i0 = warp * 32; i0 < work; i0 += QL_BATCH<T> * threads) {
+      typename QlRaw<T>::type raw[QL_BATCH<T>];
+      int rb[QL_BATCH<T>], cb[QL_BATCH<T>];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = 0.f;
-      if (i < work && k < s.d_in) ql_load8<T>(x + (row0 + r) * ld_x + k, f);
-      const float by = again && mark[r] ? ql_pow2(QL_UP - QL_DOWN) : ql_pow2(QL_UP);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (!ql_finite(f[j])) { odd[r] = 1; f[j] = 0.f; }
-        if (!again && fabsf(f[j]) > QL_LARGE) { mark[r] = 1; large = true; }
-        f[j] *= by;
-        sum += f[j] * ql_pow2(-64);         // a sum of numbers up to 2^127
+      for (int u = 0; u < QL_BATCH<T>; ++u) {
+        rb[u] = min(r, rows - 1);
+        cb[u] = c * 8;
+        raw[u] = {};
+        if (i0 + u * threads + lane < work && k0 + c * 8 < s.d_in) raw[u] = QlRaw<T>::load(x + (row0 + r) * ld_x + k0 + c * 8);
+        r += row_step;
+        c += part_step;
+        if (c >= parts) { c -= parts; ++r; }
       }
 #pragma unroll
-      for (int o = 1; o < GROUP / 8; o *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (i >= work) continue;
-      if (P == 1 && (c & (GROUP - 1)) == 0) start[(c / GROUP) * (NT * 8) + r] = sum * ql_pow2(64 - QL_RAW) * -8.f;
-      unsigned char* dst = acts + r * pitch + c * 2;
-      {
-        uint32_t p[8][3];
+      for (int u = 0; u < QL_BATCH<T>; ++u) {
+        if (i0 + u * threads >= work) break;                      // the same for the whole warp
+        const int row = rb[u];
+        uint4 out[P];
+        float sum;
+        if (QlRaw<T>::plain(raw[u]) && !(again && mark[row])) {
+          sum = QlRaw<T>::plain_pieces(raw[u], out);
+        } else {
+          // something large, infinite or NaN
+          const float by = again && mark[row] ? ql_pow2(QL_UP - QL_DOWN) : ql_pow2(QL_UP);
+          float f[8];
+          uint32_t p[8][3];
+          QlRaw<T>::widen(raw[u], f);
+          sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (j & 2) f[j] *= 0.0625f;                             // its code weighs 16
-          if constexpr (P == 1) p[j][0] = __float_as_uint(f[j]) >> 16;
-          else ql_split(f[j], p[j]);
+          for (int j = 0; j < 8; ++j) {
+            if (!ql_finite(f[j])) { odd[row] = 1; f[j] = 0.f; }
+            if (!again && fabsf(f[j]) > QL_LARGE) { mark[row] = 1; large = true; }
+            f[j] *= by;
+            sum += f[j] * ql_pow2(-QL_UP);
+            ql_split(f[j] * (j & 2 ? 0.0625f : 1.f), p[j]);
+          }
+#pragma unroll
+          for (int q = 0; q < P; ++q) out[q] = make_uint4(p[0][q] | p[1][q] << 16, p[2][q] | p[3][q] << 16, p[4][q] | p[5][q] << 16, p[6][q] | p[7][q] << 16);
         }
 #pragma unroll
-        for (int q = 0; q < P; ++q)
-          *reinterpret_cast<uint4*>(dst + q * plane) = make_uint4(p[0][q] | p[1][q] << 16, p[2][q] | p[3][q] << 16, p[4][q] | p[5][q] << 16, p[6][q] | p[7][q] << 16);
+        for (int o = 1; P == 1 && o < GROUP / 8; o *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (i0 + u * threads + lane >= work) continue;
+        if (P == 1 && (cb[u] & (GROUP - 1)) == 0) start[(cb[u] / GROUP) * (NT * 8) + row] = sum * (ql_pow2(QL_UP - QL_RAW) * -8.f);
+#pragma unroll
+        for (int q = 0; q < P; ++q) *reinterpret_cast<uint4*>(acts + q * plane + row * pitch + cb[u] * 2) = out[q];
       }
     }
-    if (again || !__syncthreads_or(large)) break;
-  }
-  __syncthreads();
-  if (threadIdx.x < rows) {
-    factor[threadIdx.x] = mark[threadIdx.x] ? ql_pow2(QL_DOWN) : 1.f;
+    large = __syncthreads_or(large && !again);
   }
   bool any_odd = false;
   for (int r = 0; r < rows; ++r) any_odd |= odd[r] != 0;
-  __syncthreads();
 
   const unsigned char* mine[NT];                                  // rows past the last one repeat it; nobody looks at their sums
 #pragma unroll
@@ -393,7 +456,7 @@ q4_linear_kernel(const T* __restrict__ x, long long ld_x, const unsigned char* _
       for (int e = 0; e < 2; ++e) {
         const int r = n * 8 + 2 * tig + e;
         if (r >= rows) continue;
-        const float by = factor[r];
+        const float by = mark[r] ? ql_pow2(QL_DOWN) : 1.f;
         float* dst = red + (wk * rows + r) * width + wn * 32 + gid;
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
