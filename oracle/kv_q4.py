@@ -67,8 +67,9 @@ class Q4CacheOracle:
     def forward_cached(self, q, k, v):
         """-> (merged [rows, H * hd] f64, how far a bf16 result may be off, elementwise).
 
-        The device rounds the rotated query, the weights and the values to bf16 (half a step: 2^-9 of each) and the result once more.  A score
-        is then off by at most d = 2^-9 sum |q_c k_c| / sqrt(hd), the weights by e^(2 d) - 1 of themselves, and the rest adds up.
+        The device rounds the rotated query to f16 (half a step: 2^-11 of it), the values to bf16 (2^-8 of each), the weights to two bf16
+        numbers (2^-16), and the result to bf16.  A score is then off by at most d = 2^-11 sum |q_c k_c| / sqrt(hd), and a little for
+        the sums in 32 bits; the weights by e^(2 d) - 1 of themselves, and the rest adds up.
         """
         first, n = len(self), q.shape[0]
         self.append(k, v)
@@ -80,9 +81,9 @@ class Q4CacheOracle:
             for h in range(self.H):
                 keys, values = self.keys[:see, h // group].astype(np.float64), self.values[:see, h // group].astype(np.float64)
                 s = keys @ q[i, h] / np.sqrt(self.hd)
-                d = (np.abs(keys) @ np.abs(q[i, h]) / np.sqrt(self.hd) * 2.0 ** -9).max()
+                d = (np.abs(keys) @ np.abs(q[i, h]) / np.sqrt(self.hd) * (2.0 ** -11 + 2.0 ** -18)).max()
                 p = np.exp(s - s.max())
                 p /= p.sum()
                 out[i, h] = p @ values
-                tol[i, h] = (p @ np.abs(values)) * (np.expm1(2 * d) + 2.0 ** -8 + 2.0 ** -14) + np.abs(out[i, h]) * 2.0 ** -9 + 1e-30
+                tol[i, h] = (p @ np.abs(values)) * (np.expm1(2 * d) + 2.0 ** -8 + 2.0 ** -14) + np.abs(out[i, h]) * 2.0 ** -8 + 1e-30
         return out.reshape(n, -1), tol.reshape(n, -1)

@@ -13,8 +13,11 @@
 // factor makes up for the 2^-133, and for the 16 at the places that have it.
 //   keys:   S = sum over groups of step * sum_c code q + base * sum_c q.  The first product takes its step in f32; the second part, bases
 //           against the queries' sums in three bf16 pieces, is one more small product on the tensor cores.  Nothing of the key is rounded.
+//           The codes enter as f16 numbers (bits * 2^-24, linear in the same way), the query as f16 under a power of two of its own: one
+//           rounding of 2^-11 of a channel at most, where bf16 has 2^-8.
 //   values: step and base belong to the position, which is what the product sums over, so they go on before it: one packed bf16
-//           instruction, one rounding of the value to bf16 (2^-9 of it; P is rounded alike).
+//           instruction, one rounding of the value to bf16 (2^-8 of it at most).  The weights enter as two bf16 numbers each, so that the value's
+//           is the only rounding of that size before the output's: error against 64 bits 2.3e-3 of the output's rms, 3.3e-3 with one.
 // What bounds it is the issue of those instructions: 148 SMs would have to do a page of 64 x 64 channels every 215 cycles to keep up with HBM.
 //
 // Page layout, HD = head_dim, NG = HD / 32:
@@ -26,6 +29,7 @@
 // quantises them into its copy of the page and into the cache: nobody else reads them, so nobody has to wait.
 
 #include <cooperative_groups.h>
+#include <cuda_fp16.h>
 #include <algorithm>
 #include <atomic>
 #include <cfloat>
@@ -42,7 +46,8 @@ constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr float RISE = 8.f;                     // weights stay below 2^8 against the reference
 constexpr float HUGE_VALUE = 1.099511627776e12f; // 2^40: a larger number counts as an infinity (a step times 2^STEP_UP is a bf16 number)
 constexpr int RAW = 133;                        // bits 0 .. 7 of a bf16 are worth bits * 2^-RAW
-constexpr int Q_UP = 80, STEP_UP = 90;          // queries times 2^Q_UP against raw key codes; value steps
+constexpr int STEP_UP = 90;                     // value steps are kept times 2^STEP_UP against raw codes
+constexpr int RAW_HALF = 24, Q_TOP = 13;        // bits 0 .. 7 of an f16: bits * 2^-24; a query's largest channel is in [2^13, 2^14) there
 __host__ __device__ constexpr float pow2(int e) {
   float v = 1.f;
   for (int i = 0; i < (e < 0 ? -e : e); ++i) v *= e < 0 ? 0.5f : 2.f;
@@ -205,7 +210,18 @@ __device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uin
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// the same from zero
+// f16 operands; the second one from zero
+__device__ __forceinline__ void mma16816_half(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816_half_new(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+// bf16 operands from zero
 __device__ __forceinline__ void mma16816_new(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
@@ -246,7 +262,7 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   return r;
 }
 
-// codes i and i + 4 of a word as raw bf16 numbers, of weight 16 where i is odd
+// codes i and i + 4 of a word as raw bf16 or f16 numbers, of weight 16 where i is odd
 template <int I>
 __device__ __forceinline__ uint32_t raw_pair(uint32_t w) { return (I < 2 ? w : w >> 8) & (I & 1 ? 0x00f000f0u : 0x000f000fu); }
 __device__ __forceinline__ __nv_bfloat162 as_pair(uint32_t v) { return *reinterpret_cast<const __nv_bfloat162*>(&v); }
@@ -298,23 +314,28 @@ __device__ __forceinline__ Words<N> load_words(const unsigned char* p) {
 // Half pages in a warp's ring.
 template <int HD> struct Ring { static constexpr int SLOTS = HD <= 64 ? 4 : 3; };
 
-// The queries' fragments and the pieces of their sums, then per warp: the ring, and the new positions of one page (at most QT of them) until
+// The queries' fragments, the pieces of their sums and their factors, then per warp: the ring, and the new positions of one page (at most QT of them) until
 // the page has come: key words, value codes, steps and bases.  In the end the partial results take the place of all that.
 template <int HD, int NQ> struct Smem {
   static constexpr int NG = Layout<HD>::NG, NP = NG == 1 ? 1 : NG / 2;
-  static constexpr int QUERIES = NQ * NG * 512, SUMS = NQ * NP * 128, FRONT = QUERIES + SUMS;
+  static constexpr int QUERIES = NQ * NG * 512, SUMS = NQ * NP * 128, FACTORS = QUERIES + SUMS, FRONT = FACTORS + (NQ * 32 + 127) / 128 * 128;
   static constexpr int RING = Ring<HD>::SLOTS * Layout<HD>::HALF, ROW = HD / 2 + HD + 8 * NG, NEW = NQ * 8 * ROW, WARP = RING + (NEW + 127) / 128 * 128;
   static constexpr int MERGE = NQ * 8 * (WARPS + 1) * (HD + 2) * 4;
   static constexpr int BYTES = FRONT + WARPS * WARP > MERGE ? FRONT + WARPS * WARP : MERGE;
 };
 
 // grid: ((sequence * kv heads + kv head) * passes + pass) * splits + split; the splits of one are a cluster when `joins` is set
-template <int HD, int NQ>
+// FOLD: the last eight columns hold at most four queries, twice.  In the products with the values the first four of them have the upper
+// parts of the weights and the last four the lower ones, so the second parts cost no products of their own.
+template <int HD, int NQ, bool FOLD>
 __global__ void __launch_bounds__(THREADS)
 attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v, int first, int rows, int splits, int slice,
                  int passes, int append, int joins, float scale_log2, bf16* __restrict__ merged, float* __restrict__ part) {
   using L = Layout<HD>;
-  constexpr int NG = L::NG, CT = HD / 16, SLOTS = Ring<HD>::SLOTS, PW = HD + 2, QT = NQ * 8;
+  constexpr int NG = L::NG, CT = HD / 16, SLOTS = Ring<HD>::SLOTS, PW = HD + 2, QT = NQ * 8 - (FOLD ? 4 : 0);
+  // Two tiles of queries of 128 channels are read again for each product: held in registers, 32 of them, they leave the rest too few
+  // (12 queries, 16 sequences of up to 32767 positions: 138 us against 144).
+  constexpr bool FAR = HD == 128 && NQ == 2;
   extern __shared__ __align__(128) unsigned char sm[];
   const int block = blockIdx.x / splits, split = blockIdx.x - block * splits, head_at = block / passes, pass = block - head_at * passes;
   const int sj = head_at / c.Hkv, kvh = head_at - sj * c.Hkv, seq = first + sj;
@@ -391,10 +412,12 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
     const bool wide = (reinterpret_cast<uintptr_t>(q) & 15) == 0;     // a head's row is a multiple of 16 bytes
     uint4* frag = reinterpret_cast<uint4*>(sm);
     uint16_t* sums = reinterpret_cast<uint16_t*>(sm + M::QUERIES);
+    float* factors = reinterpret_cast<float*>(sm + M::FACTORS);
+    constexpr int EIGHTS = (QT * HD / 8 + 31) / 32 * 32;              // whole warps: their lanes shuffle
 #pragma unroll
-    for (int i0 = 0; i0 < QT * HD / 8; i0 += THREADS) {
+    for (int i0 = 0; i0 < EIGHTS; i0 += THREADS) {
       const int i = i0 + THREADS - 32 - (int)(threadIdx.x & ~31u) + lane, at = i / (HD / 8), ch = 8 * (i % (HD / 8)), g = ch / 32, t = (ch / 8) & 3;
-      if (QT * HD / 8 < THREADS && i >= QT * HD / 8) break;           // whole warps; the first ones have new positions to see to
+      if (EIGHTS % THREADS != 0 && i >= EIGHTS) break;                // the first warps have new positions to see to
       const int qi = q0 + at, ok = qi < nq, r = ok ? qi / group : 0, h = ok ? qi - r * group : 0;
       const bf16* src = q + (((long long)sj * rows + r) * c.H + kvh * group + h) * HD;
       const int low = ch < HD / 2, f = low ? ch : ch - HD / 2;
@@ -413,18 +436,31 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = low ? x[j] * co[j] - other[j] * si[j] : x[j] * co[j] + other[j] * si[j];
       }
+      // the power of two that takes the query's largest channel to Q_TOP, and what makes up for it in the scores
+      float top = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[j]));
+#pragma unroll
+      for (int d = 1; d < HD / 8; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 100);
+      const float by = __uint_as_float((uint32_t)(127 + Q_TOP - e) << 23);
+      if (i % (HD / 8) == 0) factors[at] = scale_log2 * __uint_as_float((uint32_t)(127 + RAW_HALF - Q_TOP + e) << 23);
       uint32_t w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const __nv_bfloat162 p = __floats2bfloat162_rn(x[2 * j] * scale_log2, x[2 * j + 1] * scale_log2);
-        w[j] = as_bits(__hmul2(p, __float2bfloat162_rn(pow2(j & 1 ? Q_UP - 4 : Q_UP))));
+        __half2 p = __floats2half2_rn(x[2 * j] * by, x[2 * j + 1] * by);
         sum += __low2float(p) + __high2float(p);
+        if (j & 1) p = __hmul2(p, __float2half2_rn(0.0625f));
+        w[j] = *reinterpret_cast<const uint32_t*>(&p);
       }
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      sum *= pow2(Q_UP - RAW);
+      sum *= pow2(-RAW_HALF);
+      if (FOLD && at >= QT) continue;                                 // no such query
       const int nt = at >> 3, to = (at & 7) * 4 + t;                  // the lane that multiplies these channels
       frag[(nt * NG + g) * 32 + to] = make_uint4(w[0], w[1], w[2], w[3]);
+      const bool twice = FOLD && nt == NQ - 1;
+      if (twice) frag[(nt * NG + g) * 32 + to + 16] = make_uint4(w[0], w[1], w[2], w[3]);
       // the sum as three bf16 numbers, one for each of the lanes t = 0, 1, 2
       const bf16 s0 = __float2bfloat16_rn(sum), s1 = __float2bfloat16_rn(sum - __bfloat162float(s0));
       const bf16 s2 = __float2bfloat16_rn(sum - __bfloat162float(s0) - __bfloat162float(s1));
@@ -435,6 +471,10 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
         d[1] = __bfloat16_as_ushort(piece);
       } else {
         d[g & 1] = __bfloat16_as_ushort(piece);
+      }
+      if (twice) {
+        if (NG == 1) d[32] = 0;
+        d[32 + (NG == 1 ? 1 : g & 1)] = __bfloat16_as_ushort(piece);
       }
     }
   }
@@ -447,29 +487,33 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
     }
   }
   uint32_t qf[NQ][NG][4], qb[NQ][M::NP];              // fragments; pieces of the sums
+  float factor[NQ][2];                                // from the products' units to powers of two, of queries 2 tig and 2 tig + 1
   int lim[NQ][2];                                     // positions that queries 2 tig and 2 tig + 1 see
+  auto load_query = [&](int nt, int g) {
+    const uint4 w = reinterpret_cast<const uint4*>(sm)[(nt * NG + g) * 32 + lane];
+    qf[nt][g][0] = w.x; qf[nt][g][1] = w.y; qf[nt][g][2] = w.z; qf[nt][g][3] = w.w;
+  };
 #pragma unroll
   for (int nt = 0; nt < NQ; ++nt) {
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const uint4 w = reinterpret_cast<const uint4*>(sm)[(nt * NG + g) * 32 + lane];
-      qf[nt][g][0] = w.x; qf[nt][g][1] = w.y; qf[nt][g][2] = w.z; qf[nt][g][3] = w.w;
-    }
+    for (int g = 0; g < NG; ++g)
+      if (!FAR) load_query(nt, g);
 #pragma unroll
     for (int j = 0; j < M::NP; ++j) {
       qb[nt][j] = reinterpret_cast<const uint32_t*>(sm + M::QUERIES)[(nt * M::NP + j) * 32 + lane];
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int qe = q0 + nt * 8 + 2 * tig + e;
+      const int at = nt * 8 + (FOLD && nt == NQ - 1 ? 2 * tig & 3 : 2 * tig) + e, qe = q0 + at;
+      factor[nt][e] = reinterpret_cast<const float*>(sm + M::FACTORS)[at];
       lim[nt][e] = qe < nq ? len + qe / group + 1 : 0;
     }
   }
   const int all_see = len + q0 / group + 1;           // positions below this are seen by every query of the pass
+  const uint32_t lower = tig >= 2 ? ~0u : 0u;         // FOLD: this lane's columns have the lower parts
 
   // A weight is 2^(score - ref): ref is the maximum when it was last looked up and stays until a score passes it
-  // by RISE; until then neither the sums nor the products have to be scaled.  Scores and ref are kept times 2^(Q_UP - RAW), values times
-  // 2^(STEP_UP - RAW).
+  // by RISE; until then neither the sums nor the products have to be scaled.  Values are kept times 2^(STEP_UP - RAW).
   float ref[NQ][2], l[NQ][2], o[NQ][CT][4];
 
 #pragma unroll
@@ -531,8 +575,9 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
 #pragma unroll
         for (int nt = 0; nt < NQ; ++nt) {
           float acc[4];
-          mma16816_new(acc, a0, a1, a2, a3, qf[nt][g][0], qf[nt][g][1]);
-          mma16816(acc, b0, b1, b2, b3, qf[nt][g][2], qf[nt][g][3]);
+          if (FAR) load_query(nt, g);
+          mma16816_half_new(acc, a0, a1, a2, a3, qf[nt][g][0], qf[nt][g][1]);
+          mma16816_half(acc, b0, b1, b2, b3, qf[nt][g][2], qf[nt][g][3]);
           s[nt][mt][0] = fmaf(st0, acc[0], s[nt][mt][0]);
           s[nt][mt][1] = fmaf(st0, acc[1], s[nt][mt][1]);
           s[nt][mt][2] = fmaf(st1, acc[2], s[nt][mt][2]);
@@ -550,7 +595,7 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
           for (int e = 0; e < 4; ++e)
             if (pg * PAGE + 16 * mt + gid + 8 * (e >> 1) >= lim[nt][e & 1]) s[nt][mt][e] = -INFINITY;
     }
-    uint32_t p[NQ][4][2];
+    uint32_t p[NQ][4][2], p_lo[NQ][4][2];             // the weights as two bf16 numbers each
     bool rise = false;
     float mx[NQ][2];
 #pragma unroll
@@ -561,7 +606,7 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
 #pragma unroll
         for (int mt = 1; mt < 4; ++mt) a = fmaxf(a, fmaxf(s[nt][mt][e], s[nt][mt][e + 2]));
         mx[nt][e] = a;
-        rise |= a > ref[nt][e] + RISE * pow2(Q_UP - RAW);
+        rise |= fmaf(a, factor[nt][e], -ref[nt][e]) > RISE;
       }
     if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
@@ -572,8 +617,8 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
           a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 4));
           a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 8));
           a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 16));
-          a = fmaxf(a, ref[nt][e]);
-          const float corr = a > -INFINITY ? ex2((ref[nt][e] - a) * pow2(RAW - Q_UP)) : 1.f;
+          a = fmaxf(a * factor[nt][e], ref[nt][e]);
+          const float corr = a > -INFINITY ? ex2(ref[nt][e] - a) : 1.f;
           ref[nt][e] = a;
           l[nt][e] *= corr;
 #pragma unroll
@@ -582,9 +627,10 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
     }
 #pragma unroll
     for (int nt = 0; nt < NQ; ++nt) {
+      const bool fold = FOLD && nt == NQ - 1;
       // a query that has seen nothing yet has scores of -inf only: weights of 0 against any finite number
-      const uint64_t up = pack2(pow2(RAW - Q_UP), pow2(RAW - Q_UP));
-      const uint64_t minus = pack2(ref[nt][0] > -INFINITY ? ref[nt][0] * -pow2(RAW - Q_UP) : 0.f, ref[nt][1] > -INFINITY ? ref[nt][1] * -pow2(RAW - Q_UP) : 0.f);
+      const uint64_t up = pack2(factor[nt][0], factor[nt][1]);
+      const uint64_t minus = pack2(ref[nt][0] > -INFINITY ? -ref[nt][0] : 0.f, ref[nt][1] > -INFINITY ? -ref[nt][1] : 0.f);
       uint64_t sum = pack2(l[nt][0], l[nt][1]);
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt)
@@ -594,7 +640,10 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
           unpack2(fma2(pack2(s[nt][mt][2 * h], s[nt][mt][2 * h + 1]), up, minus), y0, y1);
           const float w0 = ex2(y0), w1 = ex2(y1);
           sum = add2(sum, pack2(w0, w1));
-          p[nt][mt][h] = transpose8x8(as_bits(__floats2bfloat162_rn(w0, w1)));
+          const uint32_t w = as_bits(__floats2bfloat162_rn(w0, w1)), less = fold ? w & lower : w;
+          const uint32_t rest = as_bits(__floats2bfloat162_rn(w0 - __uint_as_float(less << 16), w1 - __uint_as_float(less & 0xffff0000u)));
+          p[nt][mt][h] = transpose8x8(fold ? rest : w);
+          if (!fold) p_lo[nt][mt][h] = transpose8x8(rest);
         }
       unpack2(sum, l[nt][0], l[nt][1]);
     }
@@ -641,6 +690,10 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
           for (int nt = 0; nt < NQ; ++nt) {
             mma16816(o[nt][ct], a0, a1, a2, a3, p[nt][2 * w][0], p[nt][2 * w][1]);
             mma16816(o[nt][ct], b0, b1, b2, b3, p[nt][2 * w + 1][0], p[nt][2 * w + 1][1]);
+            if (!FOLD || nt < NQ - 1) {
+              mma16816(o[nt][ct], a0, a1, a2, a3, p_lo[nt][2 * w][0], p_lo[nt][2 * w][1]);
+              mma16816(o[nt][ct], b0, b1, b2, b3, p_lo[nt][2 * w + 1][0], p_lo[nt][2 * w + 1][1]);
+            }
           }
         }
       }
@@ -656,6 +709,13 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
       l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 16);
     }
 
+  if (FOLD) {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[NQ - 1][ct][e] += __shfl_xor_sync(0xffffffffu, o[NQ - 1][ct][e], 2);
+  }
+
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // ---- join the warps: [query][warp][HD + 2], then this slice's [query][HD + 2] behind it ----
   float* mb = reinterpret_cast<float*>(sm);
@@ -663,6 +723,7 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
   __syncthreads();                                    // every ring is drained
 #pragma unroll
   for (int nt = 0; nt < NQ; ++nt) {
+    if (FOLD && nt == NQ - 1 && tig >= 2) break;                      // the others have it all
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
@@ -672,7 +733,7 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float* d = mb + ((nt * 8 + 2 * tig + e) * WARPS + warp) * PW + HD;
-        d[0] = ref[nt][e] * pow2(RAW - Q_UP);
+        d[0] = ref[nt][e];
         d[1] = l[nt][e];
       }
     }
@@ -820,11 +881,11 @@ __global__ void values_kernel(Cache c, int first, int from, int count, float* __
   }
 }
 
-template <int HD, int NQ>
+template <int HD, int NQ, bool FOLD = false>
 cudaError_t go(const Cache& c, const bf16* q, const bf16* k, const bf16* v, int first, int n_seq, int rows, int splits, int slice, bool append, float scale_log2,
                bf16* merged, float* part, cudaStream_t st) {
   constexpr int smem = Smem<HD, NQ>::BYTES;
-  auto kernel = attention_kernel<HD, NQ>;
+  auto kernel = attention_kernel<HD, NQ, FOLD>;
   const int nq = rows * (c.H / c.Hkv), passes = (nq + NQ * 8 - 1) / (NQ * 8);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(splits * passes * c.Hkv * n_seq));
@@ -880,26 +941,27 @@ int queries_per_pass(int head_dim, int queries) { return queries <= 8 || head_di
 
 cudaError_t launch_attention(const Cache& c, const bf16* q, const bf16* k, const bf16* v, int first, int n_seq, int rows, int splits, int slice, bool append,
                              float scale_log2, bf16* merged, float* part, cudaStream_t st) {
-  const bool two = queries_per_pass(c.HD, rows * (c.H / c.Hkv)) == 16;
-#define Q4_GO(HD, NQ) go<HD, NQ>(c, q, k, v, first, n_seq, rows, splits, slice, append, scale_log2, merged, part, st)
+  const int nq = rows * (c.H / c.Hkv);
+  const bool two = queries_per_pass(c.HD, nq) == 16, fold = nq <= (two ? 12 : 4);
+#define Q4_GO(HD, ...) go<HD, __VA_ARGS__>(c, q, k, v, first, n_seq, rows, splits, slice, append, scale_log2, merged, part, st)
   switch (c.HD) {
-    case 32: return two ? Q4_GO(32, 2) : Q4_GO(32, 1);
-    case 64: return two ? Q4_GO(64, 2) : Q4_GO(64, 1);
-    case 128: return two ? Q4_GO(128, 2) : Q4_GO(128, 1);
-    case 256: return Q4_GO(256, 1);
+    case 32: return two ? (fold ? Q4_GO(32, 2, true) : Q4_GO(32, 2)) : fold ? Q4_GO(32, 1, true) : Q4_GO(32, 1);
+    case 64: return two ? (fold ? Q4_GO(64, 2, true) : Q4_GO(64, 2)) : fold ? Q4_GO(64, 1, true) : Q4_GO(64, 1);
+    case 128: return two ? (fold ? Q4_GO(128, 2, true) : Q4_GO(128, 2)) : fold ? Q4_GO(128, 1, true) : Q4_GO(128, 1);
+    case 256: return fold ? Q4_GO(256, 1, true) : Q4_GO(256, 1);
     default: return cudaErrorInvalidValue;
   }
 #undef Q4_GO
 }
 
-template <int HD, int NQ>
+template <int HD, int NQ, bool FOLD = false>
 int resident(int device) {
   static std::atomic<int> known[64] = {};             // per device, plus one
   std::atomic<int>& slot = known[device & 63];
   if (const int n = slot.load(std::memory_order_relaxed)) return n - 1;
   int per_sm = 0;
-  cudaFuncSetAttribute(attention_kernel<HD, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<HD, NQ>::BYTES);
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, attention_kernel<HD, NQ>, THREADS, Smem<HD, NQ>::BYTES) != cudaSuccess) {
+  cudaFuncSetAttribute(attention_kernel<HD, NQ, FOLD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<HD, NQ>::BYTES);
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, attention_kernel<HD, NQ, FOLD>, THREADS, Smem<HD, NQ>::BYTES) != cudaSuccess) {
     cudaGetLastError();
     per_sm = 1;
   }
@@ -908,12 +970,12 @@ int resident(int device) {
 }
 
 int ctas_per_sm(int head_dim, int queries, int device) {
-  const bool two = queries_per_pass(head_dim, queries) == 16;
+  const bool two = queries_per_pass(head_dim, queries) == 16, fold = queries <= (two ? 12 : 4);
   switch (head_dim) {
-    case 32: return two ? resident<32, 2>(device) : resident<32, 1>(device);
-    case 64: return two ? resident<64, 2>(device) : resident<64, 1>(device);
-    case 128: return two ? resident<128, 2>(device) : resident<128, 1>(device);
-    default: return resident<256, 1>(device);
+    case 32: return two ? (fold ? resident<32, 2, true>(device) : resident<32, 2>(device)) : fold ? resident<32, 1, true>(device) : resident<32, 1>(device);
+    case 64: return two ? (fold ? resident<64, 2, true>(device) : resident<64, 2>(device)) : fold ? resident<64, 1, true>(device) : resident<64, 1>(device);
+    case 128: return two ? (fold ? resident<128, 2, true>(device) : resident<128, 2>(device)) : fold ? resident<128, 1, true>(device) : resident<128, 1>(device);
+    default: return fold ? resident<256, 1, true>(device) : resident<256, 1>(device);
   }
 }
 

@@ -19,7 +19,7 @@ def test_the_format_rounds_to_the_nearest_of_sixteen_values():
     assert np.array_equal(y[3, 1], x[3, 1])                                # a constant group is its base
     g = x.reshape(50, 3, 2, 32)
     spread = (g.max(-1) - g.min(-1)).repeat(32, axis=-1).reshape(x.shape)
-    # half a step, the base's rounding (2^-9 of it) and the step's over fifteen steps
+    # half a step, the base's rounding (2^-8 of it) and the step's over fifteen steps
     assert (np.abs(y - x) <= spread / 30 * 1.01 + np.abs(x).max() * 2.0 ** -8).all()
     assert np.array_equal(to_bf16(np.float32([1.00390625, -1.01171875])), np.float32([1.0, -1.015625]))      # ties to even
 
