@@ -95,6 +95,17 @@ int32_t lm_get_grad(lm_model_t* model, int32_t layer, int32_t which, int32_t exp
 int32_t lm_forward_logits(lm_model_t* model, const uint32_t* ids_host, const int32_t* lengths_host, int32_t batch,
                           int32_t seq_len, float* logits_host, float* moe_logits_host);
 
+/* forward_batch without its logits: what the model gives to the tokens of the batch (logprobs_b200.h on the logits where they are, with their
+ * edge values).  Row r of a sequence scores the token that follows it:
+ *   logprob_host [batch * seq_len]         log p(token r + 1 | tokens 0 .. r), 0 where none follows or the mask leaves it out;
+ *   entropy_host [batch * seq_len]         of that distribution; optional;
+ *   top_logprob_host, top_ids_host [batch * seq_len, top_n]   the most likely tokens, 0 <= top_n <= min(vocab, LOGPROBS_MAX_TOP); null when
+ *                                          top_n is 0.
+ * A sequence's last row has an entropy and alternatives; rows behind it have 0, 0 and ids of -1.  The mean of -logprob over the predicted
+ * rows is lm_accumulate_step's lm_loss. */
+int32_t lm_score(lm_model_t* model, const uint32_t* ids_host, const int32_t* lengths_host, const uint8_t* loss_mask_host, int32_t batch,
+                 int32_t seq_len, int32_t top_n, float* logprob_host, float* entropy_host, float* top_logprob_host, int32_t* top_ids_host);
+
 /* accumulate_step: forward, fused head + loss, backward into the gradients (no optimizer step). */
 int32_t lm_accumulate_step(lm_model_t* model, const uint32_t* ids_host, const int32_t* lengths_host,
                            const uint8_t* loss_mask_host, int32_t batch, int32_t seq_len, float* lm_loss,
@@ -121,6 +132,8 @@ int32_t lm_set_optimizer_step(lm_model_t* model, int64_t step);
  * logits_host [n_sequences * rows_per_sequence, vocab] f32.  SequenceTooLong -> MOE_INVALID_INPUT, nothing appended. */
 typedef struct lm_decoder lm_decoder_t;
 int32_t lm_decoder_create(lm_model_t* model, int32_t sequences, int32_t capacity, lm_decoder_t** out);
+/* The same with the caches in 4 bits (MOE_PRECISION_Q4 of kv_attention_b200.h): a third of the bytes; head_dim 32, 64, 128 or 256. */
+int32_t lm_decoder_create_q4(lm_model_t* model, int32_t sequences, int32_t capacity, lm_decoder_t** out);
 void lm_decoder_destroy(lm_decoder_t* decoder);
 /* KvCache::clear for every layer: one sequence, or all of them when sequence < 0. */
 int32_t lm_decoder_clear(lm_model_t* model, lm_decoder_t* decoder, int32_t sequence);

@@ -128,6 +128,7 @@ def lib() -> C.CDLL:
         "lm_get_param": (i32, [vp, i32, i32, i32, vp, i32, i32]),
         "lm_get_grad": (i32, [vp, i32, i32, i32, vp, i32, i32]),
         "lm_forward_logits": (i32, [vp, vp, vp, i32, i32, vp, vp]),
+        "lm_score": (i32, [vp, vp, vp, vp, i32, i32, i32, vp, vp, vp, vp]),
         "lm_accumulate_step": (i32, [vp, vp, vp, vp, i32, i32, fp, fp]),
         "lm_zero_grad": (i32, [vp]),
         "lm_step_adam": (i32, [vp, f32, f32, f32, f32, f32, f32]),
@@ -137,6 +138,7 @@ def lib() -> C.CDLL:
         "lm_optimizer_step": (C.c_int64, [vp]),
         "lm_set_optimizer_step": (i32, [vp, C.c_int64]),
         "lm_decoder_create": (i32, [vp, i32, i32, C.POINTER(vp)]),
+        "lm_decoder_create_q4": (i32, [vp, i32, i32, C.POINTER(vp)]),
         "lm_decoder_destroy": (None, [vp]),
         "lm_decoder_clear": (i32, [vp, vp, i32]),
         "lm_forward_cached": (i32, [vp, vp, vp, i32, i32, i32, vp]),

@@ -18,6 +18,7 @@
 #include <string>
 #include <vector>
 
+#include "../../include/logprobs_b200.h"
 #include "../../include/moe_b200.h"
 #include "../../include/rmsnorm_b200.h"
 #include "../../include/transformer_b200.h"
@@ -838,6 +839,46 @@ int32_t lm_forward_logits(lm_model_t* M, const uint32_t* ids, const int32_t* len
   return MOE_OK;
 }
 
+int32_t lm_score(lm_model_t* M, const uint32_t* ids, const int32_t* lengths, const uint8_t* mask, int32_t B, int32_t S, int32_t top_n,
+                 float* logprob_host, float* entropy_host, float* top_logprob_host, int32_t* top_ids_host) {
+  LENTER(M);
+  if (top_n < 0 || top_n > std::min(LOGPROBS_MAX_TOP, M->V))
+    return lfail(M, MOE_INVALID_INPUT, "InvalidInput: top_n is 0 .. %d, got %d", std::min(LOGPROBS_MAX_TOP, M->V), top_n);
+  if (!logprob_host || (top_n > 0 && (!top_logprob_host || !top_ids_host))) return lfail(M, MOE_INVALID_INPUT, "InvalidInput: null result buffer");
+  Batch bt;
+  RC(prepare_batch(M, ids, lengths, mask, B, S, false, &bt));
+  RC(ensure_attention(M, bt));
+  RC(forward_blocks(M, bt, false));
+  RC(mm_nt(M, M->xf, bt.rows, M->d, M->wb + head_offset(M), M->V_pad, dense_meta(M, bt.rows), M->logits, M->V_pad));
+  // [n] log probabilities, [n] entropies, [n, top_n] alternatives and their ids, a slab of rows at a time through the staging buffer
+  const int slab = (int)std::min<long long>(bt.rows, M->stage_elems / (2 + 2 * top_n));
+  for (int r0 = 0; r0 < bt.rows; r0 += slab) {
+    const int n = std::min(slab, bt.rows - r0);
+    float *lp = M->stage, *h = lp + n, *top = h + n;
+    int* top_ids = (int*)(top + (size_t)n * top_n);
+    char text[160] = "";
+    const int rc = logprobs_forward(M->logits + (size_t)r0 * M->V_pad, M->V_pad, M->targets + r0, n, M->V, top_n, MOE_PRECISION_BF16, lp,
+                                    entropy_host ? h : nullptr, nullptr, top_n ? top : nullptr, top_n ? top_ids : nullptr, M->st, text, sizeof text);
+    if (rc != MOE_OK) return lfail(M, rc, "%s", text);
+    LCK(cudaMemcpyAsync(logprob_host + r0, lp, (size_t)n * 4, cudaMemcpyDeviceToHost, M->st));
+    if (entropy_host) LCK(cudaMemcpyAsync(entropy_host + r0, h, (size_t)n * 4, cudaMemcpyDeviceToHost, M->st));
+    if (top_n) {
+      LCK(cudaMemcpyAsync(top_logprob_host + (size_t)r0 * top_n, top, (size_t)n * top_n * 4, cudaMemcpyDeviceToHost, M->st));
+      LCK(cudaMemcpyAsync(top_ids_host + (size_t)r0 * top_n, top_ids, (size_t)n * top_n * 4, cudaMemcpyDeviceToHost, M->st));
+    }
+    LCK(cudaStreamSynchronize(M->st));
+  }
+  for (int r = 0; r < bt.rows; ++r) {                 // what padding rows would answer means nothing
+    if (M->valid_pin[r]) continue;
+    if (entropy_host) entropy_host[r] = 0.f;
+    for (int j = 0; j < top_n; ++j) {
+      top_logprob_host[(size_t)r * top_n + j] = 0.f;
+      top_ids_host[(size_t)r * top_n + j] = -1;
+    }
+  }
+  return check_device_flag(M);
+}
+
 int32_t lm_accumulate_step(lm_model_t* M, const uint32_t* ids, const int32_t* lengths, const uint8_t* mask, int32_t B, int32_t S,
                            float* lm_loss, float* aux_loss) {
   LENTER(M);
@@ -902,7 +943,7 @@ struct lm_decoder {
 
 extern "C" {
 
-int32_t lm_decoder_create(lm_model_t* M, int32_t sequences, int32_t capacity, lm_decoder_t** out) {
+static int32_t create_decoder(lm_model_t* M, int32_t sequences, int32_t capacity, int32_t precision, lm_decoder_t** out) {
   LENTER(M);
   if (!out) return MOE_INVALID_INPUT;
   *out = nullptr;
@@ -914,7 +955,7 @@ int32_t lm_decoder_create(lm_model_t* M, int32_t sequences, int32_t capacity, lm
   for (int l = 0; l < M->L; ++l) {
     kv_cache_config_t kc{};
     kc.sequences = sequences; kc.num_heads = M->H; kc.kv_heads = M->Hkv; kc.head_dim = M->hd; kc.capacity = capacity;
-    kc.max_seq_len = M->cfg.max_seq_len; kc.rope_base = M->cfg.rope_base; kc.rope = 1; kc.precision = MOE_PRECISION_BF16; kc.device = M->device;
+    kc.max_seq_len = M->cfg.max_seq_len; kc.rope_base = M->cfg.rope_base; kc.rope = 1; kc.precision = precision; kc.device = M->device;
     kv_cache_t* c = nullptr;
     const int rc = kv_cache_create(&kc, &c);
     if (rc != MOE_OK) {
@@ -928,6 +969,14 @@ int32_t lm_decoder_create(lm_model_t* M, int32_t sequences, int32_t capacity, lm
   }
   *out = D;
   return MOE_OK;
+}
+
+int32_t lm_decoder_create(lm_model_t* M, int32_t sequences, int32_t capacity, lm_decoder_t** out) {
+  return create_decoder(M, sequences, capacity, MOE_PRECISION_BF16, out);
+}
+
+int32_t lm_decoder_create_q4(lm_model_t* M, int32_t sequences, int32_t capacity, lm_decoder_t** out) {
+  return create_decoder(M, sequences, capacity, MOE_PRECISION_Q4, out);
 }
 
 void lm_decoder_destroy(lm_decoder_t* D) {

@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import ctypes as C
 from dataclasses import dataclass, field, replace
-from typing import Iterable, List, Optional, Sequence, Tuple
+from typing import Iterable, List, NamedTuple, Optional, Sequence, Tuple
 
 import numpy as np
 
@@ -144,6 +144,14 @@ class TokenBatch:
 
     def is_padded(self) -> bool:
         return bool((self.lengths != self.seq_len).any())
+
+
+class BatchScores(NamedTuple):
+    """What ``score_batch`` returns, host arrays of a row per token position: row r scores the token after it."""
+    logprob: np.ndarray                        # f32 [batch * seq_len], 0 where no token follows or the mask leaves it out
+    entropy: np.ndarray                        # f32 [batch * seq_len], 0 behind a sequence's end
+    top_ids: Optional[np.ndarray]              # int32 [batch * seq_len, top], the most likely first; -1 behind a sequence's end
+    top_logprobs: Optional[np.ndarray]         # f32 of the same shape
 
 
 class TransformerBuilder:
@@ -333,6 +341,20 @@ class TransformerLm:
 
     forward_train = forward_batch
 
+    def score_batch(self, batch, top: int = 0) -> BatchScores:
+        """``forward_batch`` reduced on the device to log probabilities of the batch's own tokens, entropies and ``top`` alternatives
+        (at most 32): the logits stay there.  With the batch's loss mask, the masked tokens have none."""
+        b = self._batch(batch)
+        if top < 0:
+            raise InvalidInput("top is 0 or more, got %d" % top)
+        lp, h = np.empty(b.rows, np.float32), np.empty(b.rows, np.float32)
+        ids = np.empty((b.rows, top), np.int32) if top else None
+        tlp = np.empty((b.rows, top), np.float32) if top else None
+        at = lambda a: a.ctypes.data_as(C.c_void_p) if a is not None else None
+        tokens, lengths = self._args(b)
+        self._ck(_lib.lib().lm_score(self._h, tokens, lengths, at(b.loss_mask), b.batch, b.seq_len, top, at(lp), at(h), at(tlp), at(ids)))
+        return BatchScores(lp, h, ids, tlp)
+
     def accumulate_step(self, batch) -> TotalLoss:
         b = self._batch(batch)
         lm, aux = C.c_float(), C.c_float()
@@ -372,9 +394,10 @@ class TransformerLm:
     train_step = train_step_batch
 
     # -- KV-cached decode ---------------------------------------------------------------------------
-    def new_kv_caches(self, sequences: int = 1, capacity: Optional[int] = None) -> "KvCaches":
-        """One cache per layer (transformer.rs:649-660), for ``sequences`` sequences that decode together."""
-        return KvCaches(self, sequences, capacity if capacity is not None else self.config.max_seq_len)
+    def new_kv_caches(self, sequences: int = 1, capacity: Optional[int] = None, precision: str = "bf16") -> "KvCaches":
+        """One cache per layer (transformer.rs:649-660), for ``sequences`` sequences that decode together; ``precision`` "q4" keeps
+        them in 4 bits (head_dim 32, 64, 128 or 256)."""
+        return KvCaches(self, sequences, capacity if capacity is not None else self.config.max_seq_len, precision)
 
     def forward_cached(self, ids, caches: "KvCaches", first_sequence: int = 0) -> np.ndarray:
         """``ids``: one list of new token ids per sequence (equal lengths: the prompts for a prefill, one id each
@@ -411,10 +434,13 @@ class TransformerLm:
 class KvCaches:
     """``Vec<KvCache>`` of the reference, batched over sequences; owned by the caller, tied to one model."""
 
-    def __init__(self, model: TransformerLm, sequences: int, capacity: int):
-        self._model, self.sequences, self.capacity = model, sequences, capacity
+    def __init__(self, model: TransformerLm, sequences: int, capacity: int, precision: str = "bf16"):
+        if precision not in ("bf16", "q4"):
+            raise InvalidConfig("the precision of a model's caches is 'bf16' or 'q4'")
+        self._model, self.sequences, self.capacity, self.precision = model, sequences, capacity, precision
         self._h = C.c_void_p()
-        model._ck(_lib.lib().lm_decoder_create(model._h, sequences, capacity, C.byref(self._h)))
+        create = _lib.lib().lm_decoder_create_q4 if precision == "q4" else _lib.lib().lm_decoder_create
+        model._ck(create(model._h, sequences, capacity, C.byref(self._h)))
 
     def clear(self, sequence: int = -1) -> None:
         self._model._ck(_lib.lib().lm_decoder_clear(self._model._h, self._h, sequence))
@@ -425,4 +451,4 @@ class KvCaches:
             self._h = C.c_void_p()
 
 
-__all__ = ["KvCaches", "Adam", "Sgd", "Lion", "TotalLoss", "TransformerConfig", "TransformerBuilder", "TransformerLm", "TokenBatch", "NetworkError"]
+__all__ = ["BatchScores", "KvCaches", "Adam", "Sgd", "Lion", "TotalLoss", "TransformerConfig", "TransformerBuilder", "TransformerLm", "TokenBatch", "NetworkError"]
