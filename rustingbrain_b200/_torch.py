@@ -7,25 +7,29 @@ import threading
 
 from . import _lib
 
-_local = threading.local()
+class _Local(threading.local):
+    def __init__(self):
+        self.message = C.create_string_buffer(256)
 
 
-def _message():
-    m = getattr(_local, "message", None)
-    if m is None:
-        m = _local.message = C.create_string_buffer(256)
-    return m
+_local = _Local()
+_calls = None                                # torch's current device and current stream, looked up once
 
 
 def issue(fn, tensor, stream, errors, default_error, *args) -> None:
     """``fn(*args, stream, message, message_len)`` with ``tensor``'s device current; raises for a status other than OK."""
-    import torch
+    global _calls
+    if _calls is None:
+        import torch
+        _calls = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+    current, raw_stream = _calls
     index = tensor.get_device()
-    st = torch._C._cuda_getCurrentRawStream(index) if stream is None else int(stream)
-    msg = _message()
-    if torch._C._cuda_getDevice() == index:
+    st = raw_stream(index) if stream is None else int(stream)
+    msg = _local.message
+    if current() == index:
         rc = fn(*args, st, msg, 256)
     else:
+        import torch
         with torch.cuda.device(index):
             rc = fn(*args, st, msg, 256)
     if rc != _lib.OK:

@@ -39,6 +39,7 @@ class KvCache:
                                   rope_base=rope_base, rope=1 if rope else 0,
                                   precision=_PRECISIONS[precision], device=device)
         self.device = device
+        self._dtype = self._raw_stream = None          # torch's, looked up with the first step
         self._forward = _lib.lib().kv_attention_forward_cached
         rc = _lib.lib().kv_cache_create(C.byref(cfg), C.byref(self._h))
         if rc != _lib.OK:
@@ -87,7 +88,6 @@ class KvCache:
                        n_sequences: Optional[int] = None, out=None, stream=None):
         """Device tensors q [rows, num_heads * head_dim] (scratch: may be rotated in place), k and v
         [rows, kv_heads * head_dim], rows = n_sequences * rows_per_sequence; returns the merged heads."""
-        import torch
         n_seq = self.sequences - first_sequence if n_sequences is None else n_sequences
         rows = n_seq * rows_per_sequence
         W = self.kv_heads * self.head_dim
@@ -95,21 +95,26 @@ class KvCache:
         self._rows(k, rows, W, "k")
         self._rows(v, rows, W, "v")
         if out is None:
-            out = torch.empty_like(q)
+            out = q.new_empty(q.shape)
+        else:
+            self._rows(out, rows, self.num_heads * self.head_dim, "out")
         self._check(self._forward(self._h, first_sequence, n_seq, q.data_ptr(), k.data_ptr(), v.data_ptr(), rows_per_sequence,
                                   out.data_ptr(), self._on(stream)))
         return out
 
     def _rows(self, t, rows, width, name) -> None:
-        import torch
-        dt = torch.float32 if self.precision == "f32" else torch.bfloat16
-        if not (t.is_cuda and t.is_contiguous() and t.dtype == dt and tuple(t.shape) == (rows, width)):
-            raise InvalidInput("%s must be a contiguous %s device tensor of shape %s" % (name, dt, (rows, width)))
+        if self._dtype is None:
+            import torch
+            self._dtype = torch.float32 if self.precision == "f32" else torch.bfloat16
+        if not (t.get_device() == self.device and t.is_contiguous() and t.dtype == self._dtype and t.shape == (rows, width)):
+            raise InvalidInput("%s must be a contiguous %s tensor of shape %s on cuda:%d" % (name, self._dtype, (rows, width), self.device))
 
     def _on(self, stream):
         """The given stream, or the current one of the cache's device."""
-        import torch
-        return torch._C._cuda_getCurrentRawStream(self.device) if stream is None else int(stream)
+        if self._raw_stream is None:
+            import torch
+            self._raw_stream = torch._C._cuda_getCurrentRawStream
+        return self._raw_stream(self.device) if stream is None else int(stream)
 
     def append(self, k, v, rows_per_sequence: int = 1, first_sequence: int = 0, n_sequences: Optional[int] = None, stream=None) -> None:
         """``KvCache::append`` (attention.rs:65-78): stores new keys (rotated here) and values without attending to anything."""
@@ -130,7 +135,7 @@ class KvCache:
         import torch
         n_seq = self.sequences - first_sequence if n_sequences is None else n_sequences
         shape = (max(n_seq, 0) * max(rows_per_sequence, 0), self.kv_heads * self.head_dim)
-        keys = torch.empty(shape, dtype=torch.float32, device="cuda:%d" % self.device)
+        keys = torch.empty(shape, dtype=torch.float32, device=self.device)
         values = torch.empty_like(keys)
         self._check(_lib.lib().kv_cache_newest(self._h, first_sequence, n_seq, rows_per_sequence, keys.data_ptr(), values.data_ptr(), self._on(stream)))
         return keys, values

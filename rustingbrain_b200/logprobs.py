@@ -25,20 +25,27 @@ class TokenLogProbs(NamedTuple):
     top_logprobs: Optional["torch.Tensor"]
 
 
+_precisions = {}                             # of torch's types
+
+
 def _check_logits(t, name):
-    import torch
-    if t.dim() != 2 or not t.is_cuda or t.dtype not in (torch.float32, torch.bfloat16):
+    if not _precisions:
+        import torch
+        _precisions.update({torch.float32: _lib.PRECISION_F32, torch.bfloat16: _lib.PRECISION_BF16})
+    shape, precision = t.shape, _precisions.get(t.dtype)
+    if len(shape) != 2 or not t.is_cuda or precision is None:
         raise InvalidInput("%s must be an f32 or bf16 device tensor [rows, vocab]" % name)
-    rows, vocab = t.shape
-    if vocab == 0 or (vocab > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < vocab):
+    rows, vocab = shape
+    apart, step = t.stride()
+    if vocab == 0 or (vocab > 1 and step != 1) or (rows > 1 and apart < vocab):
         raise InvalidInput("the logits of a row of %s are adjacent, and rows do not overlap" % name)
-    return rows, vocab, max(t.stride(0), vocab), _lib.PRECISION_BF16 if t.dtype == torch.bfloat16 else _lib.PRECISION_F32
+    return rows, vocab, apart if apart > vocab else vocab, precision
 
 
 def _check_row(t, rows, dtype, like, name):
     if t is None:
         return None
-    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != rows or t.device != like.device or not t.is_contiguous():
+    if t.dtype != dtype or t.shape != (rows,) or t.get_device() != like.get_device() or not t.is_contiguous():
         raise InvalidInput("%s must be a contiguous %s tensor of %d values on the logits' device" % (name, dtype, rows))
     return t.data_ptr()
 
@@ -51,11 +58,12 @@ def token_logprobs(logits, targets=None, top: int = 0, stream=None) -> TokenLogP
     t = _check_row(targets, rows, torch.int32, logits, "targets")
     if not 0 <= top <= min(vocab, MAX_TOP):
         raise InvalidInput("top is 0 .. %d, got %d" % (min(vocab, MAX_TOP), top))
-    lp, h, lse = torch.empty((3, rows), dtype=torch.float32, device=logits.device).unbind(0)
+    lp = logits.new_empty(rows, dtype=torch.float32)
+    h, lse = torch.empty_like(lp), torch.empty_like(lp)
     ids = tlp = None
     if top:
-        ids = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
-        tlp = torch.empty((rows, top), dtype=torch.float32, device=logits.device)
+        ids = logits.new_empty((rows, top), dtype=torch.int32)
+        tlp = lp.new_empty((rows, top))
     issue(_lib.lib().logprobs_forward, logits, stream, _ERRORS, CudaError, logits.data_ptr(), stride, t, rows, vocab, top, precision,
           lp.data_ptr(), h.data_ptr(), lse.data_ptr(), tlp.data_ptr() if top else None, ids.data_ptr() if top else None)
     return TokenLogProbs(lp, h, lse, ids, tlp)
@@ -67,10 +75,11 @@ def token_logprobs_backward(logits, targets, lse, entropy=None, grad_logprob=Non
     import torch
     rows, vocab, stride, precision = _check_logits(logits, "logits")
     if out is None:
-        out = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
+        out, out_stride = logits.new_empty((rows, vocab)), vocab
     elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
         raise InvalidInput("out must match the logits")
-    _, _, out_stride, _ = _check_logits(out, "out")
+    else:
+        _, _, out_stride, _ = _check_logits(out, "out")
     if lse is None or (grad_entropy is not None and entropy is None):
         raise InvalidInput("the gradient needs lse, and the entropy for a gradient of it")
     f32 = torch.float32

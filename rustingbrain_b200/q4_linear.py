@@ -26,7 +26,7 @@ class Q4Linear:
         self.packed = torch.zeros(size, dtype=torch.uint8, device="cuda:%d" % device)      # zero scales: a layer of zeros
         self._dtypes = {torch.bfloat16: _lib.PRECISION_BF16, torch.float32: _lib.PRECISION_F32}
         self._fn = _lib.lib().q4_linear_forward
-        self._at = self.packed.data_ptr()
+        self._at, self._index = self.packed.data_ptr(), self.packed.get_device()
 
     def _same_place(self, t, shape, dtype, name):
         if tuple(t.shape) != shape or t.dtype != dtype or t.device != self.packed.device or not t.is_contiguous():
@@ -55,10 +55,10 @@ class Q4Linear:
 
     def forward(self, x, out=None, stream=None):
         """``x`` [rows, d_in], f32 or bf16, rows on 16-byte boundaries; returns [rows, d_out] of the same type."""
-        precision = self._dtypes.get(x.dtype)
-        if precision is None or x.dim() != 2 or x.shape[1] != self.d_in or x.device != self.packed.device or (self.d_in > 1 and x.stride(1) != 1):
+        precision, shape = self._dtypes.get(x.dtype), x.shape
+        if precision is None or len(shape) != 2 or shape[1] != self.d_in or x.get_device() != self._index or (self.d_in > 1 and x.stride(1) != 1):
             raise InvalidInput("expected a f32 or bf16 tensor [rows, %d] on %s, the channels of a row adjacent" % (self.d_in, self.packed.device))
-        rows = x.shape[0]
+        rows = shape[0]
         if out is None:
             out = x.new_empty((rows, self.d_out))
         elif tuple(out.shape) != (rows, self.d_out) or out.dtype != x.dtype or out.device != x.device or (self.d_out > 1 and out.stride(1) != 1):
