@@ -148,23 +148,35 @@ struct Row {
   }
 };
 
-// The CTA stores `count` new positions, first_slot .. of one page.  k and v point to the first new row of this head, `stride` elements apart;
-// pos0 is the first one's position in the sequence.  `codes` is [64][HD] bytes of shared memory.
+// Rotates, quantises and stores new positions.  A CTA has the 32 positions of a page that share its value words (w of the page layout), so
+// old positions keep their codes without anybody else writing to the words; a warp takes a position, two where its registers hold 256
+// channels.  What bounds it is the time of one position from its loads to its stores: 2 prompts of 256 rows take 6 us (40 us with four
+// warps for a whole page).
+template <int HD> struct Append { static constexpr int WARPS = HD <= 128 ? 32 : 16; };
+
 template <int HD>
-__device__ void append_page(const Cache& c, unsigned char* page, const bf16* k, const bf16* v, long long stride, int first_slot, int count,
-                            int pos0, unsigned char* codes) {
+__global__ void __launch_bounds__(Append<HD>::WARPS * 32) append_kernel(Cache c, const bf16* __restrict__ k, const bf16* __restrict__ v, int first, int rows) {
   using L = Layout<HD>;
-  constexpr int NG = L::NG;
+  constexpr int NG = L::NG, HALF_PAGE = PAGE / 2;
+  __shared__ unsigned char codes[HALF_PAGE * HD];
+  const int touched = (rows + HALF_PAGE - 2) / HALF_PAGE + 1;   // half pages that rows new positions can lie in
+  const int kvh = blockIdx.x / touched % c.Hkv, sj = blockIdx.x / touched / c.Hkv, seq = first + sj, len = c.lengths[seq];
+  if (len + rows > c.cap) return;                     // reported by the launch that follows
+  const int half = len / HALF_PAGE + blockIdx.x % touched, start = half * HALF_PAGE;
+  const int p0 = max(len, start), p1 = min(len + rows, start + HALF_PAGE);
+  if (p0 >= p1) return;
+  unsigned char* page = page_at(c, seq, kvh, half / 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int r = warp; r < count; r += WARPS) {
-    const int slot = first_slot + r;
+  for (int pos = p0 + warp; pos < p1; pos += Append<HD>::WARPS) {
+    const long long at = (((long long)sj * rows + pos - len) * c.Hkv + kvh) * HD;
+    const int slot = pos % PAGE;
     Row<HD> row;
-    row.make(c, k + r * stride, v + r * stride, pos0 + r);
+    row.make(c, k + at, v + at, pos);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       const uint32_t w = row.key_word(g);
       if ((lane & 7) == 0) reinterpret_cast<uint32_t*>(page + L::KEYS)[slot * (HD / 8) + (lane >> 3) * NG + g] = w;
-      codes[r * HD + 32 * g + lane] = (unsigned char)row.vcode[g];
+      codes[(pos - start) * HD + 32 * g + lane] = (unsigned char)row.vcode[g];
       if (lane == 0) {
         uint16_t* par = reinterpret_cast<uint16_t*>(page + L::KPAR + key_param(slot, g, NG));
         par[0] = (uint16_t)row.kstep[g];
@@ -175,33 +187,20 @@ __device__ void append_page(const Cache& c, unsigned char* page, const bf16* k, 
     }
   }
   __syncthreads();
-  // a value word holds eight positions: this CTA is the only one that writes to the page, old positions keep their codes
   uint32_t* vw = reinterpret_cast<uint32_t*>(page + L::VALUES);
-  for (int i = threadIdx.x; i < HD * 8; i += THREADS) {
-    const int ch = i >> 3, t = (i & 7) >> 1, w = i & 1;
+  for (int i = threadIdx.x; i < HD * 4; i += Append<HD>::WARPS * 32) {
+    const int ch = i >> 2, t = i & 3, word = ch * 8 + t * 2 + (half & 1);
     uint32_t set = 0, val = 0;
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
-      const int p = 16 * (2 * w + ((n & 3) >> 1)) + 8 * (n & 1) + 2 * t + (n >> 2), r = p - first_slot;
-      if (r >= 0 && r < count) {
+      const int p = start + 16 * ((n & 3) >> 1) + 8 * (n & 1) + 2 * t + (n >> 2);
+      if (p >= p0 && p < p1) {
         set |= 15u << (4 * n);
-        val |= (uint32_t)codes[r * HD + ch] << (4 * n);
+        val |= (uint32_t)codes[(p - start) * HD + ch] << (4 * n);
       }
     }
-    if (set) vw[i] = set == 0xffffffffu ? val : (vw[i] & ~set) | val;
+    if (set) vw[word] = set == 0xffffffffu ? val : (vw[word] & ~set) | val;
   }
-}
-
-template <int HD>
-__global__ void __launch_bounds__(THREADS) append_kernel(Cache c, const bf16* __restrict__ k, const bf16* __restrict__ v, int first, int rows) {
-  __shared__ unsigned char codes[PAGE * HD];
-  const int touched = (rows + PAGE - 2) / PAGE + 1;   // pages that rows new positions can lie in
-  const int kvh = blockIdx.x / touched % c.Hkv, sj = blockIdx.x / touched / c.Hkv, seq = first + sj, len = c.lengths[seq];
-  if (len + rows > c.cap) return;                     // reported by the launch that follows
-  const int page = len / PAGE + blockIdx.x % touched, p0 = max(len, page * PAGE), p1 = min(len + rows, (page + 1) * PAGE);
-  if (p0 >= p1) return;
-  const long long W = (long long)c.Hkv * HD, at = ((long long)sj * rows + p0 - len) * W + kvh * HD;
-  append_page<HD>(c, page_at(c, seq, kvh, page), k + at, v + at, W, p0 - page * PAGE, p1 - p0, p0, codes);
 }
 
 // ---- attention ----
@@ -925,12 +924,12 @@ cudaError_t launch_tables(float* cos_t, float* sin_t, int positions, int head_di
 }
 
 cudaError_t launch_append(const Cache& c, const bf16* k, const bf16* v, int first, int n_seq, int rows, cudaStream_t st) {
-  const dim3 grid((unsigned)(((rows + PAGE - 2) / PAGE + 1) * c.Hkv * n_seq));
+  const dim3 grid((unsigned)(((rows + PAGE / 2 - 2) / (PAGE / 2) + 1) * c.Hkv * n_seq));
   switch (c.HD) {
-    case 32: append_kernel<32><<<grid, THREADS, 0, st>>>(c, k, v, first, rows); break;
-    case 64: append_kernel<64><<<grid, THREADS, 0, st>>>(c, k, v, first, rows); break;
-    case 128: append_kernel<128><<<grid, THREADS, 0, st>>>(c, k, v, first, rows); break;
-    case 256: append_kernel<256><<<grid, THREADS, 0, st>>>(c, k, v, first, rows); break;
+    case 32: append_kernel<32><<<grid, Append<32>::WARPS * 32, 0, st>>>(c, k, v, first, rows); break;
+    case 64: append_kernel<64><<<grid, Append<64>::WARPS * 32, 0, st>>>(c, k, v, first, rows); break;
+    case 128: append_kernel<128><<<grid, Append<128>::WARPS * 32, 0, st>>>(c, k, v, first, rows); break;
+    case 256: append_kernel<256><<<grid, Append<256>::WARPS * 32, 0, st>>>(c, k, v, first, rows); break;
     default: return cudaErrorInvalidValue;
   }
   count_launch();
