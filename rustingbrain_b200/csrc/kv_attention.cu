@@ -541,6 +541,7 @@ __global__ void kv_set_lengths_kernel(int* lengths, int* full, int first, int co
 // A call that stores rows without attending to anything moves the lengths on by itself; a sequence without room is marked.
 __global__ void kv_advance_kernel(int* lengths, int* full, int first, int count, int rows, int cap) {
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  pdl_follow();
   if (i >= count) return;
   if (lengths[first + i] + rows > cap) full[first + i] = 1;
   else lengths[first + i] += rows;
@@ -549,6 +550,7 @@ __global__ void kv_advance_kernel(int* lengths, int* full, int first, int count,
 // Takes the newest rows of every sequence back.  A sequence whose last step was skipped for want of room has nothing to take back.
 __global__ void kv_rollback_kernel(int* lengths, const int* full, int first, int count, int rows) {
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  pdl_follow();
   if (i < count && !full[first + i]) lengths[first + i] = max(0, lengths[first + i] - rows);
 }
 
@@ -960,9 +962,7 @@ int32_t kv_cache_append(kv_cache_t* c, int32_t first, int32_t n_seq, const void*
     count_launch();
     KCK(cudaGetLastError());
   }
-  kv_advance_kernel<<<ceil_div(n_seq, 256), 256, 0, st>>>(c->lengths, c->full, first, n_seq, rows, g.capacity);
-  count_launch();
-  KCK(cudaGetLastError());
+  KCK(launch_following(kv_advance_kernel, ceil_div(n_seq, 256), 1, 256, 0, st, c->lengths, c->full, first, n_seq, rows, g.capacity));
   for (int i = 0; i < n_seq; ++i) c->host_len[first + i] += rows;
   return MOE_OK;
 }
@@ -975,9 +975,7 @@ int32_t kv_cache_rollback(kv_cache_t* c, int32_t first, int32_t n_seq, int32_t r
     if (c->host_len[first + i] < rows)
       return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: sequence %d holds %d positions, cannot drop %d", first + i, c->host_len[first + i], rows);
   KCK(cudaSetDevice(c->cfg.device));
-  kv_rollback_kernel<<<ceil_div(n_seq, 256), 256, 0, (cudaStream_t)stream>>>(c->lengths, c->full, first, n_seq, rows);
-  count_launch();
-  KCK(cudaGetLastError());
+  KCK(launch_following(kv_rollback_kernel, ceil_div(n_seq, 256), 1, 256, 0, (cudaStream_t)stream, c->lengths, c->full, first, n_seq, rows));
   for (int i = 0; i < n_seq; ++i) c->host_len[first + i] -= rows;
   return MOE_OK;
 }

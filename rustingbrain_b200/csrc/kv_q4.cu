@@ -158,6 +158,7 @@ template <int HD>
 __global__ void __launch_bounds__(Append<HD>::WARPS * 32) append_kernel(Cache c, const bf16* __restrict__ k, const bf16* __restrict__ v, int first, int rows) {
   using L = Layout<HD>;
   constexpr int NG = L::NG, HALF_PAGE = PAGE / 2;
+  pdl_follow();
   __shared__ unsigned char codes[HALF_PAGE * HD];
   const int touched = (rows + HALF_PAGE - 2) / HALF_PAGE + 1;   // half pages that rows new positions can lie in
   const int kvh = blockIdx.x / touched % c.Hkv, sj = blockIdx.x / touched / c.Hkv, seq = first + sj, len = c.lengths[seq];
@@ -340,6 +341,7 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
   const int sj = head_at / c.Hkv, kvh = head_at - sj * c.Hkv, seq = first + sj;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
   const int group = c.H / c.Hkv, nq = rows * group, q0 = pass * QT;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int len = c.lengths[seq], total = len + rows;
   if (total > c.cap) {                                // no room: nothing is stored or advanced, the step's rows are zeros
     if (threadIdx.x == 0) c.full[seq] = 1;
@@ -786,7 +788,7 @@ merge_kernel(Cache c, const float* __restrict__ part, int first, int rows, int s
   __shared__ float sums[WARPS][PW];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long at = blockIdx.x;                    // (sequence * rows + row) * heads + head
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the slices are written
+  pdl_follow();                                       // the slices are written
   const int row_at = (int)(at / c.H), h = (int)(at - (long long)row_at * c.H), sj = row_at / rows, row = row_at - sj * rows, seq = first + sj;
   const int len = c.lengths[seq], total = len + rows, group = c.H / c.Hkv;
   if (total > c.cap) return;                          // marked, and its rows zeroed, by the step
@@ -859,6 +861,7 @@ __global__ void tables_kernel(float* cos_t, float* sin_t, int positions, int hal
 
 __global__ void values_kernel(Cache c, int first, int from, int count, float* __restrict__ keys, float* __restrict__ values) {
   const int row = blockIdx.x, sj = row / count, seq = first + sj, W = c.Hkv * c.HD, NG = c.HD / GROUP;
+  pdl_follow();
   const int len = c.lengths[seq], pos = (from < 0 ? len - count : from) + row - sj * count;
   for (int i = threadIdx.x; i < W; i += blockDim.x) {
     float kv = 0.f, vv = 0.f;
@@ -886,32 +889,12 @@ cudaError_t go(const Cache& c, const bf16* q, const bf16* k, const bf16* v, int 
   constexpr int smem = Smem<HD, NQ>::BYTES;
   auto kernel = attention_kernel<HD, NQ, FOLD>;
   const int nq = rows * (c.H / c.Hkv), passes = (nq + NQ * 8 - 1) / (NQ * 8);
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(splits * passes * c.Hkv * n_seq));
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
   const bool joins = part == nullptr;
-  if (joins) { cfg.attrs = attr; cfg.numAttrs = 1; }
-  attr[0].val.clusterDim.x = splits;
-  count_launch();
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, c, q, k, v, first, rows, splits, slice, passes, append ? 1 : 0, joins ? 1 : 0, scale_log2, merged, part);
+  const cudaError_t e = launch_following(kernel, (unsigned)(splits * passes * c.Hkv * n_seq), joins ? splits : 1, THREADS, smem, st, c, q, k, v, first, rows,
+                                         splits, slice, passes, append ? 1 : 0, joins ? 1 : 0, scale_log2, merged, part);
   if (e != cudaSuccess || joins) return e;
   // resident as soon as the step's last CTA has only its results to write
-  cudaLaunchConfig_t join{};
-  join.gridDim = dim3((unsigned)(n_seq * rows * c.H));
-  join.blockDim = dim3(THREADS);
-  join.stream = st;
-  cudaLaunchAttribute early[1];
-  early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early[0].val.programmaticStreamSerializationAllowed = 1;
-  join.attrs = early;
-  join.numAttrs = 1;
-  count_launch();
-  return cudaLaunchKernelEx(&join, merge_kernel<HD>, c, (const float*)part, first, rows, splits, slice, NQ * 8, merged);
+  return launch_following(merge_kernel<HD>, (unsigned)(n_seq * rows * c.H), 1, THREADS, 0, st, c, (const float*)part, first, rows, splits, slice, NQ * 8, merged);
 }
 
 }  // namespace
@@ -924,16 +907,14 @@ cudaError_t launch_tables(float* cos_t, float* sin_t, int positions, int head_di
 }
 
 cudaError_t launch_append(const Cache& c, const bf16* k, const bf16* v, int first, int n_seq, int rows, cudaStream_t st) {
-  const dim3 grid((unsigned)(((rows + PAGE / 2 - 2) / (PAGE / 2) + 1) * c.Hkv * n_seq));
+  const unsigned grid = (unsigned)(((rows + PAGE / 2 - 2) / (PAGE / 2) + 1) * c.Hkv * n_seq);
   switch (c.HD) {
-    case 32: append_kernel<32><<<grid, Append<32>::WARPS * 32, 0, st>>>(c, k, v, first, rows); break;
-    case 64: append_kernel<64><<<grid, Append<64>::WARPS * 32, 0, st>>>(c, k, v, first, rows); break;
-    case 128: append_kernel<128><<<grid, Append<128>::WARPS * 32, 0, st>>>(c, k, v, first, rows); break;
-    case 256: append_kernel<256><<<grid, Append<256>::WARPS * 32, 0, st>>>(c, k, v, first, rows); break;
+    case 32: return launch_following(append_kernel<32>, grid, 1, Append<32>::WARPS * 32, 0, st, c, k, v, first, rows);
+    case 64: return launch_following(append_kernel<64>, grid, 1, Append<64>::WARPS * 32, 0, st, c, k, v, first, rows);
+    case 128: return launch_following(append_kernel<128>, grid, 1, Append<128>::WARPS * 32, 0, st, c, k, v, first, rows);
+    case 256: return launch_following(append_kernel<256>, grid, 1, Append<256>::WARPS * 32, 0, st, c, k, v, first, rows);
     default: return cudaErrorInvalidValue;
   }
-  count_launch();
-  return cudaGetLastError();
 }
 
 int queries_per_pass(int head_dim, int queries) { return queries <= 8 || head_dim == 256 ? 8 : 16; }
@@ -979,9 +960,7 @@ int ctas_per_sm(int head_dim, int queries, int device) {
 }
 
 cudaError_t launch_values(const Cache& c, int first, int n_seq, int from, int count, float* keys, float* values, cudaStream_t st) {
-  values_kernel<<<(unsigned)(n_seq * count), 128, 0, st>>>(c, first, from, count, keys, values);
-  count_launch();
-  return cudaGetLastError();
+  return launch_following(values_kernel, (unsigned)(n_seq * count), 1, 128, 0, st, c, first, from, count, keys, values);
 }
 
 }  // namespace q4

@@ -260,6 +260,7 @@ q4_linear_kernel(const T* __restrict__ x, long long ld_x, const unsigned char* _
                  QlShape s, QlPlan plan) {
   constexpr int P = QlPieces<T>::N, SUBS = GROUP / 32, PER_UNIT = QL_CHANNELS / GROUP, BYTES = ql_unit_bytes(GROUP);
   extern __shared__ __align__(128) unsigned char ql_sm[];
+  pdl_follow();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
   const int threads = blockDim.x, wk_count = plan.wk, wn_count = plan.warps / wk_count, wk = warp % wk_count, wn = warp / wk_count;
   const int cluster = plan.cluster, rank = blockIdx.x % cluster, pass = blockIdx.x / cluster % plan.passes, tile0 = blockIdx.x / cluster / plan.passes;
@@ -593,17 +594,8 @@ cudaError_t ql_launch(const T* x, long long ld_x, const void* packed, T* y, long
     if (e != cudaSuccess) return e;
     raised.fetch_or(bit, std::memory_order_relaxed);
   }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(plan.clusters * plan.passes * plan.cluster));
-  cfg.blockDim = dim3(plan.warps * 32);
-  cfg.dynamicSmemBytes = plan.bytes;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = plan.cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-  if (plan.cluster > 1) { cfg.attrs = attr; cfg.numAttrs = 1; }
-  count_launch();
-  return cudaLaunchKernelEx(&cfg, kernel, x, ld_x, (const unsigned char*)packed, y, ld_y, rows, s, plan);
+  return launch_following(kernel, (unsigned)(plan.clusters * plan.passes * plan.cluster), plan.cluster, plan.warps * 32, plan.bytes, st, x, ld_x,
+                          (const unsigned char*)packed, y, ld_y, rows, s, plan);
 }
 
 template <typename T, int GROUP>

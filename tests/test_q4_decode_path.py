@@ -242,3 +242,56 @@ def test_the_models_decode_over_a_cache_in_4_bits(H, Hkv, hd):
     with pytest.raises(InvalidInput, match="SequenceTooLong"):
         dev.forward_cached([list(seqs[0][:10])], caches, first_sequence=0)
     dev.close()
+
+
+@pytest.mark.gpu
+def test_inputs_that_come_from_another_stream():
+    """Kernels that are let in while their predecessor runs: what they read comes from a second stream, eager and captured, and each call's
+    input is overwritten as soon as it has been read."""
+    L = Q4Linear(256, 512)
+    g = torch.Generator(device="cuda").manual_seed(8)
+    L.set_weight(torch.randn(512, 256, generator=g, device="cuda"))
+    xs = torch.randn(20, 4, 256, generator=g, device="cuda").bfloat16()
+    t = torch.randint(0, 512, (4,), generator=g, device="cuda", dtype=torch.int32)
+    torch.cuda.synchronize()
+    want = []
+    for x in xs:
+        y = L(x)
+        torch.cuda.synchronize()
+        s = token_logprobs(y, t)
+        torch.cuda.synchronize()
+        want.append((y, s.logprob, token_logprobs_backward(y, t, s.lse, s.entropy, s.lse, s.entropy)))
+    torch.cuda.synchronize()
+    main, side = torch.cuda.Stream(), torch.cuda.Stream()
+    x, y, d = torch.zeros_like(xs[0]), torch.zeros_like(want[0][0]), torch.zeros_like(want[0][2])
+    pile = [(torch.zeros_like(y), torch.zeros_like(want[0][1]), torch.zeros_like(d)) for _ in xs]
+
+    def run():
+        for i in range(len(xs)):
+            side.wait_stream(main)
+            with torch.cuda.stream(side):
+                x.copy_(xs[i])
+            main.wait_stream(side)
+            L(x, out=y)
+            s = token_logprobs(y, t)
+            token_logprobs_backward(y, t, s.lse, s.entropy, s.lse, s.entropy, out=d)
+            for a, b in zip(pile[i], (y, s.logprob, d)):
+                a.copy_(b)
+
+    def check():
+        torch.cuda.synchronize()
+        for got, w in zip(pile, want):
+            for a, b in zip(got, w):
+                assert torch.equal(a, b)
+                a.zero_()
+        torch.cuda.synchronize()
+
+    with torch.cuda.stream(main):
+        run()
+    check()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=main):
+        run()
+    for _ in range(3):
+        graph.replay()
+        check()
