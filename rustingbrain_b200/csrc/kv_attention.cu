@@ -741,12 +741,13 @@ int forward_q4(kv_cache* c, int first, int n_seq, const void* q, const void* k, 
   //    one length;
   //  - slices of one size for all sequences, joined by a second launch: for lengths that differ, and for a few long sequences.
   // Chosen by what they would take, in microseconds: a page takes a CTA its share of 6000 bytes a nanosecond, though at least a quarter
-  // of the microsecond that a warp needs for one of 64 channels; a CTA's start and end and the second launch take about 3 each.
+  // of the microsecond that a warp needs for one of 64 channels; a CTA's start and end take about 6 (with 3 here, more and shorter slices:
+  // 16 sequences of up to 32767 positions, 12 queries a head, 143 us instead of 131), the second launch 3.
   const double bytes = (double)q4::page_bytes(g.head_dim);
   auto estimate = [&](long long active, int slice) {
     const long long waves = (active + slots - 1) / slots;
     const double page = std::max(0.25 * g.head_dim / 64, bytes * (double)std::min(active, slots) / 6e6);
-    return (double)waves * (slice * page + 3.0);
+    return (double)waves * (slice * page + 6.0);
   };
   int splits = (int)std::min<long long>(q4::CLUSTER, std::max<long long>(1, slots / ctas));
   splits = std::max(1, std::min(splits, ceil_div(longest, 4)));
