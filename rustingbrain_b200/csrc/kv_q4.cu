@@ -19,6 +19,9 @@
 //           instruction, one rounding of the value to bf16 (2^-8 of it at most).  The weights enter as two bf16 numbers each, so that the value's
 //           is the only rounding of that size before the output's: error against 64 bits 2.3e-3 of the output's rms, 3.3e-3 with one.
 // What bounds it is the issue of those instructions: 148 SMs would have to do a page of 64 x 64 channels every 215 cycles to keep up with HBM.
+// Measured with a rollback behind each step, in a graph: 64 sequences of 4096 positions, 16/4 heads of 64, 26.5 us (bf16 cache: 58 us), of
+// 16384 73 us (0.84 of the copy bandwidth for each further byte); 16 of 0 .. 32767, 32/8 heads of 128, one row 71 us, three rows 119 us,
+// where the bytes alone take 51 us; one of 700 8.4 us, one of 32000 12.7 us.
 //
 // Page layout, HD = head_dim, NG = HD / 32:
 //   keys    [64 positions][4 t][NG g] words: channels 32 g + 8 t + 2 i + e at nibble i + 4 e
@@ -150,8 +153,8 @@ struct Row {
 
 // Rotates, quantises and stores new positions.  A CTA has the 32 positions of a page that share its value words (w of the page layout), so
 // old positions keep their codes without anybody else writing to the words; a warp takes a position, two where its registers hold 256
-// channels.  What bounds it is the time of one position from its loads to its stores: 2 prompts of 256 rows take 6 us (40 us with four
-// warps for a whole page).
+// channels.  What bounds it is the time of one position from its loads to its stores: 2 prompts of 256 rows take 9 us with a cold cache
+// (40 us with four warps for a whole page).
 template <int HD> struct Append { static constexpr int WARPS = HD <= 128 ? 32 : 16; };
 
 template <int HD>

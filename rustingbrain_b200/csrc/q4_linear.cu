@@ -19,6 +19,10 @@
 // tile to tile; its warps split the reduction of a tile.  More rows are passes side by side, which find the weights in L2.  Where there
 // are fewer tiles than SMs the CTAs of a cluster split the reduction too.  Partial sums meet in (distributed) shared memory, always in
 // the same order: one launch, no workspace.
+//
+// Measured in a graph: 1 x 1024 -> 2816 3.8 us; 8 x 4096 -> 24576 20.1 us, 16 rows 24 us, 64 rows 61 us (the bytes: 8.25 us); f32 3 x 2048 -> 32003
+// 17.6 us (5.7 us).  What bounds the large ones is the issue of instructions, 1.9 a cycle and SM; 64 x 1024 -> 5632, 11.9 us, brings in
+// its activations for a quarter of that.
 
 #include <cooperative_groups.h>
 #include <algorithm>
