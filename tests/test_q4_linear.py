@@ -31,6 +31,10 @@ def test_arguments_are_checked_before_any_device_work():
     for bad in (dict(x=None), dict(y=None), dict(packed=None), dict(packed=off(8)), dict(x=off(2)), dict(x=off(8)), dict(y=off(1)), dict(ldx=63),
                 dict(ldy=7), dict(rows=-1), dict(rows=2, ldx=68), dict(rows=64 * 65536)):
         assert fwd(**bad) == _lib.INVALID_INPUT and msg.value, bad
+    # y on top of x, or on a part of it: x is 64 channels of 128 bytes
+    for bad in (dict(y=p), dict(y=off(126)), dict(rows=3, ldx=72, ldy=72, y=off(126)), dict(rows=3, ldx=72, ldy=72, y=off(130)),
+                dict(rows=3, ldx=72, ldy=80, y=off(128)), dict(rows=2, ldx=128, ldy=128, y=off(256 + 120)), dict(x=off(16), y=off(14))):
+        assert fwd(**bad) == _lib.INVALID_INPUT and b"overlaps" in msg.value, bad
     assert L.q4_linear_pack(None, p, p, 8, 64, 32, None, msg, 128) == _lib.INVALID_INPUT
     assert L.q4_linear_pack(p, None, p, 8, 64, 32, None, msg, 128) == _lib.INVALID_INPUT
     assert L.q4_linear_quantize(None, p, 8, 64, 32, None, msg, 128) == _lib.INVALID_INPUT
@@ -180,3 +184,17 @@ def test_streams_graphs_and_errors():
             Q4Linear(64, 4).set_codes(codes, scales)
     with pytest.raises(InvalidInput):
         Q4Linear(64, 4).set_weight(torch.zeros(4, 64, device="cuda").bfloat16())
+
+
+@pytest.mark.gpu
+def test_rows_of_x_and_y_side_by_side_in_one_buffer():
+    layer, w = _layer(64, 40, 32, 21)
+    buf = torch.randn(5, 112, device="cuda", generator=torch.Generator(device="cuda").manual_seed(22)).bfloat16()
+    x, y = buf[:, :64], buf[:, 64:104]
+    rest = buf[:, 104:].clone()
+    want = layer(x)
+    layer(x, out=y)
+    assert torch.equal(y, want) and torch.equal(buf[:, 104:], rest)
+    _check(y, x, w)
+    with pytest.raises(InvalidInput, match="overlaps"):
+        layer(x, out=buf[:, 60:100])
