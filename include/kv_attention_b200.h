@@ -21,7 +21,8 @@
  * in f32 arithmetic, rounding to even, rotation included (two products and their sum, not contracted; the angles are computed in 64 bits).
  * A step's own new positions are read back from the cache like all others.  If a position's key or value of a kv head holds a NaN, an
  * infinity or a number above 2^40 in magnitude, its key and value stand for NaN: what attends to it is NaN, what does not is untouched.
- * Neither call below allocates on such a cache, so every step can be captured; q is left alone.
+ * A query with an infinity, a NaN or a number above 2^116 (after the rotation) may give NaN, in its own row and head.
+ * Neither call below allocates on such a cache, so every step can be captured; q is left alone.  At most 2^30 positions.
  */
 #ifndef KV_ATTENTION_B200_H
 #define KV_ATTENTION_B200_H

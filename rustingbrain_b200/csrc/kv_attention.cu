@@ -788,16 +788,16 @@ int forward_q4(kv_cache* c, int first, int n_seq, const void* q, const void* k, 
 // The checks that every call with new rows makes.
 int check_step(kv_cache* c, int first, int n_seq, int rows) {
   const kv_cache_config_t& g = c->cfg;
-  if (first < 0 || n_seq <= 0 || first + n_seq > g.sequences)
-    return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: sequences %d .. %d of %d", first, first + n_seq - 1, g.sequences);
+  if (first < 0 || n_seq <= 0 || n_seq > g.sequences - first)
+    return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: sequences %d .. %lld of %d", first, (long long)first + n_seq - 1, g.sequences);
   if (rows <= 0) return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: empty step or null buffer");
   if ((long long)n_seq * rows * g.num_heads > 0x7fffffffll) return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: too many rows");
   return MOE_OK;
 }
 int check_room(kv_cache* c, int first, int n_seq, int rows) {
   for (int i = 0; i < n_seq; ++i)
-    if (c->host_len[first + i] + rows > c->cfg.capacity)
-      return kv_fail(c, MOE_INVALID_INPUT, "SequenceTooLong: length %d, max_seq_len %d (sequence %d)", c->host_len[first + i] + rows, c->cfg.capacity, first + i);
+    if (rows > c->cfg.capacity - c->host_len[first + i])
+      return kv_fail(c, MOE_INVALID_INPUT, "SequenceTooLong: length %lld, max_seq_len %d (sequence %d)", (long long)c->host_len[first + i] + rows, c->cfg.capacity, first + i);
   return MOE_OK;
 }
 
@@ -825,6 +825,7 @@ int32_t kv_cache_create(const kv_cache_config_t* config, kv_cache_t** out) {
     return kv_fail(c, MOE_INVALID_CONFIG, "InvalidConfig: precision is f32, bf16 or q4");
   if (is_q4 && !q4::head_dim_ok(g.head_dim)) return kv_fail(c, MOE_UNSUPPORTED, "Unsupported: head_dim %d of a 4-bit cache (32, 64, 128, 256)", g.head_dim);
   if (g.max_seq_len < g.capacity) return kv_fail(c, MOE_INVALID_CONFIG, "InvalidConfig: capacity %d exceeds max_seq_len %d", g.capacity, g.max_seq_len);
+  if (is_q4 && g.capacity > 1 << 30) return kv_fail(c, MOE_UNSUPPORTED, "Unsupported: more than 2^30 positions in a 4-bit cache");
   KCK(cudaSetDevice(g.device));
   cudaDeviceProp prop;
   KCK(cudaGetDeviceProperties(&prop, g.device));

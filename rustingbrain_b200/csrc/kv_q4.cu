@@ -446,7 +446,7 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
       for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[j]));
 #pragma unroll
       for (int d = 1; d < HD / 8; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-      const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 100);
+      const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 116);
       const float by = __uint_as_float((uint32_t)(127 + Q_TOP - e) << 23);
       if (i % (HD / 8) == 0) factors[at] = scale_log2 * __uint_as_float((uint32_t)(127 + RAW_HALF - Q_TOP + e) << 23);
       uint32_t w[4];

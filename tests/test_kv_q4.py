@@ -41,6 +41,8 @@ def test_configurations_are_checked_before_any_device_work():
         assert rc == _lib.UNSUPPORTED and "4-bit" in text
     for bad in (dict(num_heads=3), dict(head_dim=7), dict(sequences=0), dict(capacity=17), dict(precision=4), dict(precision=_lib.PRECISION_Q8)):
         assert _create(**bad)[0] == _lib.INVALID_CONFIG, bad
+    rc, text = _create(capacity=(1 << 30) + 1, max_seq_len=(1 << 30) + 1)
+    assert rc == _lib.UNSUPPORTED and "2^30" in text
     L = _lib.lib()
     assert L.kv_cache_append(None, 0, 1, None, None, 1, None) == _lib.INVALID_INPUT
     assert L.kv_cache_rollback(None, 0, 1, 1, None) == _lib.INVALID_INPUT
@@ -357,3 +359,36 @@ def test_append_newest_and_rollback_on_the_other_caches(precision):
     cache.rollback(1, 1, 1)
     again = cache.forward_cached(d(q[29:]), d(k[29:]), d(v[29:]), first_sequence=1, n_sequences=1)
     assert torch.equal(got, again) and cache.lengths() == [0, 30]
+
+
+@pytest.mark.gpu
+def test_ranges_that_wrap_around():
+    """A first sequence or a number of rows whose sum with what is there passes 31 bits is refused like any other."""
+    for precision, dt in (("q4", torch.bfloat16), ("f32", torch.float32)):
+        cache = KvCache(2, 1, 1, 32, capacity=8, precision=precision)
+        k = torch.ones(2, 32, device="cuda", dtype=dt)
+        cache.append(k, k)
+        p, L, st = C.c_void_p(k.data_ptr()), _lib.lib(), 0
+        big = 2 ** 31 - 1
+        for first, n, rows in ((big, 1, 1), (1, big, 1), (2, 1, 1), (0, 1, big), (0, 1, 8), (1, 2, 1)):
+            assert L.kv_cache_append(cache._h, first, n, p, p, rows, st) == _lib.INVALID_INPUT, (first, n, rows)
+            assert L.kv_attention_forward_cached(cache._h, first, n, p, p, p, rows, p, st) == _lib.INVALID_INPUT
+            assert L.kv_cache_rollback(cache._h, first, n, rows, st) == _lib.INVALID_INPUT
+            assert L.kv_cache_newest(cache._h, first, n, rows, p, p, st) == _lib.INVALID_INPUT
+        assert cache.lengths() == [1, 1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,Hkv,hd", [(4, 1, 64), (10, 1, 32), (16, 1, 128), (4, 1, 256)])
+def test_queries_of_any_size(H, Hkv, hd):
+    """Queries of 2^110 against keys of 2^-112, and the other way round; small and large queries in one pass keep their own scale."""
+    for up, down in ((110, -112), (-110, 30), (0, 0)):
+        cache, o = KvCache(1, H, Hkv, hd, capacity=100, precision="q4"), Q4CacheOracle(H, Hkv, hd, 100)
+        _, k, v = _rows(90, H, Hkv, hd, 31)
+        k = k * np.float32(2.0 ** down)
+        cache.append(_dev(k), _dev(v), rows_per_sequence=90)
+        o.append(k, v)
+        q, k, v = _rows(1, H, Hkv, hd, 32)
+        q = q.reshape(H, hd) * np.float32(2.0) ** (up - 3 * np.arange(H, dtype=np.float32))[:, None] if up <= 0 else q * np.float32(2.0 ** up)
+        q, k = q.reshape(1, -1), k * np.float32(2.0 ** down)
+        _close(cache.forward_cached(_dev(q), _dev(k), _dev(v)), o.forward_cached(q, k, v))
