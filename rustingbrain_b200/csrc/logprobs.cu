@@ -11,7 +11,8 @@
 // One CTA takes a row.  When there are fewer rows than would fill the machine, a cluster of 2, 4 or 8 CTAs takes one and
 // joins its sums and candidate lists through distributed shared memory: still one launch and no workspace.
 //
-// Measured in a graph: 8192 x 32000 bf16 94 us, 0.86 of the copy bandwidth (the exponentials' pipe is at 0.7); 64 x 131071 f32 with 5 alternatives
+// Measured in a graph: 8192 x 32000 bf16 94 us, 0.86 of the copy bandwidth (without half of the exponentials 93 us; CTAs that stay for
+// several rows and load the next one early 105 us); 64 x 131071 f32 with 5 alternatives
 // 13 us; one row of 32000 with 20 alternatives 9.2 us.  Gradient of 4096 x 32000 bf16 85 us, 0.95 of the copy bandwidth.
 
 #include <cooperative_groups.h>

@@ -39,7 +39,7 @@ class KvCache:
                                   rope_base=rope_base, rope=1 if rope else 0,
                                   precision=_PRECISIONS[precision], device=device)
         self.device = device
-        self._dtype = self._raw_stream = None          # torch's, looked up with the first step
+        self._dtype = self._raw_stream = self._f32 = None      # torch's, looked up with the first step
         self._forward = _lib.lib().kv_attention_forward_cached
         rc = _lib.lib().kv_cache_create(C.byref(cfg), C.byref(self._h))
         if rc != _lib.OK:
@@ -132,11 +132,12 @@ class KvCache:
     def newest(self, rows_per_sequence: int = 1, first_sequence: int = 0, n_sequences: Optional[int] = None, stream=None):
         """The newest rows of every sequence of the range as the cache holds them: f32 device tensors
         [n_sequences * rows_per_sequence, kv_heads * head_dim], keys (after the rotation) and values."""
-        import torch
         n_seq = self.sequences - first_sequence if n_sequences is None else n_sequences
         shape = (max(n_seq, 0) * max(rows_per_sequence, 0), self.kv_heads * self.head_dim)
-        keys = torch.empty(shape, dtype=torch.float32, device=self.device)
-        values = torch.empty_like(keys)
+        if self._f32 is None:
+            import torch
+            self._f32 = torch.empty(0, dtype=torch.float32, device=self.device)
+        keys, values = self._f32.new_empty(shape), self._f32.new_empty(shape)
         self._check(_lib.lib().kv_cache_newest(self._h, first_sequence, n_seq, rows_per_sequence, keys.data_ptr(), values.data_ptr(), self._on(stream)))
         return keys, values
 
