@@ -20,7 +20,7 @@
 //           is the only rounding of that size before the output's: error against 64 bits 2.3e-3 of the output's rms, 3.3e-3 with one.
 // What bounds it is the issue of those instructions: 148 SMs would have to do a page of 64 x 64 channels every 215 cycles to keep up with HBM.
 // Measured with a rollback behind each step, in a graph: 64 sequences of 4096 positions, 16/4 heads of 64, 26.5 us (bf16 cache: 58 us), of
-// 16384 73 us (0.84 of the copy bandwidth for each further byte); 16 of 0 .. 32767, 32/8 heads of 128, one row 71 us, three rows 119 us,
+// 16384 73 us (0.84 of the copy bandwidth for each further byte); 16 of 0 .. 32767, 32/8 heads of 128, one row 71 us, three rows 117 us,
 // where the bytes alone take 51 us; one of 700 8.4 us, one of 32000 12.7 us.
 //
 // Page layout, HD = head_dim, NG = HD / 32:
@@ -394,14 +394,17 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
 #pragma unroll
   for (int i = 0; i < SLOTS - 1; ++i) issue();
 
-  // ---- this warp's new positions, if its first page has any: quantised while the page and the queries are under way.  A row in `fresh` is
-  // the key's words in page order, the value's codes, then step | base of the key's and of the value's groups. ----
-  const int new0 = max(len, pg * PAGE), news = append && pg >= pg0 ? max(0, min(total, (pg + 1) * PAGE) - new0) : 0;
-  for (int r = 0; r < news; ++r) {
-    const long long at = (((long long)sj * rows + new0 + r - len) * c.Hkv + kvh) * HD;
-    unsigned char* f = fresh + r * M::ROW;
+  // ---- the slice's new positions: quantised while the pages and the queries are under way, each by another warp, into `fresh` of the warp
+  // whose first page has them.  A row there is the key's words in page order, the value's codes, then step | base of the key's and of the
+  // value's groups.  (Three rows one after the other in the page's own warp: 16 x 0 .. 32767 takes 119 us instead of 116.5.) ----
+  const int new0 = max(len, pg * PAGE), news = append && pg >= pg0 ? max(0, min(total, (pg + 1) * PAGE) - new0) : 0;   // this warp's
+  for (int pos = len + warp; append && pos < total; pos += WARPS) {
+    const int page = pos / PAGE;
+    if (page < pg0 || page >= pend) continue;         // in another slice
+    const long long at = (((long long)sj * rows + pos - len) * c.Hkv + kvh) * HD;
+    unsigned char* f = sm + M::FRONT + (pend - 1 - page) * M::WARP + M::RING + (pos - max(len, page * PAGE)) * M::ROW;
     Row<HD> row;
-    row.make(c, k + at, v + at, new0 + r);
+    row.make(c, k + at, v + at, pos);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       const uint32_t w = row.key_word(g);
@@ -411,7 +414,7 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
     }
   }
 
-  // ---- queries: rotated, scaled to base 2, rounded to bf16 once; eight channels of one query a thread and turn ----
+  // ---- queries: rotated, rounded once to f16 under a power of two of their own; eight channels of one query a thread and turn ----
   {
     const bool wide = (reinterpret_cast<uintptr_t>(q) & 15) == 0;     // a head's row is a multiple of 16 bytes
     uint4* frag = reinterpret_cast<uint4*>(sm);
