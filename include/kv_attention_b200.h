@@ -76,7 +76,7 @@ int32_t kv_cache_lengths(kv_cache_t* cache, int32_t* lengths_host, void* stream)
  * projections BEFORE rotation (`project`, attention.rs:920-944, rotates queries and keys; here the call
  * does).  q is scratch: one kernel path rotates it in place, the other rotates in registers and leaves it
  * alone, so its contents after the call are unspecified; k and v are read only.
- * merged [rows, num_heads * head_dim] is the input of the output projection.
+ * merged [rows, num_heads * head_dim] is the input of the output projection; it may be q itself and overlaps nothing else.
  * SequenceTooLong -> MOE_INVALID_INPUT when a cache would pass its capacity (rope.rs:194-200); nothing
  * is appended in that case. */
 int32_t kv_attention_forward_cached(kv_cache_t* cache, int32_t first_sequence, int32_t n_sequences, void* q,

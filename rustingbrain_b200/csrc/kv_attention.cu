@@ -850,8 +850,13 @@ int32_t kv_cache_create(const kv_cache_config_t* config, kv_cache_t** out) {
   KCK(cudaMemset(c->lengths, 0, sizeof(int) * g.sequences));
   KCK(cudaMalloc(&c->full, sizeof(int) * g.sequences));
   KCK(cudaMemset(c->full, 0, sizeof(int) * g.sequences));
-  c->host_len.assign(g.sequences, 0);
-  c->host_full.assign(g.sequences, 0);
+  try {
+    c->host_len.assign(g.sequences, 0);
+    c->host_full.assign(g.sequences, 0);
+    c->pages.reserve(g.sequences);                    // so that a step does not allocate
+  } catch (const std::bad_alloc&) {
+    return kv_fail(c, MOE_OUT_OF_MEMORY, "OutOfMemory: host copies of the lengths of %d sequences", g.sequences);
+  }
   // slice results of one decode step (one row per sequence) at the largest slice count, so that a serving
   // loop never allocates; a prefill with more rows grows it once
   c->part_floats = (size_t)g.sequences * g.num_heads * KV_MAX_SPLITS * (g.head_dim + 2);

@@ -392,3 +392,23 @@ def test_queries_of_any_size(H, Hkv, hd):
         q = q.reshape(H, hd) * np.float32(2.0) ** (up - 3 * np.arange(H, dtype=np.float32))[:, None] if up <= 0 else q * np.float32(2.0 ** up)
         q, k = q.reshape(1, -1), k * np.float32(2.0 ** down)
         _close(cache.forward_cached(_dev(q), _dev(k), _dev(v)), o.forward_cached(q, k, v))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,rows", [([70, 70], 1), ([3, 900], 1), ([600, 20], 5), ([0, 64], 40)])
+def test_the_result_may_take_the_queries_place(lens, rows):
+    """Clusters, slices and several passes; rows behind the last sequence stay as they were."""
+    H, Hkv, hd, S = 8, 2, 64, len(lens)
+    caches = [KvCache(S, H, Hkv, hd, capacity=1000, precision="q4") for _ in range(2)]
+    for c in caches:
+        for s, n in enumerate(lens):
+            if n:
+                _, k, v = _rows(n, H, Hkv, hd, 50 + s)
+                c.append(_dev(k), _dev(v), rows_per_sequence=n, first_sequence=s, n_sequences=1)
+    q, k, v = (_dev(a) for a in _rows(S * rows, H, Hkv, hd, 60))
+    want = caches[0].forward_cached(q, k, v, rows_per_sequence=rows)
+    buf = torch.cat([q, torch.full((3, H * hd), 7.0, device="cuda").bfloat16()])
+    got = caches[1].forward_cached(buf[:S * rows], k, v, rows_per_sequence=rows, out=buf[:S * rows])
+    assert torch.equal(got, want) and bool((buf[S * rows:] == 7).all())
+    with pytest.raises(InvalidInput):
+        caches[1].forward_cached(q, k, v, rows_per_sequence=rows, out=torch.empty(S * rows, Hkv * hd, device="cuda", dtype=torch.bfloat16))
