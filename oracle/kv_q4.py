@@ -1,4 +1,4 @@
-"""Checker of the KV cache held in 4 bits: the stated format in 32-bit steps, the attention in 64 bits.  Test infrastructure only.
+"""Oracle of the KV cache held in 4 bits: the stated format in 32-bit steps, the attention in 64 bits.  Test infrastructure only.
 
 The arithmetic between the projections follows attention.rs:344-398 (rotate, append, softmax(q K^T / sqrt(head_dim)) V over the
 positions a query sees); what the cache stands for follows the rule in include/kv_attention_b200.h.

@@ -827,9 +827,7 @@ int32_t kv_cache_create(const kv_cache_config_t* config, kv_cache_t** out) {
   if (g.max_seq_len < g.capacity) return kv_fail(c, MOE_INVALID_CONFIG, "InvalidConfig: capacity %d exceeds max_seq_len %d", g.capacity, g.max_seq_len);
   if (is_q4 && g.capacity > 1 << 30) return kv_fail(c, MOE_UNSUPPORTED, "Unsupported: more than 2^30 positions in a 4-bit cache");
   KCK(cudaSetDevice(g.device));
-  cudaDeviceProp prop;
-  KCK(cudaGetDeviceProperties(&prop, g.device));
-  c->sm_count = prop.multiProcessorCount;
+  KCK(cudaDeviceGetAttribute(&c->sm_count, cudaDevAttrMultiProcessorCount, g.device));
   if (is_q4) {
     const size_t bytes = (size_t)g.sequences * g.kv_heads * q4::head_pages(g.capacity) * q4::page_bytes(g.head_dim);
     if (cudaMalloc(&c->keys, bytes) != cudaSuccess) {
