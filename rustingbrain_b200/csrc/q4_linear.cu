@@ -440,11 +440,9 @@ q4_linear_kernel(const T* __restrict__ x, long long ld_x, const unsigned char* _
               const uint4 b = *reinterpret_cast<const uint4*>(mine[n] + q * plane + off);
 #pragma unroll
               for (int m = 0; m < 2; ++m) {
-                {
-                  if (opens && q == 0) ql_mma_bf16(part[m][n], from, a[m][0], a[m][1], a[m][2], a[m][3], b.x, b.y);
-                  else ql_mma_bf16(part[m][n], a[m][0], a[m][1], a[m][2], a[m][3], b.x, b.y);
-                  ql_mma_bf16(part[m][n], a[m][4], a[m][5], a[m][6], a[m][7], b.z, b.w);
-                }
+                if (opens && q == 0) ql_mma_bf16(part[m][n], from, a[m][0], a[m][1], a[m][2], a[m][3], b.x, b.y);
+                else ql_mma_bf16(part[m][n], a[m][0], a[m][1], a[m][2], a[m][3], b.x, b.y);
+                ql_mma_bf16(part[m][n], a[m][4], a[m][5], a[m][6], a[m][7], b.z, b.w);
               }
             }
           }
@@ -530,6 +528,7 @@ bool ql_plan(const QlShape& s, int rows, int live, QlPlan* out) {
   constexpr double issue = (70 + 4 * (P == 1 ? 28 + 6 * NT : 48 + 18 * NT) + QL_CHANNELS / (P == 1 ? GROUP : 32) * (6 + 18 * NT));
   constexpr double products = 16 * NT * 2.1 * P;
   const int most[4] = {8, 8, 12, 16}, limit[4] = {113 * 1024, 227 * 1024, 227 * 1024, 227 * 1024}, resident[4] = {2, 1, 1, 1};
+  const double first[4] = {700, 2700, 3200, 3700}, more[4] = {3500, 5000, 6500, 8000};
   const int at_once[4] = {SM, 74, 33, 15};   // clusters of 1, 2, 4 and 8 SMs that the machine holds: they do not cross the borders of a GPC
   double best = -1;
   QlPlan p{};
@@ -564,7 +563,7 @@ bool ql_plan(const QlShape& s, int rows, int live, QlPlan* out) {
         const double unit = std::max(p.warps * on_sm * std::max(hbm, std::max(issue / rate, products)), std::max(350.0, 1100.0 / (p.stages - 1)));
         const double fill = 1500 + (double)live * p.slice * 16 / 32 * (P == 1 ? 50 : 110) * on_sm / rate;
         const double waves = (double)((ctas + on_sm * room - 1) / (on_sm * room));
-        const double time = waves * (fill + rounds * (each * unit + (p.cluster > 1 ? 5000.0 : 700.0)));
+        const double time = waves * (fill + rounds * each * unit + first[log] + (rounds - 1) * more[log]);
         if (best < 0 || time < best) { best = time; *out = p; }
       }
     }
