@@ -20,9 +20,9 @@
 // are fewer tiles than SMs the CTAs of a cluster split the reduction too.  Partial sums meet in (distributed) shared memory, always in
 // the same order: one launch, no workspace.
 //
-// Measured in a graph: 1 x 1024 -> 2816 3.8 us; 8 x 4096 -> 24576 20.1 us, 16 rows 24 us, 64 rows 61 us (the bytes: 8.25 us); f32 3 x 2048 -> 32003
-// 17.6 us (5.7 us).  What bounds the large ones is the issue of instructions, 1.9 a cycle and SM; 64 x 1024 -> 5632, 11.9 us, brings in
-// its activations for a quarter of that.
+// Measured in a graph: 1 x 1024 -> 2816 3.9 us; 8 x 4096 -> 24576 16.6 us, one row 14.8 us, 16 rows 22 us, 64 rows 61 us (the bytes: 8.25 us); f32
+// 3 x 2048 -> 32003 17.7 us (5.7 us).  What bounds the large ones is the issue of instructions, 2 a cycle and SM, and the start; 64 x 1024 ->
+// 5632, 9.9 us, brings in its activations for a quarter of that.
 
 #include <cooperative_groups.h>
 #include <algorithm>
@@ -520,15 +520,17 @@ bool ql_sizes_ok(int d_out, int d_in, int group) {
 
 // How to cut a product with `live` <= NT * 8 rows a pass: of the ways that fit, the one that should be done first.  False: none fits.
 // The estimate is in cycles of an SM and counts what was measured: a unit takes an SM the issue of its instructions (0.17 a cycle for each warp, up to 2.6), its
-// products (2.1 cycles each) or its share of HBM (24 bytes a cycle), whichever is longest, and a warp no less than its latency; joining
-// a tile takes 700 cycles, over a cluster 5000; a thread takes 50 to 110 instructions for eight activations.
+// products (2.1 cycles each) or its share of HBM (24 bytes a cycle), whichever is longest, and a warp no less than its latency; a thread takes
+// 50 to 110 instructions for eight activations.  Joining a CTA's only tile takes 1200 cycles, over a cluster 2700 to 3700; each further tile,
+// for which the warps drain and fill again, 3500 and 5000 to 8000.  So a cluster of two often pays by making rounds fewer: 8 x 4096 -> 24576
+// 16.6 us against 19.3 without clusters and 22.3 with four SMs, but 1 x 1024 -> 2816 3.9 us without and 5.0 with two.
 template <typename T, int NT, int GROUP>
 bool ql_plan(const QlShape& s, int rows, int live, QlPlan* out) {
   constexpr int P = QlPieces<T>::N, BYTES = ql_unit_bytes(GROUP), SM = 148;
   constexpr double issue = (70 + 4 * (P == 1 ? 28 + 6 * NT : 48 + 18 * NT) + QL_CHANNELS / (P == 1 ? GROUP : 32) * (6 + 18 * NT));
   constexpr double products = 16 * NT * 2.1 * P;
   const int most[4] = {8, 8, 12, 16}, limit[4] = {113 * 1024, 227 * 1024, 227 * 1024, 227 * 1024}, resident[4] = {2, 1, 1, 1};
-  const double first[4] = {700, 2700, 3200, 3700}, more[4] = {3500, 5000, 6500, 8000};
+  const double first[4] = {1200, 2700, 3200, 3700}, more[4] = {3500, 5000, 6500, 8000};
   const int at_once[4] = {SM, 74, 33, 15};   // clusters of 1, 2, 4 and 8 SMs that the machine holds: they do not cross the borders of a GPC
   double best = -1;
   QlPlan p{};
