@@ -75,6 +75,9 @@ template <typename T> __device__ __forceinline__ T from_f32(float v);
 template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ bf16 from_f32<bf16>(float v) { return __float2bfloat16_rn(v); }
 
+// rows of skipped steps; a graph may be replayed any number of times
+__device__ __forceinline__ int kv_add_rows(int skipped, int rows) { return rows > 0x7fffffff - skipped ? 0x7fffffff : skipped + rows; }
+
 struct KvShape {
   int H, Hkv, HD, cap, rows;      // rows = new rows per sequence
   int first;                      // first sequence of the range
@@ -507,13 +510,16 @@ kv_partial_tc_kernel(const bf16* __restrict__ q, const bf16* __restrict__ knew, 
 // ---- merge the slices, write the merged heads, advance the cache lengths ----
 template <typename T>
 __global__ void kv_merge_kernel(const float* __restrict__ part, T* __restrict__ merged, int* __restrict__ lengths,
-                                const int* __restrict__ full, KvShape s, int splits) {
+                                const int* __restrict__ full, int* __restrict__ skipped, KvShape s, int splits) {
   const int PW = s.HD + 2;
   const int rh = blockIdx.x;                      // row * H + head
-  if (full[s.first + rh / s.H / s.rows]) {
+  const int row = rh / s.H, head = rh - row * s.H, seq = s.first + row / s.rows;
+  const bool speaks = head == 0 && row % s.rows == 0 && threadIdx.x == 0;   // one thread per sequence
+  if (full[seq]) {
     // the attention kernel found this sequence's cache full: zeros out, length unchanged; the mark stays
     // until the host reads it (kv_cache_lengths) or the sequence is truncated
     for (int c = threadIdx.x; c < s.HD; c += blockDim.x) merged[(size_t)rh * s.HD + c] = from_f32<T>(0.f);
+    if (speaks) skipped[seq] = kv_add_rows(skipped[seq], s.rows);
     return;
   }
   const float* src = part + (size_t)rh * splits * PW;
@@ -528,30 +534,42 @@ __global__ void kv_merge_kernel(const float* __restrict__ part, T* __restrict__ 
     }
     merged[(size_t)rh * s.HD + c] = from_f32<T>(den > 0.f ? num / den : 0.f);   // activations.rs:65-69
   }
-  // one thread per sequence moves its length on (every earlier launch of this step has read it)
-  const int row = rh / s.H, head = rh - row * s.H;
-  if (head == 0 && row % s.rows == 0 && threadIdx.x == 0) lengths[s.first + row / s.rows] += s.rows;
+  // every earlier launch of this step has read the length
+  if (speaks) {
+    lengths[seq] += s.rows;
+    skipped[seq] = 0;
+  }
 }
 
-__global__ void kv_set_lengths_kernel(int* lengths, int* full, int first, int count, int value) {
+__global__ void kv_set_lengths_kernel(int* lengths, int* full, int* skipped, int first, int count, int value) {
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
-  if (i < count) { lengths[first + i] = value; full[first + i] = 0; }
+  if (i < count) { lengths[first + i] = value; full[first + i] = 0; skipped[first + i] = 0; }
 }
 
 // A call that stores rows without attending to anything moves the lengths on by itself; a sequence without room is marked.
-__global__ void kv_advance_kernel(int* lengths, int* full, int first, int count, int rows, int cap) {
+__global__ void kv_advance_kernel(int* lengths, int* full, int* skipped, int first, int count, int rows, int cap) {
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
   pdl_follow();
   if (i >= count) return;
-  if (lengths[first + i] + rows > cap) full[first + i] = 1;
-  else lengths[first + i] += rows;
+  if (lengths[first + i] + rows > cap) {
+    full[first + i] = 1;
+    skipped[first + i] = kv_add_rows(skipped[first + i], rows);
+  } else {
+    lengths[first + i] += rows;
+    skipped[first + i] = 0;
+  }
 }
 
-// Takes the newest rows of every sequence back.  A sequence whose last step was skipped for want of room has nothing to take back.
-__global__ void kv_rollback_kernel(int* lengths, const int* full, int first, int count, int rows) {
+// Takes the newest rows of every sequence back.  The rows of steps that were skipped since the last one that was taken are the
+// newest of all: they count as taken back first, since nothing of them is there.  The mark of a skipped step is only a report
+// (it stays until the host reads it), so it does not decide.
+__global__ void kv_rollback_kernel(int* lengths, int* skipped, int first, int count, int rows) {
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
   pdl_follow();
-  if (i < count && !full[first + i]) lengths[first + i] = max(0, lengths[first + i] - rows);
+  if (i >= count) return;
+  const int never = min(rows, skipped[first + i]);
+  skipped[first + i] -= never;
+  lengths[first + i] = max(0, lengths[first + i] - (rows - never));
 }
 
 // The newest `rows` positions of every sequence as f32, one CTA per position; a position that is not held reads 0.
@@ -584,6 +602,7 @@ struct kv_cache {
   int* tickets = nullptr;           // 4-bit caches: CTAs of a sequence that are done with it, zero between calls
   int* lengths = nullptr;           // device, one per sequence
   int* full = nullptr;              // device, one per sequence: set by a step that found no room (a replayed graph can get there)
+  int* skipped = nullptr;           // device, one per sequence: rows of the steps skipped since the last one that was taken, less those taken back
   std::vector<int> host_full;
   std::vector<int> pages;           // 4-bit caches: scratch of a step's host side
   std::vector<int> host_len;        // mirror: every change goes through this object
@@ -708,7 +727,7 @@ int forward_t(kv_cache* c, int first, int n_seq, void* q, const void* k, const v
   }
   KCK(launch_partial<T>(c, (const T*)q, (const T*)k, (const T*)v, s, n_seq, splits, st));
   kv_merge_kernel<T><<<n_seq * rows * g.num_heads, std::min(256, std::max(32, g.head_dim)), 0, st>>>(
-      c->part, (T*)merged, c->lengths, c->full, s, splits);
+      c->part, (T*)merged, c->lengths, c->full, c->skipped, s, splits);
   count_launch();
   KCK(cudaGetLastError());
   for (int i = 0; i < n_seq; ++i) c->host_len[first + i] += rows;
@@ -717,7 +736,7 @@ int forward_t(kv_cache* c, int first, int n_seq, void* q, const void* k, const v
 
 q4::Cache q4_view(const kv_cache* c) {
   const kv_cache_config_t& g = c->cfg;
-  return q4::Cache{(unsigned char*)c->keys, c->lengths, c->full, c->tickets, c->cos_t, c->sin_t, g.num_heads, g.kv_heads, g.head_dim, g.capacity, g.rope};
+  return q4::Cache{(unsigned char*)c->keys, c->lengths, c->full, c->skipped, c->tickets, c->cos_t, c->sin_t, g.num_heads, g.kv_heads, g.head_dim, g.capacity, g.rope};
 }
 
 // The step on a 4-bit cache.  Nothing is allocated.
@@ -848,6 +867,8 @@ int32_t kv_cache_create(const kv_cache_config_t* config, kv_cache_t** out) {
   KCK(cudaMemset(c->lengths, 0, sizeof(int) * g.sequences));
   KCK(cudaMalloc(&c->full, sizeof(int) * g.sequences));
   KCK(cudaMemset(c->full, 0, sizeof(int) * g.sequences));
+  KCK(cudaMalloc(&c->skipped, sizeof(int) * g.sequences));
+  KCK(cudaMemset(c->skipped, 0, sizeof(int) * g.sequences));
   try {
     c->host_len.assign(g.sequences, 0);
     c->host_full.assign(g.sequences, 0);
@@ -890,7 +911,7 @@ int32_t kv_cache_create(const kv_cache_config_t* config, kv_cache_t** out) {
 
 void kv_cache_destroy(kv_cache_t* c) {
   if (!c) return;
-  cudaFree(c->keys); cudaFree(c->values); cudaFree(c->lengths); cudaFree(c->full); cudaFree(c->cos_t); cudaFree(c->sin_t);
+  cudaFree(c->keys); cudaFree(c->values); cudaFree(c->lengths); cudaFree(c->full); cudaFree(c->skipped); cudaFree(c->cos_t); cudaFree(c->sin_t);
   cudaFree(c->part); cudaFree(c->read_buf); cudaFree(c->tickets);
   delete c;
 }
@@ -905,7 +926,7 @@ int32_t kv_cache_truncate(kv_cache_t* c, int32_t sequence, int32_t length, void*
   for (int i = 0; i < count; ++i)
     if (c->host_len[first + i] < length)
       return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: sequence %d holds %d positions, cannot keep %d", first + i, c->host_len[first + i], length);
-  kv_set_lengths_kernel<<<ceil_div(count, 256), 256, 0, (cudaStream_t)stream>>>(c->lengths, c->full, first, count, length);
+  kv_set_lengths_kernel<<<ceil_div(count, 256), 256, 0, (cudaStream_t)stream>>>(c->lengths, c->full, c->skipped, first, count, length);
   count_launch();
   KCK(cudaGetLastError());
   for (int i = 0; i < count; ++i) c->host_len[first + i] = length;
@@ -926,6 +947,7 @@ int32_t kv_cache_lengths(kv_cache_t* c, int32_t* lengths_host, void* stream) {
   for (int i = 0; i < c->cfg.sequences; ++i)
     if (c->host_full[i]) {
       KCK(cudaMemsetAsync(c->full, 0, sizeof(int) * c->cfg.sequences, (cudaStream_t)stream));
+      KCK(cudaMemsetAsync(c->skipped, 0, sizeof(int) * c->cfg.sequences, (cudaStream_t)stream));   // the host knows now
       KCK(cudaStreamSynchronize((cudaStream_t)stream));
       return kv_fail(c, MOE_INVALID_INPUT, "SequenceTooLong: a step found the cache of sequence %d full at length %d of %d; the step was skipped for it (output zeros, nothing stored)",
                      i, c->host_len[i], c->cfg.capacity);
@@ -967,7 +989,7 @@ int32_t kv_cache_append(kv_cache_t* c, int32_t first, int32_t n_seq, const void*
     count_launch();
     KCK(cudaGetLastError());
   }
-  KCK(launch_following(kv_advance_kernel, ceil_div(n_seq, 256), 1, 256, 0, st, c->lengths, c->full, first, n_seq, rows, g.capacity));
+  KCK(launch_following(kv_advance_kernel, ceil_div(n_seq, 256), 1, 256, 0, st, c->lengths, c->full, c->skipped, first, n_seq, rows, g.capacity));
   for (int i = 0; i < n_seq; ++i) c->host_len[first + i] += rows;
   return MOE_OK;
 }
@@ -980,7 +1002,7 @@ int32_t kv_cache_rollback(kv_cache_t* c, int32_t first, int32_t n_seq, int32_t r
     if (c->host_len[first + i] < rows)
       return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: sequence %d holds %d positions, cannot drop %d", first + i, c->host_len[first + i], rows);
   KCK(cudaSetDevice(c->cfg.device));
-  KCK(launch_following(kv_rollback_kernel, ceil_div(n_seq, 256), 1, 256, 0, (cudaStream_t)stream, c->lengths, c->full, first, n_seq, rows));
+  KCK(launch_following(kv_rollback_kernel, ceil_div(n_seq, 256), 1, 256, 0, (cudaStream_t)stream, c->lengths, c->skipped, first, n_seq, rows));
   for (int i = 0; i < n_seq; ++i) c->host_len[first + i] -= rows;
   return MOE_OK;
 }

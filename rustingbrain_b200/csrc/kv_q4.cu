@@ -347,7 +347,10 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int len = c.lengths[seq], total = len + rows;
   if (total > c.cap) {                                // no room: nothing is stored or advanced, the step's rows are zeros
-    if (threadIdx.x == 0) c.full[seq] = 1;
+    if (threadIdx.x == 0) {
+      c.full[seq] = 1;
+      if (split == 0 && pass == 0 && kvh == 0) c.skipped[seq] = rows > 0x7fffffff - c.skipped[seq] ? 0x7fffffff : c.skipped[seq] + rows;
+    }
     if (split == 0)
       for (int i = threadIdx.x; i < min(QT, nq - q0) * HD; i += THREADS) {
         const int qi = q0 + i / HD, r = qi / group, g = qi - r * group;
@@ -491,6 +494,7 @@ attention_kernel(Cache c, const bf16* __restrict__ q, const bf16* __restrict__ k
     if (atomicAdd(c.tickets + seq, 1) == splits * passes * c.Hkv - 1) {
       c.tickets[seq] = 0;
       c.lengths[seq] = total;
+      c.skipped[seq] = 0;
     }
   }
   uint32_t qf[NQ][NG][4], qb[NQ][M::NP];              // fragments; pieces of the sums
@@ -852,6 +856,7 @@ merge_kernel(Cache c, const float* __restrict__ part, int first, int rows, int s
   if (threadIdx.x == 0 && atomicAdd(c.tickets + seq, 1) == rows * c.H - 1) {
     c.tickets[seq] = 0;
     c.lengths[seq] = total;
+    c.skipped[seq] = 0;
   }
 }
 

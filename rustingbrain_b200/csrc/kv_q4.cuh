@@ -17,6 +17,7 @@ struct Cache {
   unsigned char* pages;                // [sequence][kv head][page], page_bytes each
   int* lengths;                        // [sequence]
   int* full;                           // [sequence]: a step found no room
+  int* skipped;                        // [sequence]: rows of the steps skipped since the last one that was taken
   int* tickets;                        // [sequence], zero between calls
   const float *cos_t, *sin_t;          // [position][head_dim / 2]
   int H, Hkv, HD, cap, rope;

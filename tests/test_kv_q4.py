@@ -412,3 +412,87 @@ def test_the_result_may_take_the_queries_place(lens, rows):
     assert torch.equal(got, want) and bool((buf[S * rows:] == 7).all())
     with pytest.raises(InvalidInput):
         caches[1].forward_cached(q, k, v, rows_per_sequence=rows, out=torch.empty(S * rows, Hkv * hd, device="cuda", dtype=torch.bfloat16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("precision,what", [("q4", "step"), ("q4", "append"), ("bf16", "append"), ("f32", "append")])
+@pytest.mark.parametrize("drafts", [1, 3])
+def test_rollback_behind_a_step_that_was_skipped(precision, what, drafts):
+    """Captured: a step of four rows that does not fit, `drafts` steps of one row that do, and their rollback.  What was skipped left
+    nothing behind, what was taken goes again; a rollback over both takes back only what is there."""
+    H, Hkv, hd, cap, n = 4, 2, 64, 12, 9
+    cache = KvCache(2, H, Hkv, hd, cap, precision=precision)
+    dt = torch.float32 if precision == "f32" else torch.bfloat16
+    dev = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda().to(dt)
+    _, k0, v0 = _rows(n, H, Hkv, hd, 70)
+    cache.append(dev(k0[:6]), dev(v0[:6]), rows_per_sequence=6, first_sequence=0, n_sequences=1)
+    cache.append(dev(k0[:2]), dev(v0[:2]), rows_per_sequence=2, first_sequence=1, n_sequences=1)
+    side, graphs, data = torch.cuda.Stream(), {}, {}
+    torch.cuda.synchronize()
+    for rows in (4, 1):                                        # captured while the host's copy of the lengths says that they fit
+        data[rows] = tuple(dev(a) for a in _rows(rows, H, Hkv, hd, 71 + rows))
+        graphs[rows] = torch.cuda.CUDAGraph()
+        q, k, v = data[rows]
+        with torch.cuda.graph(graphs[rows], stream=side):
+            if what == "step":
+                data[rows] += (cache.forward_cached(q, k, v, rows_per_sequence=rows, first_sequence=0, n_sequences=1),)
+            else:
+                cache.append(k, v, rows_per_sequence=rows, first_sequence=0, n_sequences=1)
+    assert cache.lengths() == [6, 2]
+    cache.append(dev(k0[6:]), dev(v0[6:]), rows_per_sequence=n - 6, first_sequence=0, n_sequences=1)
+    before = None if precision != "q4" else Q4CacheOracle(H, Hkv, hd, cap)
+    if before is not None:
+        before.append(k0, v0)
+    torch.cuda.synchronize()
+    graphs[4].replay()                                         # 9 + 4 > 12: skipped
+    for _ in range(drafts):
+        graphs[1].replay()                                     # up to 12
+    torch.cuda.synchronize()
+    if what == "step":
+        assert float(data[4][3].abs().max()) == 0 and float(data[1][3].abs().max()) > 0
+    cache.rollback(drafts, first_sequence=0, n_sequences=1)
+    with pytest.raises(InvalidInput, match="SequenceTooLong"):
+        cache.lengths()
+    assert cache.lengths() == [n, 2]
+    if before is not None:
+        _same_cache(cache, 0, before)
+    for _ in range(5):                                         # three fit, two do not
+        graphs[1].replay()
+    torch.cuda.synchronize()
+    cache.rollback(1, first_sequence=0, n_sequences=1)         # of the two
+    cache.rollback(2, first_sequence=0, n_sequences=1)         # the other, and the newest that is there
+    with pytest.raises(InvalidInput, match="SequenceTooLong"):
+        cache.lengths()
+    assert cache.lengths() == [cap - 1, 2]
+    cache.rollback(1)                                          # nothing is owed any more, and the other sequence is an ordinary one
+    assert cache.lengths() == [cap - 2, 1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("precision", ["bf16", "f32"])
+def test_rollback_of_steps_that_a_marked_cache_skips(precision):
+    """The caches of 16 and 32 bits take no step while a mark is unread: those rows are taken back without a trace too."""
+    H, Hkv, hd, cap = 4, 2, 64, 8
+    cache = KvCache(1, H, Hkv, hd, cap, precision=precision)
+    dt = torch.float32 if precision == "f32" else torch.bfloat16
+    q, k, v = (torch.from_numpy(a).cuda().to(dt) for a in _rows(3, H, Hkv, hd, 80))
+    cache.forward_cached(q, k, v, rows_per_sequence=3)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.forward_cached(q.clone(), k, v, rows_per_sequence=3)
+    assert cache.lengths() == [3]
+    for _ in range(3):                                         # 6, then twice no room
+        graph.replay()
+    torch.cuda.synchronize()
+    cache.rollback(1)
+    cache.rollback(2)                                          # the second of the skipped steps
+    with pytest.raises(InvalidInput, match="SequenceTooLong"):
+        cache.lengths()
+    assert cache.lengths() == [6]
+    graph.replay()
+    torch.cuda.synchronize()
+    cache.rollback(4)                                          # a skipped step and one row
+    with pytest.raises(InvalidInput, match="SequenceTooLong"):
+        cache.lengths()
+    assert cache.lengths() == [5]
