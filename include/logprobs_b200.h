@@ -9,7 +9,8 @@
  *
  *   grad_x[r, v] = grad_logprob[r] * (1[v == target[r]] - p[r, v]) - grad_entropy[r] * p[r, v] * (log p[r, v] + entropy[r])
  *
- * Sums are f32 whatever the logits' type.  Edge values:
+ * Sums are f32 whatever the logits' type.  Log probabilities are never above 0; the one of a near-certain token is off by about 2^-23, not by a
+ * part of itself.  Edge values:
  *   - a masked logit is -inf: probability 0, nothing added to the entropy, gradient 0; it may appear among the
  *     alternatives (with log probability -inf) once the others are used up.  Lowest finite values are ordinary values.
  *   - a row of -inf only has no distribution: lse = logprob = -inf, entropy 0, gradient 0.

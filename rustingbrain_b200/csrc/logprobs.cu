@@ -494,13 +494,15 @@ logprobs_kernel(const T* __restrict__ x, long long stride, const int* __restrict
   }
   __syncthreads();
   total = sh.cta;
-  // y - log2 s keeps the small numbers small: the log probability of a near-certain token is accurate relative to itself
+  // y - log2 s keeps the small numbers small.  What is left of a near-certain token is off by 2^-23 or so: s has the token's own 2^y beside
+  // the rest, and neither that nor its logarithm is exact.  So it can come out above 0, where no log probability is.
   const float l2 = log2f(total.s);
   const bool empty = total.s == 0.f;                // nothing but -inf
   auto log_p = [&](float f) {
     if (empty) return f != f ? f : -INFINITY;
-    if (fabsf(f) > LP_BIG || fabsf(total.m) > LP_BIG) return (f - total.m) - l2 * LP_LN2;   // the lowest finite value stays finite
-    return (lp_y(f, total.m) - l2) * LP_LN2;
+    const float v = fabsf(f) > LP_BIG || fabsf(total.m) > LP_BIG ? (f - total.m) - l2 * LP_LN2   // the lowest finite value stays finite
+                                                                 : (lp_y(f, total.m) - l2) * LP_LN2;
+    return v > 0.f ? 0.f : v;
   };
   if (tid == 0) {
     const float lse = empty ? -INFINITY : fabsf(total.m) > LP_BIG ? fmaf(l2, LP_LN2, total.m) : (__fmul_rn(total.m, LP_LOG2E) + l2) * LP_LN2;

@@ -299,3 +299,24 @@ def test_results_do_not_depend_on_the_run():
     first = token_logprobs(x, t, top=8)
     for _ in range(5):
         assert all(torch.equal(a, b) for a, b in zip(first, token_logprobs(x, t, top=8)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_no_probability_above_one(dtype):
+    """One token left, logits of every size: its log probability is 0, and what rounding leaves of it is not above 0."""
+    from rustingbrain_b200.logprobs import token_logprobs
+    rows, V = 4096, 40
+    x = torch.full((rows, V), -INF, device="cuda")
+    t = torch.arange(rows, device="cuda") % V
+    x[torch.arange(rows, device="cuda"), t] = torch.linspace(-40, 40, rows, device="cuda")
+    x, t = x.to(dtype), t.to(torch.int32)
+    got = token_logprobs(x, t, top=2)
+    _check(x, t, 2, got)
+    assert float(got.logprob.max()) <= 0 and float(got.top_logprobs.max()) <= 0
+    assert float(got.entropy.min()) >= 0
+    x[1::2, :] = 0.0                             # a peak far above the others
+    x[torch.arange(rows, device="cuda"), t.long()] += 30.0
+    got = token_logprobs(x, t, top=2)
+    _check(x, t, 2, got)
+    assert float(got.logprob.max()) <= 0 and float(got.top_logprobs.max()) <= 0
