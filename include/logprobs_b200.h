@@ -40,7 +40,8 @@ int32_t logprobs_forward(const void* x, int64_t row_stride, const int32_t* targe
                          int32_t precision, float* logprob, float* entropy, float* lse, float* top_logprob, int32_t* top_ids,
                          void* stream, char* message, int32_t message_len);
 
-/* grad_x has x's type, its rows grad_stride elements apart; it may be x itself (same stride), otherwise the two do not overlap.
+/* grad_x has x's type, its rows grad_stride elements apart; it may be x itself (same stride); otherwise the two share
+ * nothing, though their rows may lie between one another, and an overlap is InvalidInput.
  * lse and entropy are the forward call's.  grad_logprob or grad_entropy may be null: no such term (entropy may then be null too). */
 int32_t logprobs_backward(const void* x, int64_t row_stride, const int32_t* targets, const float* lse, const float* entropy,
                           const float* grad_logprob, const float* grad_entropy, int32_t rows, int32_t vocab, int32_t precision,

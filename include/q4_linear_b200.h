@@ -40,7 +40,8 @@ int32_t q4_linear_quantize(const float* weights, void* packed, int32_t d_out, in
 int32_t q4_linear_dequantize(const void* packed, float* weights, int32_t d_out, int32_t d_in, int32_t group, void* stream, char* message,
                              int32_t message_len);
 
-/* x rows are ld_x elements apart and start on 16-byte boundaries; y rows are ld_y elements apart.  y does not overlap x.
+/* x rows are ld_x elements apart and start on 16-byte boundaries; y rows are ld_y elements apart.  y does not overlap x
+ * (InvalidInput), though their rows may lie between one another.
  * rows is at most 65535; rows == 0 is a call that does nothing. */
 int32_t q4_linear_forward(const void* x, int64_t ld_x, const void* packed, void* y, int64_t ld_y, int32_t rows, int32_t d_in,
                           int32_t d_out, int32_t group, int32_t precision, void* stream, char* message, int32_t message_len);

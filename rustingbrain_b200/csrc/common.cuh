@@ -81,6 +81,21 @@ inline cudaError_t launch_following(void (*kernel)(Params...), unsigned grid, un
   return cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
 }
 
+// Whether `rows` rows of a_bytes, a_ld bytes apart, share a byte with as many of b_bytes, b_ld apart.  Rows may lie between one another.
+inline bool rows_overlap(const void* a, long long a_ld, const void* b, long long b_ld, long long a_bytes, long long b_bytes, long long rows) {
+  const long long at = (long long)reinterpret_cast<uintptr_t>(a), bt = (long long)reinterpret_cast<uintptr_t>(b);
+  if (at >= bt + (rows - 1) * b_ld + b_bytes || bt >= at + (rows - 1) * a_ld + a_bytes) return false;
+  for (long long i = 0; i < rows; ++i) {
+    const long long from = at + i * a_ld - bt, to = from + a_bytes;     // the row, counted from b
+    if (to <= 0) continue;
+    // the first row of b that ends behind `from`: it is the one that begins first of those
+    const long long j = from < b_bytes ? 0 : (from - b_bytes) / b_ld + 1;
+    if (j < rows && j * b_ld < to) return true;
+    if (rows > 1 && a_ld == b_ld && i > 0) break;                       // the further rows lie alike
+  }
+  return false;
+}
+
 __host__ __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 __host__ __device__ inline int round_up(int a, int b) { return ceil_div(a, b) * b; }
 

@@ -653,6 +653,8 @@ int32_t logprobs_backward(const void* x, int64_t row_stride, const int32_t* targ
   const size_t elem = precision == MOE_PRECISION_BF16 ? 2 : 4;
   if (reinterpret_cast<uintptr_t>(x) % elem || reinterpret_cast<uintptr_t>(grad_x) % elem)
     return lp_fail(message, message_len, MOE_INVALID_INPUT, "InvalidInput: buffers are not aligned to their type");
+  if (x != grad_x && rows_overlap(x, (long long)row_stride * elem, grad_x, (long long)grad_stride * elem, (long long)vocab * elem, (long long)vocab * elem, rows))
+    return lp_fail(message, message_len, MOE_INVALID_INPUT, "InvalidInput: the gradient overlaps the logits and is not in their place");
   const long long per_run = (long long)LP_THREADS * LP_UNROLL * (16 / elem);
   const long long runs = (vocab + per_run - 1) / per_run;
   if (runs * rows > 0x7fffffffll) return lp_fail(message, message_len, MOE_INVALID_INPUT, "InvalidInput: too many rows");

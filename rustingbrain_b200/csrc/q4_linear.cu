@@ -685,14 +685,9 @@ int32_t q4_linear_forward(const void* x, int64_t ld_x, const void* packed, void*
   if (!x || !y) return ql_fail(message, message_len, MOE_INVALID_INPUT, "InvalidInput: null buffer");
   if (reinterpret_cast<uintptr_t>(x) % 16 || (rows > 1 && (ld_x * elem) % 16) || reinterpret_cast<uintptr_t>(y) % elem)
     return ql_fail(message, message_len, MOE_INVALID_INPUT, "InvalidInput: rows of x start on 16-byte boundaries");
-  // x is read while y is written: their rows may lie in one buffer side by side, but share nothing
-  const long long xa = (long long)reinterpret_cast<uintptr_t>(x), ya = (long long)reinterpret_cast<uintptr_t>(y);
-  const long long x_end = xa + ((rows - 1) * (long long)ld_x + d_in) * elem, y_end = ya + ((rows - 1) * (long long)ld_y + d_out) * elem;
-  if (xa < y_end && ya < x_end) {
-    const long long row = (long long)ld_x * elem, apart = ((ya - xa) % row + row) % row;     // from a row of x to the next of y behind it
-    if (rows == 1 || ld_x != ld_y || apart < (long long)d_in * elem || apart + (long long)d_out * elem > row)
-      return ql_fail(message, message_len, MOE_INVALID_INPUT, "InvalidInput: y overlaps x");
-  }
+  // x is read while y is written
+  if (rows_overlap(x, (long long)ld_x * elem, y, (long long)ld_y * elem, (long long)d_in * elem, (long long)d_out * elem, rows))
+    return ql_fail(message, message_len, MOE_INVALID_INPUT, "InvalidInput: y overlaps x");
   const QlShape s = ql_shape(d_out, d_in, group);
   const cudaError_t e = precision == MOE_PRECISION_BF16 ? ql_dispatch<bf16>(x, ld_x, packed, y, ld_y, rows, s, (cudaStream_t)stream)
                                                         : ql_dispatch<float>(x, ld_x, packed, y, ld_y, rows, s, (cudaStream_t)stream);

@@ -320,3 +320,41 @@ def test_no_probability_above_one(dtype):
     got = token_logprobs(x, t, top=2)
     _check(x, t, 2, got)
     assert float(got.logprob.max()) <= 0 and float(got.top_logprobs.max()) <= 0
+
+
+def test_a_gradient_that_overlaps_the_logits_is_refused():
+    """In place, or beside the logits: anything else would overwrite logits that another row's gradient has yet to read."""
+    buf = (C.c_float * 256)()
+    p = C.addressof(buf)
+
+    def back(x, xs, g, gs, rows, vocab=8, precision=_lib.PRECISION_F32):
+        msg = C.create_string_buffer(128)
+        o = C.c_void_p(p)
+        rc = _lib.lib().logprobs_backward(C.c_void_p(p + x), xs, None, o, o, o, o, rows, vocab, precision, C.c_void_p(p + g), gs, None, msg, 128)
+        return rc, msg.value
+    for bad in ((0, 8, 4, 8, 1), (4, 8, 0, 8, 1), (0, 8, 28, 8, 1), (0, 8, 32, 8, 2), (0, 16, 16, 16, 3), (0, 16, 60, 16, 3), (0, 16, 36, 16, 3),
+                (0, 16, 32, 24, 3), (64, 16, 4, 8, 3), (0, 8, 8, 8, 1, 8, _lib.PRECISION_BF16)):
+        rc, text = back(*bad)
+        assert rc == _lib.INVALID_INPUT and b"overlap" in text, bad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradients_beside_their_logits(dtype):
+    """Rows of the gradient between those of the logits, on either side and at distances of their own."""
+    from rustingbrain_b200.logprobs import token_logprobs, token_logprobs_backward
+    V, rows = 100, 5
+    g = torch.linspace(-1, 1, rows, device="cuda")
+    t = torch.arange(rows, device="cuda", dtype=torch.int32)
+    for x_at, x_step, d_at, d_step in ((0, 200, 100, 200), (100, 200, 0, 200), (0, 213, 107, 213), (0, 200, 100, 400), (100, 600, 0, 300), (0, 100, 500, 300)):
+        buf = torch.full((4000,), 7.0, device="cuda", dtype=dtype)
+        x = buf.as_strided((rows, V), (x_step, 1), x_at)
+        d = buf.as_strided((rows, V), (d_step, 1), d_at)
+        x.copy_(_logits(rows, V, dtype, 50))
+        base = x.clone()
+        f = token_logprobs(x, t)
+        want = token_logprobs_backward(base, t, f.lse, f.entropy, g, g)
+        token_logprobs_backward(x, t, f.lse, f.entropy, g, g, out=d)
+        assert torch.equal(d, want) and torch.equal(x, base)
+    with pytest.raises(InvalidInput, match="overlap"):
+        token_logprobs_backward(x, t, f.lse, f.entropy, g, g, out=buf.as_strided((rows, V), (x_step, 1), 50))
