@@ -546,8 +546,9 @@ logprobs_backward_kernel(const T* x, long long stride, const int* __restrict__ t
   const int mis = (int)((reinterpret_cast<uintptr_t>(xr) & 15) / sizeof(T));
   const bool wide = ((reinterpret_cast<uintptr_t>(xr) ^ reinterpret_cast<uintptr_t>(gr)) & 15) == 0;
   if (!wide) {
-    const int end = (int)min((long long)vocab, (long long)(run + 1) * RUN * N);
-    for (int i = run * RUN * N + (int)threadIdx.x; i < end; i += LP_THREADS) gr[i] = from_f32<T>(one(to_f32<T>(xr[i]), i));
+    // unsigned: the last step passes a vocabulary of 2^31 - 1
+    const unsigned end = (unsigned)min((long long)vocab, (long long)(run + 1) * RUN * N);
+    for (unsigned i = (unsigned)run * RUN * N + threadIdx.x; i < end; i += LP_THREADS) gr[i] = from_f32<T>(one(to_f32<T>(xr[i]), (int)i));
     return;
   }
   const int head = min(vocab, mis ? N - mis : 0), vecs = (vocab - head) / N, tail = head + vecs * N;

@@ -358,3 +358,25 @@ def test_gradients_beside_their_logits(dtype):
         assert torch.equal(d, want) and torch.equal(x, base)
     with pytest.raises(InvalidInput, match="overlap"):
         token_logprobs_backward(x, t, f.lse, f.entropy, g, g, out=buf.as_strided((rows, V), (x_step, 1), 50))
+
+
+@pytest.mark.gpu
+def test_the_largest_vocabulary():
+    """A row of 2^31 - 1 logits, whose gradient lies off their 16-byte boundary: indices end at the last number of 31 bits."""
+    from rustingbrain_b200.logprobs import token_logprobs, token_logprobs_backward
+    V = 2 ** 31 - 1
+    x = torch.zeros(1, V, device="cuda", dtype=torch.bfloat16)
+    x[0, V - 1], x[0, 5] = 4.0, 3.0
+    t = torch.tensor([V - 1], device="cuda", dtype=torch.int32)
+    got = token_logprobs(x, t, top=3)
+    assert got.top_ids[0].tolist() == [V - 1, 5, 0]
+    lse, g = torch.ones(1, device="cuda"), torch.ones(1, device="cuda")
+    for shift in (0, 1):
+        flat = torch.full((V + 9,), 7.0, device="cuda", dtype=torch.bfloat16)
+        out = flat[shift:shift + V].view(1, V)
+        token_logprobs_backward(x, t, lse, grad_logprob=g, out=out)
+        for at, want in ((0, -np.exp(-1.0)), (5, -np.exp(2.0)), (V // 2, -np.exp(-1.0)), (V - 2, -np.exp(-1.0)), (V - 1, 1 - np.exp(3.0))):
+            assert abs(float(out[0, at]) - want) <= abs(want) * (2.0 ** -8 + 2.0 ** -20), (shift, at)
+        assert int((out == out[0, 0]).sum()) == V - 2
+        assert bool((flat[:shift] == 7).all()) and bool((flat[shift + V:] == 7).all())
+        del flat, out
