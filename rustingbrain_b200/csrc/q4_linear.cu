@@ -7,11 +7,12 @@
 // (32 outputs) and their scales are a unit, which a warp brings into its own ring in shared memory, several units ahead.
 //
 // A code plus 8 needs no conversion: bits 0 .. 7 of a bf16 are a number linear in them, bits * 2^-133 (below 128 it is subnormal, and the
-// next binade goes on in the same steps).  So a code is cut out of its word and is an operand, at weight 1 or, where it comes out four
-// bits further up, 16: five instructions for eight codes.  The activations make up for the powers of two, and the 8 that the codes have
-// too much is where the sum of a group starts: -8 times the sum of its activations.  Products are exact, and the group's scale is applied
-// to its f32 sum.  An f32 activation is three bf16 numbers that add up to it; there the 8 is taken off the codes, whose sums then
-// stay small enough for the accuracy of f32.
+// next binade goes on in the same steps).  So a code is cut out of its word, at weight 1 or, where it comes out four bits further up, 16, and one
+// packed subtraction takes the 8 off: nine instructions for eight codes.  The activations make up for the powers of two.  Products are
+// exact, and the group's scale is applied to its f32 sum.  An f32 activation is three bf16 numbers that add up to it.
+// (Without the subtraction a group's sum has to start at -8 times the sum of its activations.  That is 12 % faster for 8 x 4096 -> 24576, the
+// same for 64 rows, and wrong: the tensor cores cut the terms of a product off at 2^-23 or so of the largest, so a channel 1e5 times as large as its
+// neighbours takes 1 % off the result even where all its codes are 0.)
 // (e4m3 operands would take three instructions for eight codes, but mma.sync has no e4m3 product of its own here: it costs two bf16 ones
 // and the conversions.)
 //
@@ -141,11 +142,11 @@ __device__ __forceinline__ void ql_mma_bf16(float* c, uint32_t a0, uint32_t a1, 
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// the same with a start of its own
-__device__ __forceinline__ void ql_mma_bf16(float* d, const float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+// the same from zero
+__device__ __forceinline__ void ql_mma_bf16_new(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void ql_copy16(uint32_t smem, const void* gmem) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
@@ -154,7 +155,7 @@ __device__ __forceinline__ void ql_copy16(uint32_t smem, const void* gmem) {
 template <int I>
 __device__ __forceinline__ uint32_t ql_raw(uint32_t w) { return (I < 2 ? w : w >> 8) & (I & 1 ? 0x00f000f0u : 0x000f000fu); }
 
-// ... less 8 (or 128): the codes themselves
+// ... less 8 (or 128): the codes themselves, and exactly 0 for a code of 0
 template <int I>
 __device__ __forceinline__ uint32_t ql_signed(uint32_t w) {
   const uint32_t v = ql_raw<I>(w), eight = I & 1 ? 0x00800080u : 0x00080008u;
@@ -178,7 +179,7 @@ __device__ __forceinline__ void ql_split(float x, uint32_t* p) {
   }
 }
 // Eight activations as they were loaded.  `plain` ones (finite, at most QL_LARGE) become operands here: times 2^QL_UP, and 2^-4 less where the
-// code weighs 16; returned is their sum.
+// code weighs 16.
 template <typename T> constexpr int QL_BATCH = sizeof(T) == 2 ? 4 : 2;
 template <typename T> struct QlRaw;
 template <> struct QlRaw<bf16> {
@@ -201,11 +202,8 @@ template <> struct QlRaw<bf16> {
     const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(__habs2(pair(a.v.x)), __habs2(pair(a.v.y))), __hmax2_nan(__habs2(pair(a.v.z)), __habs2(pair(a.v.w))));
     return __low2float(m) <= QL_LARGE && __high2float(m) <= QL_LARGE;
   }
-  static __device__ __forceinline__ float plain_pieces(const type& a, uint4* out) {
-    float f[8];
-    widen(a, f);
+  static __device__ __forceinline__ void plain_pieces(const type& a, uint4* out) {
     out[0] = make_uint4(times(a.v.x, ql_pow2(QL_UP)), times(a.v.y, ql_pow2(QL_UP - 4)), times(a.v.z, ql_pow2(QL_UP)), times(a.v.w, ql_pow2(QL_UP - 4)));
-    return ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
   }
 };
 template <> struct QlRaw<float> {
@@ -223,7 +221,7 @@ template <> struct QlRaw<float> {
     for (int j = 0; j < 8; ++j) ok &= fabsf(f[j]) <= QL_LARGE;
     return ok;
   }
-  static __device__ __forceinline__ float plain_pieces(const type& t, uint4* out) {
+  static __device__ __forceinline__ void plain_pieces(const type& t, uint4* out) {
     float f[8];
     uint32_t p[8][3];
     widen(t, f);
@@ -239,21 +237,19 @@ template <> struct QlRaw<float> {
 #pragma unroll
     for (int q = 0; q < 3; ++q)
       out[q] = make_uint4(p[0][q] >> 16 | p[1][q], p[2][q] >> 16 | p[3][q], p[4][q] >> 16 | p[5][q], p[6][q] >> 16 | p[7][q]);
-    return 0.f;                                       // not used: the codes are taken without their 8
   }
 };
 
 template <typename T> struct QlPieces { static constexpr int N = 1; };
 template <> struct QlPieces<float> { static constexpr int N = 3; };
 
-// How a launch cuts the product, and where things lie in shared memory: marks of the rows first; then the starts of the group sums
-// [group][NT * 8] f32; the activations [piece][row][2 bytes a channel, and 64 that keep the 16-byte loads of a warp off each
+// How a launch cuts the product, and where things lie in shared memory: marks of the rows first; then the activations [piece][row][2 bytes a channel, and 64 that keep the 16-byte loads of a warp off each
 // other's banks]; the warps' rings; the partial sums [buffer][wk][row][outputs of the tile] f32.
 struct QlPlan {
   int warps, wk, cluster;              // warps of a CTA, those of them along the reduction; CTAs along it
   int tiles, passes, clusters;         // tiles of outputs; passes over the rows; clusters that share the tiles of a pass
   int slice, per_pass, stages, buffers;   // units of the reduction per CTA, at most; rows per pass; units in a ring; buffers of partial sums
-  int starts, acts, rings, sums, bytes;
+  int acts, rings, sums, bytes;
 };
 constexpr int QL_FRONT = 2 * QL_ROWS * 4;
 
@@ -274,7 +270,6 @@ q4_linear_kernel(const T* __restrict__ x, long long ld_x, const unsigned char* _
   const int pitch = plan.slice * QL_CHANNELS * 2 + 64, plane = rows * pitch;
   int* mark = reinterpret_cast<int*>(ql_sm);                      // by row: one above QL_LARGE is there
   int* odd = mark + QL_ROWS;                                      // something infinite or NaN is there
-  float* start = reinterpret_cast<float*>(ql_sm + plan.starts);
   unsigned char* acts = ql_sm + plan.acts;
 
   // ---- the warp's units: of the tiles tile0, tile0 + clusters, .. those from ubeg + wk on in steps of wk_count ----
@@ -331,31 +326,25 @@ q4_linear_kernel(const T* __restrict__ x, long long ld_x, const unsigned char* _
         if (i0 + u * threads >= work) break;                      // the same for the whole warp
         const int row = rb[u];
         uint4 out[P];
-        float sum;
         if (QlRaw<T>::plain(raw[u]) && !(again && mark[row])) {
-          sum = QlRaw<T>::plain_pieces(raw[u], out);
+          QlRaw<T>::plain_pieces(raw[u], out);
         } else {
           // something large, infinite or NaN
           const float by = again && mark[row] ? ql_pow2(QL_UP - QL_DOWN) : ql_pow2(QL_UP);
           float f[8];
           uint32_t p[8][3];
           QlRaw<T>::widen(raw[u], f);
-          sum = 0.f;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             if (!ql_finite(f[j])) { odd[row] = 1; f[j] = 0.f; }
             if (!again && fabsf(f[j]) > QL_LARGE) { mark[row] = 1; large = true; }
             f[j] *= by;
-            sum += f[j] * ql_pow2(-QL_UP);
             ql_split(f[j] * (j & 2 ? 0.0625f : 1.f), p[j]);
           }
 #pragma unroll
           for (int q = 0; q < P; ++q) out[q] = make_uint4(p[0][q] | p[1][q] << 16, p[2][q] | p[3][q] << 16, p[4][q] | p[5][q] << 16, p[6][q] | p[7][q] << 16);
         }
-#pragma unroll
-        for (int o = 1; P == 1 && o < GROUP / 8; o *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (i0 + u * threads + lane >= work) continue;
-        if (P == 1 && (cb[u] & (GROUP - 1)) == 0) start[(cb[u] / GROUP) * (NT * 8) + row] = sum * (ql_pow2(QL_UP - QL_RAW) * -8.f);
 #pragma unroll
         for (int q = 0; q < P; ++q) *reinterpret_cast<uint4*>(acts + q * plane + row * pitch + cb[u] * 2) = out[q];
       }
@@ -419,28 +408,17 @@ q4_linear_kernel(const T* __restrict__ x, long long ld_x, const unsigned char* _
 #pragma unroll
           for (int m = 0; m < 2; ++m) {
             const uint32_t lo = g ? w[m].z : w[m].x, hi = g ? w[m].w : w[m].y;
-            if constexpr (P == 1) {
-              a[m][0] = ql_raw<0>(lo); a[m][1] = ql_raw<0>(hi); a[m][2] = ql_raw<1>(lo); a[m][3] = ql_raw<1>(hi);
-              a[m][4] = ql_raw<2>(lo); a[m][5] = ql_raw<2>(hi); a[m][6] = ql_raw<3>(lo); a[m][7] = ql_raw<3>(hi);
-            } else {
-              a[m][0] = ql_signed<0>(lo); a[m][1] = ql_signed<0>(hi); a[m][2] = ql_signed<1>(lo); a[m][3] = ql_signed<1>(hi);
-              a[m][4] = ql_signed<2>(lo); a[m][5] = ql_signed<2>(hi); a[m][6] = ql_signed<3>(lo); a[m][7] = ql_signed<3>(hi);
-            }
+            a[m][0] = ql_signed<0>(lo); a[m][1] = ql_signed<0>(hi); a[m][2] = ql_signed<1>(lo); a[m][3] = ql_signed<1>(hi);
+            a[m][4] = ql_signed<2>(lo); a[m][5] = ql_signed<2>(hi); a[m][6] = ql_signed<3>(lo); a[m][7] = ql_signed<3>(hi);
           }
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            float from[4] = {0.f, 0.f, 0.f, 0.f};
-            if (P == 1 && opens) {
-              const float2 v = *reinterpret_cast<const float2*>(start + (c0 / GROUP + grp) * (NT * 8) + n * 8 + 2 * tig);
-              from[0] = from[2] = v.x;
-              from[1] = from[3] = v.y;
-            }
 #pragma unroll
             for (int q = 0; q < P; ++q) {
               const uint4 b = *reinterpret_cast<const uint4*>(mine[n] + q * plane + off);
 #pragma unroll
               for (int m = 0; m < 2; ++m) {
-                if (opens && q == 0) ql_mma_bf16(part[m][n], from, a[m][0], a[m][1], a[m][2], a[m][3], b.x, b.y);
+                if (opens && q == 0) ql_mma_bf16_new(part[m][n], a[m][0], a[m][1], a[m][2], a[m][3], b.x, b.y);
                 else ql_mma_bf16(part[m][n], a[m][0], a[m][1], a[m][2], a[m][3], b.x, b.y);
                 ql_mma_bf16(part[m][n], a[m][4], a[m][5], a[m][6], a[m][7], b.z, b.w);
               }
@@ -469,7 +447,7 @@ q4_linear_kernel(const T* __restrict__ x, long long ld_x, const unsigned char* _
       }
     const int n0 = tile * width;
     if (any_odd) {
-      // infinities and NaN took part as 0 above (an infinity against a sum's start would be NaN): add what they really give
+      // infinities and NaN took part as 0 above (cut into pieces an infinity would be NaN): add what they really give
       __syncthreads();
       for (int i = threadIdx.x; i < rows * width; i += threads) {
         const int r = i / width, n = n0 + i % width;
@@ -543,8 +521,7 @@ bool ql_plan(const QlShape& s, int rows, int live, QlPlan* out) {
       p.warps = most[way];
       p.slice = (s.units + p.cluster - 1) / p.cluster;
       if (p.cluster > 1 && s.units < 2 * p.cluster) break;
-      p.starts = QL_FRONT;
-      p.acts = p.starts + up(p.slice * QL_CHANNELS / GROUP * NT * 8 * 4);
+      p.acts = QL_FRONT;
       p.rings = p.acts + up(P * live * (p.slice * QL_CHANNELS * 2 + 64));
       const int sums = live * 32 * p.warps * 4;
       bool fits = false;

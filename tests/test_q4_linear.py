@@ -198,3 +198,50 @@ def test_rows_of_x_and_y_side_by_side_in_one_buffer():
     _check(y, x, w)
     with pytest.raises(InvalidInput, match="overlaps"):
         layer(x, out=buf[:, 60:100])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("ratio", [2.0 ** 4, 2.0 ** 10, 2.0 ** 17])
+def test_an_outlier_whose_codes_are_zero(group, ratio):
+    """bf16: a code enters as code + 8, so a channel costs its group accuracy whatever its codes.  A product of the tensor core adds 16 numbers
+    and the sum so far, each cut off at 2^-23 of the largest, which is at most 15 times the group's sum of |x|; group / 16 products: 17 * 15 / 16 *
+    group * 2^-23, below group * 2^-19, of scale * sum |x|.  That is the header's bound; the mean over channels stays far below it."""
+    from rustingbrain_b200.q4_linear import Q4Linear
+    g = torch.Generator(device="cuda").manual_seed(31)
+    d_in, d_out, rows = 512, 200, 9
+    codes = torch.randint(-8, 8, (d_out, d_in), device="cuda", generator=g).to(torch.int8)
+    codes[:, 77] = 0
+    scales = (torch.rand(d_out, d_in // group, device="cuda", generator=g) + 0.1).bfloat16()
+    layer = Q4Linear(d_in, d_out, group_size=group)
+    layer.set_codes(codes, scales)
+    w = codes.double() * scales.double().repeat_interleave(group, dim=1)
+    x = torch.randn(rows, d_in, device="cuda", generator=g).bfloat16()
+    x[:, 77] = ratio
+    y, want = layer.forward(x), x.double() @ w.t()
+    sums = x.double().abs().view(rows, -1, group).sum(2)                        # [rows, groups]
+    cut = (sums @ scales.double().t()) * group * 2.0 ** -19
+    tol = want.abs() * 2.0 ** -8 + cut + (x.double().abs() @ w.abs().t()) * d_in * 2.0 ** -24
+    assert bool(((y.double() - want).abs() <= tol).all())
+    # a half step of bf16 and, of outputs of 4.6 * sqrt(512) scales, the outlier's part: 2^-23 of 8 ratio for each of group / 16 products
+    rel = float((y.double() - want).norm() / want.norm())
+    assert rel <= 2.0 ** -8 + ratio * 8 * 2.0 ** -23 * (group / 16) / (4.6 * 512 ** 0.5) * 2, rel
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,rows,d_in,group", [(torch.float32, 9, 16384, 32), (torch.float32, 16, 16416, 32), (torch.float32, 17, 65536, 128),
+                                                   (torch.float32, 1, 65536, 64), (torch.bfloat16, 9, 49152, 32), (torch.bfloat16, 16, 65536, 64),
+                                                   (torch.bfloat16, 40, 65536, 128), (torch.bfloat16, 1, 65504, 32)])
+def test_rows_of_very_many_channels(dtype, rows, d_in, group):
+    """Where fewer than 16 (or 8) rows fit a pass."""
+    layer, w = _layer(d_in, 3, group, 32)
+    x = torch.randn(rows, d_in, device="cuda", generator=torch.Generator(device="cuda").manual_seed(33)).to(dtype)
+    out = torch.full((rows + 2, 3), 7.0, device="cuda", dtype=dtype)
+    y = layer.forward(x, out=out[1:-1])
+    want = x.double() @ w.t()
+    most = x.double().abs() @ w.abs().t()
+    # as in _check, with the groups' roundings counted as the 2^-24 each that they are: at most one for every 32 channels
+    tol = want.abs() * torch.finfo(dtype).eps / 2 * 1.0001 + most * ((17 + 15 * 17) * (group / 16) * 2.0 ** -23 + d_in / 32 * 2.0 ** -24)
+    assert bool(((y.double() - want).abs() <= tol).all()), float(((y.double() - want).abs() - tol).max())
+    assert bool((out[0] == 7).all()) and bool((out[-1] == 7).all())
+    assert torch.equal(layer.forward(x), y)
