@@ -499,13 +499,13 @@ bool ql_sizes_ok(int d_out, int d_in, int group) {
 // How to cut a product with `live` <= NT * 8 rows a pass: of the ways that fit, the one that should be done first.  False: none fits.
 // The estimate is in cycles of an SM and counts what was measured: a unit takes an SM the issue of its instructions (0.17 a cycle for each warp, up to 2.6), its
 // products (2.1 cycles each) or its share of HBM (24 bytes a cycle), whichever is longest, and a warp no less than its latency; a thread takes
-// 50 to 110 instructions for eight activations.  Joining a CTA's only tile takes 1200 cycles, over a cluster 2700 to 3700; each further tile,
-// for which the warps drain and fill again, 3500 and 5000 to 8000.  So a cluster of two often pays by making rounds fewer: 8 x 4096 -> 24576
-// 16.6 us against 19.3 without clusters and 22.3 with four SMs, but 1 x 1024 -> 2816 3.9 us without and 5.0 with two.
+// 38 to 110 instructions for eight activations.  Joining a CTA's only tile takes 1200 cycles, over a cluster 2700 to 3700; each further tile,
+// for which the warps drain and fill again, 3500 and 5000 to 8000.  So a cluster of two pays where it makes rounds fewer: 8 x 4096 -> 24576 f32
+// 25.3 us against 41 without clusters and 30 with four SMs, but 1 x 1024 -> 2816 4.1 us without and 5.1 with two.
 template <typename T, int NT, int GROUP>
 bool ql_plan(const QlShape& s, int rows, int live, QlPlan* out) {
   constexpr int P = QlPieces<T>::N, BYTES = ql_unit_bytes(GROUP), SM = 148;
-  constexpr double issue = (70 + 4 * (P == 1 ? 28 + 6 * NT : 48 + 18 * NT) + QL_CHANNELS / (P == 1 ? GROUP : 32) * (6 + 18 * NT));
+  constexpr double issue = (70 + 4 * (P == 1 ? 44 + 5 * NT : 48 + 18 * NT) + QL_CHANNELS / (P == 1 ? GROUP : 32) * (6 + 18 * NT));
   constexpr double products = 16 * NT * 2.1 * P;
   const int most[4] = {8, 8, 12, 16}, limit[4] = {113 * 1024, 227 * 1024, 227 * 1024, 227 * 1024}, resident[4] = {2, 1, 1, 1};
   const double first[4] = {1200, 2700, 3200, 3700}, more[4] = {3500, 5000, 6500, 8000};
@@ -540,7 +540,7 @@ bool ql_plan(const QlShape& s, int rows, int live, QlPlan* out) {
         const double hbm = BYTES / 24.0 / p.passes * std::min(1.0, (double)ctas / SM / on_sm);
         const double rate = std::min(2.6, 0.17 * p.warps * on_sm);
         const double unit = std::max(p.warps * on_sm * std::max(hbm, std::max(issue / rate, products)), std::max(350.0, 1100.0 / (p.stages - 1)));
-        const double fill = 1500 + (double)live * p.slice * 16 / 32 * (P == 1 ? 50 : 110) * on_sm / rate;
+        const double fill = 1500 + (double)live * p.slice * 16 / 32 * (P == 1 ? 38 : 110) * on_sm / rate;
         const double waves = (double)((ctas + on_sm * room - 1) / (on_sm * room));
         const double time = waves * (fill + rounds * each * unit + first[log] + (rounds - 1) * more[log]);
         if (best < 0 || time < best) { best = time; *out = p; }
