@@ -5,9 +5,11 @@
  *   y[r, n] = sum_k x[r, k] * w[n, k],    w[n, k] = scale[n, k / group] * code[n, k]
  *
  * code is -8 .. 7, scale a bf16 number, group 32, 64 or 128 input channels; d_in is a multiple of the group and at most 65536, d_out anything.
- * x and y are both f32 (MOE_PRECISION_F32) or both bf16 (MOE_PRECISION_BF16).  Products of codes and activations are exact, sums are f32,
- * y is rounded once; the order of the sums depends on the sizes only, so results do not depend on the run.  An infinity or a NaN of x
- * or of a scale appears in the outputs it takes part in.
+ * x and y are both f32 (MOE_PRECISION_F32) or both bf16 (MOE_PRECISION_BF16).  Products of codes and activations are exact, whatever the
+ * activations' sizes (below 2^-110, f32 ones lose their last bits); sums are f32, those of 16 channels on the tensor cores, which cut the terms off at
+ * about 2^-23 of the largest of them; a group's sum is scaled in f32 and y rounded once.  The order of the sums depends on the sizes only, so
+ * results do not depend on the run.  A channel whose code is 0 adds exactly 0.  An infinity or a NaN of x or of a scale appears in the outputs it takes
+ * part in (0 times an infinity is NaN).
  *
  * Meant for decode batches: 16 rows at a time (fewer where d_in is very large), more rows are passes side by side over the same weights.
  *

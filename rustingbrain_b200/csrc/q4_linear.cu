@@ -6,12 +6,12 @@
 // channels of a product may come in any order, the activations' 8 channels are one 16-byte shared load of the B operand.  Two such blocks
 // (32 outputs) and their scales are a unit, which a warp brings into its own ring in shared memory, several units ahead.
 //
-// A code plus 8 needs no conversion: bits 0 .. 7 of a bf16 are a number linear in them, bits * 2^-133 (below 128 it is subnormal, and the
-// next binade goes on in the same steps).  So a code is cut out of its word, at weight 1 or, where it comes out four bits further up, 16, and one
-// packed subtraction takes the 8 off: nine instructions for eight codes.  The activations make up for the powers of two.  Products are
-// exact, and the group's scale is applied to its f32 sum.  An f32 activation is three bf16 numbers that add up to it.
-// (Without the subtraction a group's sum has to start at -8 times the sum of its activations.  That is 12 % faster for 8 x 4096 -> 24576, the
-// same for 64 rows, and wrong: the tensor cores cut the terms of a product off at 2^-23 or so of the largest, so a channel 1e5 times as large as its
+// Bits 0 .. 7 of a bf16 are a number linear in them, bits * 2^-133 (below 128 it is subnormal, and the next binade goes on in the same
+// steps).  So a code plus 8 is cut out of its word, at weight 1 or, where it comes out four bits further up, 16, and one packed multiply-add makes
+// two of them code * 2^-6: nine instructions for eight codes.  The activations enter as they are, whatever their size; an f32 one is three
+// bf16 numbers that add up to it.  Products are exact, the group's scale is applied to its f32 sum, and infinities and NaN go their own way.
+// (The cut-out bits themselves as operands, a group's sum starting at -8 times the sum of its activations, would save four of the nine
+// instructions and is wrong: the tensor cores cut the terms of a product off at 2^-23 or so of the largest, so a channel 1e5 times as large as its
 // neighbours takes 1 % off the result even where all its codes are 0.)
 // (e4m3 operands would take three instructions for eight codes, but mma.sync has no e4m3 product of its own here: it costs two bf16 ones
 // and the conversions.)
@@ -21,9 +21,8 @@
 // are fewer tiles than SMs the CTAs of a cluster split the reduction too.  Partial sums meet in (distributed) shared memory, always in
 // the same order: one launch, no workspace.
 //
-// Measured in a graph: 1 x 1024 -> 2816 3.9 us; 8 x 4096 -> 24576 16.6 us, one row 14.8 us, 16 rows 22 us, 64 rows 61 us (the bytes: 8.25 us); f32
-// 3 x 2048 -> 32003 17.7 us (5.7 us).  What bounds the large ones is the issue of instructions, 2 a cycle and SM, and the start; 64 x 1024 ->
-// 5632, 9.9 us, brings in its activations for a quarter of that.
+// Measured in a graph: 1 x 1024 -> 2816 3.5 us; 8 x 4096 -> 24576 15.9 us, one row 14.9 us, 16 rows 19.6 us, 64 rows 61.6 us (the bytes: 8.25 us); 64 x
+// 1024 -> 5632 7.8 us; f32 3 x 2048 -> 32003 17.1 us (5.7 us).  What bounds them: see the counters in the table of measurements.
 
 #include <cooperative_groups.h>
 #include <algorithm>
@@ -40,13 +39,8 @@ namespace moe {
 namespace {
 
 constexpr int QL_MAX_WARPS = 16;
-constexpr int QL_ROWS = 16;              // batch rows per pass
-
 constexpr int QL_MAX_IN = 1 << 16;       // a row of f32 activations, cut over a cluster, fits shared memory
-constexpr int QL_RAW = 133;              // bits 0 .. 7 of a bf16 are worth bits * 2^-QL_RAW
-constexpr int QL_UP = 88, QL_DOWN = 96;  // activations times 2^QL_UP, those of a row with one above 2^38 times 2^(QL_UP - QL_DOWN)
-constexpr float QL_LARGE = 274877906944.f;
-
+constexpr int QL_CODE = 6;               // operands are codes times 2^-QL_CODE
 __host__ __device__ constexpr float ql_pow2(int e) {
   float v = 1.f;
   for (int i = 0; i < (e < 0 ? -e : e); ++i) v *= e < 0 ? 0.5f : 2.f;
@@ -151,87 +145,43 @@ __device__ __forceinline__ void ql_mma_bf16_new(float* d, uint32_t a0, uint32_t 
 __device__ __forceinline__ void ql_copy16(uint32_t smem, const void* gmem) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
 }
-// codes i and i + 4 of a word as raw bf16 numbers, of weight 16 where i is odd
+__device__ __forceinline__ __nv_bfloat162 ql_pair(uint32_t v) { return *reinterpret_cast<const __nv_bfloat162*>(&v); }
+// codes i and i + 4 of a word, times 2^-QL_CODE; exact
 template <int I>
-__device__ __forceinline__ uint32_t ql_raw(uint32_t w) { return (I < 2 ? w : w >> 8) & (I & 1 ? 0x00f000f0u : 0x000f000fu); }
-
-// ... less 8 (or 128): the codes themselves, and exactly 0 for a code of 0
-template <int I>
-__device__ __forceinline__ uint32_t ql_signed(uint32_t w) {
-  const uint32_t v = ql_raw<I>(w), eight = I & 1 ? 0x00800080u : 0x00080008u;
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&eight));
+__device__ __forceinline__ uint32_t ql_codes(uint32_t w) {
+  const uint32_t bits = (I < 2 ? w : w >> 8) & (I & 1 ? 0x00f000f0u : 0x000f000fu);      // (code + 8) * 2^-133, times 16 where I is odd
+  const __nv_bfloat162 r = __hfma2(ql_pair(bits), __float2bfloat162_rn(ql_pow2(133 - QL_CODE - (I & 1 ? 4 : 0))), __float2bfloat162_rn(-8.f * ql_pow2(-QL_CODE)));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-__device__ __forceinline__ bool ql_finite(float x) { return fabsf(x) <= 3.4028234663852886e38f; }
-// An f32 number as three bf16 numbers that add up to it, each the leading 8 bits of what is left.
-__device__ __forceinline__ void ql_split(float x, uint32_t* p) {
-  if (!ql_finite(x)) {
-    p[0] = x != x ? 0x7fc0u : __float_as_uint(x) >> 16;
-    p[1] = p[2] = 0;
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 3; ++i) {
-    const uint32_t top = __float_as_uint(x) & 0xffff0000u;
-    p[i] = top >> 16;
-    x -= __uint_as_float(top);
-  }
-}
-// Eight activations as they were loaded.  `plain` ones (finite, at most QL_LARGE) become operands here: times 2^QL_UP, and 2^-4 less where the
-// code weighs 16.
+// Eight activations as they are loaded, and as operands.
 template <typename T> constexpr int QL_BATCH = sizeof(T) == 2 ? 4 : 2;
 template <typename T> struct QlRaw;
 template <> struct QlRaw<bf16> {
   struct type { uint4 v; };
   static __device__ __forceinline__ type load(const bf16* p) { return {__ldg(reinterpret_cast<const uint4*>(p))}; }
-  static __device__ __forceinline__ void widen(const type& a, float* f) {
-    const uint32_t w[4] = {a.v.x, a.v.y, a.v.z, a.v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[2 * i] = __uint_as_float(w[i] << 16);
-      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-  }
-  static __device__ __forceinline__ __nv_bfloat162 pair(uint32_t v) { return *reinterpret_cast<const __nv_bfloat162*>(&v); }
-  static __device__ __forceinline__ uint32_t times(uint32_t v, float by) {
-    const __nv_bfloat162 r = __hmul2(pair(v), __float2bfloat162_rn(by));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
-  static __device__ __forceinline__ bool plain(const type& a) {
-    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(__habs2(pair(a.v.x)), __habs2(pair(a.v.y))), __hmax2_nan(__habs2(pair(a.v.z)), __habs2(pair(a.v.w))));
-    return __low2float(m) <= QL_LARGE && __high2float(m) <= QL_LARGE;
-  }
-  static __device__ __forceinline__ void plain_pieces(const type& a, uint4* out) {
-    out[0] = make_uint4(times(a.v.x, ql_pow2(QL_UP)), times(a.v.y, ql_pow2(QL_UP - 4)), times(a.v.z, ql_pow2(QL_UP)), times(a.v.w, ql_pow2(QL_UP - 4)));
-  }
+  static __device__ __forceinline__ void pieces(const type& a, uint4* out) { out[0] = a.v; }
 };
 template <> struct QlRaw<float> {
   struct type { float4 a, b; };
   static __device__ __forceinline__ type load(const float* p) { return {__ldg(reinterpret_cast<const float4*>(p)), __ldg(reinterpret_cast<const float4*>(p) + 1)}; }
-  static __device__ __forceinline__ void widen(const type& t, float* f) {
-    *reinterpret_cast<float4*>(f) = t.a;
-    *reinterpret_cast<float4*>(f + 4) = t.b;
-  }
-  static __device__ __forceinline__ bool plain(const type& t) {
-    float f[8];
-    widen(t, f);
-    bool ok = true;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) ok &= fabsf(f[j]) <= QL_LARGE;
-    return ok;
-  }
-  static __device__ __forceinline__ void plain_pieces(const type& t, uint4* out) {
+  // three bf16 numbers that add up to each, the leading 8 bits of what is left; an infinity or a NaN is one alone
+  static __device__ __forceinline__ void pieces(const type& t, uint4* out) {
     float f[8];
     uint32_t p[8][3];
-    widen(t, f);
+    *reinterpret_cast<float4*>(f) = t.a;
+    *reinterpret_cast<float4*>(f + 4) = t.b;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      float v = f[j] * ql_pow2(j & 2 ? QL_UP - 4 : QL_UP);
+      float v = f[j];
 #pragma unroll
       for (int q = 0; q < 3; ++q) {
         p[j][q] = __float_as_uint(v) & 0xffff0000u;
         v -= __uint_as_float(p[j][q]);
+      }
+      if (!(fabsf(f[j]) <= 3.4028234663852886e38f)) {
+        p[j][0] = f[j] != f[j] ? 0x7fc00000u : __float_as_uint(f[j]);
+        p[j][1] = p[j][2] = 0;
       }
     }
 #pragma unroll
@@ -243,15 +193,14 @@ template <> struct QlRaw<float> {
 template <typename T> struct QlPieces { static constexpr int N = 1; };
 template <> struct QlPieces<float> { static constexpr int N = 3; };
 
-// How a launch cuts the product, and where things lie in shared memory: marks of the rows first; then the activations [piece][row][2 bytes a channel, and 64 that keep the 16-byte loads of a warp off each
-// other's banks]; the warps' rings; the partial sums [buffer][wk][row][outputs of the tile] f32.
+// How a launch cuts the product, and where things lie in shared memory: the activations [piece][row][2 bytes a channel, and 64 that keep
+// the 16-byte loads of a warp off each other's banks]; the warps' rings; the partial sums [buffer][wk][row][outputs of the tile] f32.
 struct QlPlan {
   int warps, wk, cluster;              // warps of a CTA, those of them along the reduction; CTAs along it
   int tiles, passes, clusters;         // tiles of outputs; passes over the rows; clusters that share the tiles of a pass
   int slice, per_pass, stages, buffers;   // units of the reduction per CTA, at most; rows per pass; units in a ring; buffers of partial sums
-  int acts, rings, sums, bytes;
+  int rings, sums, bytes;
 };
-constexpr int QL_FRONT = 2 * QL_ROWS * 4;
 
 // grid: (clusters * passes) * cluster, the passes over the same tiles next to each other
 template <typename T, int NT, int GROUP>
@@ -268,9 +217,7 @@ q4_linear_kernel(const T* __restrict__ x, long long ld_x, const unsigned char* _
   const int ubeg = (int)((long long)s.units * rank / cluster), uend = (int)((long long)s.units * (rank + 1) / cluster);
   const int k0 = ubeg * QL_CHANNELS, channels = (uend - ubeg) * QL_CHANNELS;
   const int pitch = plan.slice * QL_CHANNELS * 2 + 64, plane = rows * pitch;
-  int* mark = reinterpret_cast<int*>(ql_sm);                      // by row: one above QL_LARGE is there
-  int* odd = mark + QL_ROWS;                                      // something infinite or NaN is there
-  unsigned char* acts = ql_sm + plan.acts;
+  unsigned char* acts = ql_sm;
 
   // ---- the warp's units: of the tiles tile0, tile0 + clusters, .. those from ubeg + wk on in steps of wk_count ----
   const int first = ubeg + wk;
@@ -302,57 +249,29 @@ q4_linear_kernel(const T* __restrict__ x, long long ld_x, const unsigned char* _
 
   // ---- the activations of the slice, eight channels of a row at a time, several loads of a thread in flight ----
   const int parts = channels / 8, work = rows * parts, row_step = threads / parts, part_step = threads - row_step * parts;
-  if (threadIdx.x < 2 * QL_ROWS) mark[threadIdx.x] = 0;
-  __syncthreads();
-  int again = 0;
-  for (bool large = true; large; ++again) {
-    large = false;
-    int r = threadIdx.x / parts, c = threadIdx.x - r * parts;
-    for (int i0 = warp * 32; i0 < work; i0 += QL_BATCH<T> * threads) {
-      typename QlRaw<T>::type raw[QL_BATCH<T>];
-      int rb[QL_BATCH<T>], cb[QL_BATCH<T>];
+  int r = threadIdx.x / parts, c = threadIdx.x - r * parts;
+  for (int i0 = threadIdx.x; i0 < work; i0 += QL_BATCH<T> * threads) {
+    typename QlRaw<T>::type raw[QL_BATCH<T>];
+    int to[QL_BATCH<T>];
 #pragma unroll
-      for (int u = 0; u < QL_BATCH<T>; ++u) {
-        rb[u] = min(r, rows - 1);
-        cb[u] = c * 8;
-        raw[u] = {};
-        if (i0 + u * threads + lane < work && k0 + c * 8 < s.d_in) raw[u] = QlRaw<T>::load(x + (row0 + r) * ld_x + k0 + c * 8);
-        r += row_step;
-        c += part_step;
-        if (c >= parts) { c -= parts; ++r; }
-      }
-#pragma unroll
-      for (int u = 0; u < QL_BATCH<T>; ++u) {
-        if (i0 + u * threads >= work) break;                      // the same for the whole warp
-        const int row = rb[u];
-        uint4 out[P];
-        if (QlRaw<T>::plain(raw[u]) && !(again && mark[row])) {
-          QlRaw<T>::plain_pieces(raw[u], out);
-        } else {
-          // something large, infinite or NaN
-          const float by = again && mark[row] ? ql_pow2(QL_UP - QL_DOWN) : ql_pow2(QL_UP);
-          float f[8];
-          uint32_t p[8][3];
-          QlRaw<T>::widen(raw[u], f);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            if (!ql_finite(f[j])) { odd[row] = 1; f[j] = 0.f; }
-            if (!again && fabsf(f[j]) > QL_LARGE) { mark[row] = 1; large = true; }
-            f[j] *= by;
-            ql_split(f[j] * (j & 2 ? 0.0625f : 1.f), p[j]);
-          }
-#pragma unroll
-          for (int q = 0; q < P; ++q) out[q] = make_uint4(p[0][q] | p[1][q] << 16, p[2][q] | p[3][q] << 16, p[4][q] | p[5][q] << 16, p[6][q] | p[7][q] << 16);
-        }
-        if (i0 + u * threads + lane >= work) continue;
-#pragma unroll
-        for (int q = 0; q < P; ++q) *reinterpret_cast<uint4*>(acts + q * plane + row * pitch + cb[u] * 2) = out[q];
-      }
+    for (int u = 0; u < QL_BATCH<T>; ++u) {
+      to[u] = r * pitch + c * 16;
+      raw[u] = {};                                                // zeros behind the last channel
+      if (i0 + u * threads < work && k0 + c * 8 < s.d_in) raw[u] = QlRaw<T>::load(x + (row0 + r) * ld_x + k0 + c * 8);
+      r += row_step;
+      c += part_step;
+      if (c >= parts) { c -= parts; ++r; }
     }
-    large = __syncthreads_or(large && !again);
+#pragma unroll
+    for (int u = 0; u < QL_BATCH<T>; ++u) {
+      if (i0 + u * threads >= work) break;
+      uint4 out[P];
+      QlRaw<T>::pieces(raw[u], out);
+#pragma unroll
+      for (int q = 0; q < P; ++q) *reinterpret_cast<uint4*>(acts + q * plane + to[u]) = out[q];
+    }
   }
-  bool any_odd = false;
-  for (int r = 0; r < rows; ++r) any_odd |= odd[r] != 0;
+  __syncthreads();
 
   const unsigned char* mine[NT];                                  // rows past the last one repeat it; nobody looks at their sums
 #pragma unroll
@@ -408,8 +327,8 @@ q4_linear_kernel(const T* __restrict__ x, long long ld_x, const unsigned char* _
 #pragma unroll
           for (int m = 0; m < 2; ++m) {
             const uint32_t lo = g ? w[m].z : w[m].x, hi = g ? w[m].w : w[m].y;
-            a[m][0] = ql_signed<0>(lo); a[m][1] = ql_signed<0>(hi); a[m][2] = ql_signed<1>(lo); a[m][3] = ql_signed<1>(hi);
-            a[m][4] = ql_signed<2>(lo); a[m][5] = ql_signed<2>(hi); a[m][6] = ql_signed<3>(lo); a[m][7] = ql_signed<3>(hi);
+            a[m][0] = ql_codes<0>(lo); a[m][1] = ql_codes<0>(hi); a[m][2] = ql_codes<1>(lo); a[m][3] = ql_codes<1>(hi);
+            a[m][4] = ql_codes<2>(lo); a[m][5] = ql_codes<2>(hi); a[m][6] = ql_codes<3>(lo); a[m][7] = ql_codes<3>(hi);
           }
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
@@ -437,29 +356,14 @@ q4_linear_kernel(const T* __restrict__ x, long long ld_x, const unsigned char* _
       for (int e = 0; e < 2; ++e) {
         const int r = n * 8 + 2 * tig + e;
         if (r >= rows) continue;
-        const float by = mark[r] ? ql_pow2(QL_DOWN) : 1.f;
         float* dst = red + (wk * rows + r) * width + wn * 32 + gid;
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-          dst[16 * m] = acc[m][n][e] * ql_pow2(QL_RAW - QL_UP) * by;
-          dst[16 * m + 8] = acc[m][n][2 + e] * ql_pow2(QL_RAW - QL_UP) * by;
+          dst[16 * m] = acc[m][n][e] * ql_pow2(QL_CODE);
+          dst[16 * m + 8] = acc[m][n][2 + e] * ql_pow2(QL_CODE);
         }
       }
     const int n0 = tile * width;
-    if (any_odd) {
-      // infinities and NaN took part as 0 above (cut into pieces an infinity would be NaN): add what they really give
-      __syncthreads();
-      for (int i = threadIdx.x; i < rows * width; i += threads) {
-        const int r = i / width, n = n0 + i % width;
-        if (!odd[r] || n >= s.d_out) continue;
-        float v = 0.f;
-        for (int k = k0; k < min(k0 + channels, s.d_in); ++k) {
-          const float f = to_f32<T>(x[(row0 + r) * ld_x + k]);
-          if (!ql_finite(f)) v += f * ql_weight(packed, s, n, k);
-        }
-        red[i] += v;
-      }
-    }
     if (cluster > 1) cl.sync(); else __syncthreads();
     const int count = cluster * wk_count;
     for (int i = rank * threads + threadIdx.x; i < rows * width / 4; i += cluster * threads) {
@@ -499,9 +403,9 @@ bool ql_sizes_ok(int d_out, int d_in, int group) {
 // How to cut a product with `live` <= NT * 8 rows a pass: of the ways that fit, the one that should be done first.  False: none fits.
 // The estimate is in cycles of an SM and counts what was measured: a unit takes an SM the issue of its instructions (0.17 a cycle for each warp, up to 2.6), its
 // products (2.1 cycles each) or its share of HBM (24 bytes a cycle), whichever is longest, and a warp no less than its latency; a thread takes
-// 38 to 110 instructions for eight activations.  Joining a CTA's only tile takes 1200 cycles, over a cluster 2700 to 3700; each further tile,
+// 20 to 100 instructions for eight activations.  Joining a CTA's only tile takes 1200 cycles, over a cluster 2700 to 3700; each further tile,
 // for which the warps drain and fill again, 3500 and 5000 to 8000.  So a cluster of two pays where it makes rounds fewer: 8 x 4096 -> 24576 f32
-// 25.3 us against 41 without clusters and 30 with four SMs, but 1 x 1024 -> 2816 4.1 us without and 5.1 with two.
+// 25.1 us against 40 without clusters and 29 with four SMs, but 1 x 1024 -> 2816 3.5 us without and 4.6 with two.
 template <typename T, int NT, int GROUP>
 bool ql_plan(const QlShape& s, int rows, int live, QlPlan* out) {
   constexpr int P = QlPieces<T>::N, BYTES = ql_unit_bytes(GROUP), SM = 148;
@@ -521,8 +425,7 @@ bool ql_plan(const QlShape& s, int rows, int live, QlPlan* out) {
       p.warps = most[way];
       p.slice = (s.units + p.cluster - 1) / p.cluster;
       if (p.cluster > 1 && s.units < 2 * p.cluster) break;
-      p.acts = QL_FRONT;
-      p.rings = p.acts + up(P * live * (p.slice * QL_CHANNELS * 2 + 64));
+      p.rings = up(P * live * (p.slice * QL_CHANNELS * 2 + 64));
       const int sums = live * 32 * p.warps * 4;
       bool fits = false;
       for (p.stages = 4; p.stages >= 2 && !fits; p.stages -= !fits)
@@ -540,7 +443,7 @@ bool ql_plan(const QlShape& s, int rows, int live, QlPlan* out) {
         const double hbm = BYTES / 24.0 / p.passes * std::min(1.0, (double)ctas / SM / on_sm);
         const double rate = std::min(2.6, 0.17 * p.warps * on_sm);
         const double unit = std::max(p.warps * on_sm * std::max(hbm, std::max(issue / rate, products)), std::max(350.0, 1100.0 / (p.stages - 1)));
-        const double fill = 1500 + (double)live * p.slice * 16 / 32 * (P == 1 ? 38 : 110) * on_sm / rate;
+        const double fill = 1500 + (double)live * p.slice * 16 / 32 * (P == 1 ? 20 : 100) * on_sm / rate;
         const double waves = (double)((ctas + on_sm * room - 1) / (on_sm * room));
         const double time = waves * (fill + rounds * each * unit + first[log] + (rounds - 1) * more[log]);
         if (best < 0 || time < best) { best = time; *out = p; }

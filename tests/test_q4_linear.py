@@ -245,3 +245,25 @@ def test_rows_of_very_many_channels(dtype, rows, d_in, group):
     assert bool(((y.double() - want).abs() <= tol).all()), float(((y.double() - want).abs() - tol).max())
     assert bool((out[0] == 7).all()) and bool((out[-1] == 7).all())
     assert torch.equal(layer.forward(x), y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,d_in", [(4, 256), (20, 1024)])
+def test_a_huge_channel_that_no_weight_takes_leaves_the_others_alone(dtype, rows, d_in):
+    """Activations of 2^39 to 2^126 in a group whose scales are 0, beside others of 2^-6: the row's result is that of the others."""
+    from rustingbrain_b200.q4_linear import Q4Linear
+    g = torch.Generator(device="cuda").manual_seed(30)
+    codes = torch.randint(-8, 8, (96, d_in), device="cuda", generator=g).to(torch.int8)
+    scales = (torch.rand(96, d_in // 32, device="cuda", generator=g) + 0.1).bfloat16()
+    scales[:, 1] = 0
+    layer = Q4Linear(d_in, 96, group_size=32)
+    layer.set_codes(codes, scales)
+    w = codes.double() * scales.double().repeat_interleave(32, dim=1)
+    x = (torch.randn(rows, d_in, device="cuda", generator=g) * 2.0 ** -6).to(dtype)
+    clean = layer.forward(x)
+    for r, e in enumerate((38, 39, 60, 126)):
+        x[r, 32 + 7 * r] = 1.5 * 2.0 ** e
+    y = layer.forward(x)
+    _check(y, x, w)
+    assert torch.equal(y[4:], clean[4:])
