@@ -87,7 +87,8 @@ class KvCache:
     def forward_cached(self, q, k, v, rows_per_sequence: int = 1, first_sequence: int = 0,
                        n_sequences: Optional[int] = None, out=None, stream=None):
         """Device tensors q [rows, num_heads * head_dim] (scratch: may be rotated in place), k and v
-        [rows, kv_heads * head_dim], rows = n_sequences * rows_per_sequence; returns the merged heads."""
+        [rows, kv_heads * head_dim], rows = n_sequences * rows_per_sequence; returns the merged heads, in ``out`` (of any shape with as many values, q itself too)
+        where it is given."""
         n_seq = self.sequences - first_sequence if n_sequences is None else n_sequences
         rows = n_seq * rows_per_sequence
         W = self.kv_heads * self.head_dim
@@ -96,8 +97,8 @@ class KvCache:
         self._rows(v, rows, W, "v")
         if out is None:
             out = q.new_empty(q.shape)
-        else:
-            self._rows(out, rows, self.num_heads * self.head_dim, "out")
+        elif not (out.get_device() == self.device and out.is_contiguous() and out.dtype == self._dtype and out.numel() == q.numel()):
+            raise InvalidInput("out must be a contiguous %s tensor of %d values on cuda:%d" % (self._dtype, q.numel(), self.device))
         self._check(self._forward(self._h, first_sequence, n_seq, q.data_ptr(), k.data_ptr(), v.data_ptr(), rows_per_sequence,
                                   out.data_ptr(), self._on(stream)))
         return out

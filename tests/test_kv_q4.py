@@ -496,3 +496,21 @@ def test_rollback_of_steps_that_a_marked_cache_skips(precision):
     with pytest.raises(InvalidInput, match="SequenceTooLong"):
         cache.lengths()
     assert cache.lengths() == [5]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("precision", ["q4", "bf16", "f32"])
+def test_out_has_any_shape(precision):
+    H, Hkv, hd, S, rows = 4, 2, 64, 3, 2
+    dt = torch.float32 if precision == "f32" else torch.bfloat16
+    caches = [KvCache(S, H, Hkv, hd, 16, precision=precision) for _ in range(2)]
+    q, k, v = (torch.from_numpy(a).cuda().to(dt) for a in _rows(S * rows, H, Hkv, hd, 90))
+    want = caches[0].forward_cached(q.clone(), k, v, rows_per_sequence=rows)
+    out = torch.empty(S, rows, H, hd, device="cuda", dtype=dt)
+    got = caches[1].forward_cached(q.clone(), k, v, rows_per_sequence=rows, out=out)
+    assert got is out and torch.equal(out.view(S * rows, H * hd), want)
+    for bad in (torch.empty(S * rows, H * hd + 1, device="cuda", dtype=dt), torch.empty(S * rows, H * hd, dtype=dt), torch.empty(S, H, rows, hd, device="cuda", dtype=dt).transpose(1, 2),
+                torch.empty(S * rows, H * hd, device="cuda", dtype=torch.float64)):
+        with pytest.raises(InvalidInput):
+            caches[0].forward_cached(q, k, v, rows_per_sequence=rows, out=bad)
+    assert caches[0].lengths() == [rows] * S
