@@ -1,7 +1,12 @@
 """How the stateless calls of the C ABI are issued for torch tensors: on the tensors' device and, unless a stream is given, on
-that device's current stream."""
+that device's current stream.
+
+A stream is given by its number.  What the call reads has to be there for that stream, which is the caller's to see to; what the call returns
+is that stream's memory, as if it had been the current one.
+"""
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import threading
 
@@ -14,6 +19,18 @@ class _Local(threading.local):
 
 _local = _Local()
 _calls = None                                # torch's current device and current stream, looked up once
+
+
+_no_change = contextlib.nullcontext()
+
+
+def memory_of(stream, device):
+    """Inside it, torch allocates for the given stream (None: for the current one, as always): memory that is let go before the stream has
+    written it is then not given out elsewhere."""
+    if stream is None:
+        return _no_change
+    import torch
+    return torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=device))
 
 
 def issue(fn, tensor, stream, errors, default_error, *args) -> None:

@@ -12,6 +12,7 @@ from typing import List, Optional
 import numpy as np
 
 from . import _lib
+from ._torch import memory_of
 from .moe import CudaError, InvalidConfig, InvalidInput, NetworkError, _stream
 
 _ERRORS = {_lib.INVALID_CONFIG: InvalidConfig, _lib.INVALID_INPUT: InvalidInput, _lib.UNSUPPORTED: InvalidConfig}
@@ -96,7 +97,8 @@ class KvCache:
         self._rows(k, rows, W, "k")
         self._rows(v, rows, W, "v")
         if out is None:
-            out = q.new_empty(q.shape)
+            with memory_of(stream, q.device):
+                out = q.new_empty(q.shape)
         elif not (out.get_device() == self.device and out.is_contiguous() and out.dtype == self._dtype and out.numel() == q.numel()):
             raise InvalidInput("out must be a contiguous %s tensor of %d values on cuda:%d" % (self._dtype, q.numel(), self.device))
         self._check(self._forward(self._h, first_sequence, n_seq, q.data_ptr(), k.data_ptr(), v.data_ptr(), rows_per_sequence,
@@ -138,7 +140,8 @@ class KvCache:
         if self._f32 is None:
             import torch
             self._f32 = torch.empty(0, dtype=torch.float32, device=self.device)
-        keys, values = self._f32.new_empty(shape), self._f32.new_empty(shape)
+        with memory_of(stream, self._f32.device):
+            keys, values = self._f32.new_empty(shape), self._f32.new_empty(shape)
         self._check(_lib.lib().kv_cache_newest(self._h, first_sequence, n_seq, rows_per_sequence, keys.data_ptr(), values.data_ptr(), self._on(stream)))
         return keys, values
 

@@ -8,7 +8,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 from . import _lib
-from ._torch import issue
+from ._torch import issue, memory_of
 from .moe import CudaError, InvalidConfig, InvalidInput
 
 MAX_TOP = 32
@@ -58,12 +58,13 @@ def token_logprobs(logits, targets=None, top: int = 0, stream=None) -> TokenLogP
     t = _check_row(targets, rows, torch.int32, logits, "targets")
     if not 0 <= top <= min(vocab, MAX_TOP):
         raise InvalidInput("top is 0 .. %d, got %d" % (min(vocab, MAX_TOP), top))
-    lp = logits.new_empty(rows, dtype=torch.float32)
-    h, lse = torch.empty_like(lp), torch.empty_like(lp)
     ids = tlp = None
-    if top:
-        ids = logits.new_empty((rows, top), dtype=torch.int32)
-        tlp = lp.new_empty((rows, top))
+    with memory_of(stream, logits.device):
+        lp = logits.new_empty(rows, dtype=torch.float32)
+        h, lse = torch.empty_like(lp), torch.empty_like(lp)
+        if top:
+            ids = logits.new_empty((rows, top), dtype=torch.int32)
+            tlp = lp.new_empty((rows, top))
     issue(_lib.lib().logprobs_forward, logits, stream, _ERRORS, CudaError, logits.data_ptr(), stride, t, rows, vocab, top, precision,
           lp.data_ptr(), h.data_ptr(), lse.data_ptr(), tlp.data_ptr() if top else None, ids.data_ptr() if top else None)
     return TokenLogProbs(lp, h, lse, ids, tlp)
@@ -75,7 +76,8 @@ def token_logprobs_backward(logits, targets, lse, entropy=None, grad_logprob=Non
     import torch
     rows, vocab, stride, precision = _check_logits(logits, "logits")
     if out is None:
-        out, out_stride = logits.new_empty((rows, vocab)), vocab
+        with memory_of(stream, logits.device):
+            out, out_stride = logits.new_empty((rows, vocab)), vocab
     elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
         raise InvalidInput("out must match the logits")
     else:

@@ -7,14 +7,17 @@ puts around a ``KvCache`` and for an output head.
 from __future__ import annotations
 
 from . import _lib
-from ._torch import issue
+from ._torch import issue, memory_of
 from .moe import CudaError, InvalidConfig, InvalidInput
 
 _ERRORS = {_lib.INVALID_CONFIG: InvalidConfig, _lib.INVALID_INPUT: InvalidInput, _lib.UNSUPPORTED: InvalidConfig}
 
 
 class Q4Linear:
-    """``Linear::new(d_in, d_out)`` without a bias; weights start at zero and come from ``set_weight`` (quantised here) or ``set_codes``."""
+    """``Linear::new(d_in, d_out)`` without a bias; weights start at zero and come from ``set_weight`` (quantised here) or ``set_codes``.
+
+    Every call takes a ``stream`` (its number; None: the current one).  The caller orders calls that set weights against those that read them, and
+    what a call reads against its stream."""
 
     def __init__(self, d_in: int, d_out: int, group_size: int = 32, device: int = 0):
         import torch
@@ -24,6 +27,8 @@ class Q4Linear:
             raise InvalidConfig("d_in (%d) is a multiple of the group (%d), which is 32, 64 or 128, and d_out (%d) is positive"
                                 % (d_in, group_size, d_out))
         self.packed = torch.zeros(size, dtype=torch.uint8, device="cuda:%d" % device)      # zero scales: a layer of zeros
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(device).synchronize()    # the zeros are there before weights of any stream
         self._dtypes = {torch.bfloat16: _lib.PRECISION_BF16, torch.float32: _lib.PRECISION_F32}
         self._fn = _lib.lib().q4_linear_forward
         self._at, self._index = self.packed.data_ptr(), self.packed.get_device()
@@ -49,7 +54,8 @@ class Q4Linear:
     def weight(self, stream=None):
         """What the layer stands for: f32 [d_out, d_in]."""
         import torch
-        w = torch.empty((self.d_out, self.d_in), dtype=torch.float32, device=self.packed.device)
+        with memory_of(stream, self.packed.device):
+            w = torch.empty((self.d_out, self.d_in), dtype=torch.float32, device=self.packed.device)
         issue(_lib.lib().q4_linear_dequantize, self.packed, stream, _ERRORS, CudaError, self._at, w.data_ptr(), self.d_out, self.d_in, self.group_size)
         return w
 
@@ -60,7 +66,8 @@ class Q4Linear:
             raise InvalidInput("expected a f32 or bf16 tensor [rows, %d] on %s, the channels of a row adjacent" % (self.d_in, self.packed.device))
         rows = shape[0]
         if out is None:
-            out = x.new_empty((rows, self.d_out))
+            with memory_of(stream, x.device):
+                out = x.new_empty((rows, self.d_out))
         elif tuple(out.shape) != (rows, self.d_out) or out.dtype != x.dtype or out.device != x.device or (self.d_out > 1 and out.stride(1) != 1):
             raise InvalidInput("out must be [%d, %d], of x's type and on its device" % (rows, self.d_out))
         issue(self._fn, x, stream, _ERRORS, CudaError, x.data_ptr(), x.stride(0) if rows > 1 else self.d_in, self._at, out.data_ptr(),

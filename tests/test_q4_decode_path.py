@@ -295,3 +295,65 @@ def test_inputs_that_come_from_another_stream():
     for _ in range(3):
         graph.replay()
         check()
+
+
+def _busy():
+    torch.cuda._sleep(100_000_000)               # about 50 ms of the current stream
+
+
+@pytest.mark.gpu
+def test_weights_set_on_a_stream_of_their_own():
+    """The zeros that a new layer starts with do not land on top of weights that another stream has packed."""
+    g = torch.Generator(device="cuda").manual_seed(40)
+    codes = torch.randint(-8, 8, (64, 128), device="cuda", generator=g).to(torch.int8)
+    scales = torch.rand(64, 4, device="cuda", generator=g).bfloat16()
+    weight = torch.randn(64, 128, device="cuda", generator=g)
+    want = codes.float() * scales.float().repeat_interleave(32, dim=1)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for set_it in (lambda l: l.set_codes(codes, scales, stream=side.cuda_stream), lambda l: l.set_weight(weight, stream=side.cuda_stream)):
+        _busy()
+        layer = Q4Linear(128, 64)
+        set_it(layer)
+        torch.cuda.synchronize()
+        assert float(layer.weight().abs().max()) > 0
+    _busy()
+    layer = Q4Linear(128, 64)
+    layer.set_codes(codes, scales, stream=side.cuda_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(layer.weight(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["linear", "weight", "logprobs", "gradient", "step", "newest"])
+def test_results_of_a_given_stream_are_its_own_memory(what):
+    """A result that is dropped before its stream has written it is not handed out on another stream meanwhile."""
+    side = torch.cuda.Stream()
+    layer = Q4Linear(128, 4096)
+    layer.set_weight(torch.ones(4096, 128, device="cuda"))
+    x = torch.ones(64, 128, device="cuda")
+    logits, lse = torch.ones(64, 4096, device="cuda"), torch.ones(64, device="cuda")
+    cache = KvCache(64, 16, 16, 128, capacity=4, precision="bf16")
+    qkv = [torch.ones(64, 2048, device="cuda").bfloat16() for _ in range(3)]
+    cache.append(qkv[1], qkv[2])
+    st = side.cuda_stream
+    call = {"linear": lambda: [layer.forward(x, stream=st)], "weight": lambda: [layer.weight(stream=st)],
+            "logprobs": lambda: [t for t in token_logprobs(logits, None, top=32, stream=st)],
+            "gradient": lambda: [token_logprobs_backward(logits, None, lse, grad_logprob=lse, stream=st)],
+            "step": lambda: [cache.forward_cached(*qkv, stream=st)], "newest": lambda: list(cache.newest(stream=st))}[what]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        _busy()
+    got = call()
+    shapes = [(t.shape, t.dtype) for t in got]
+    del got
+    mine = [torch.full(s, 7, device="cuda", dtype=d) for s, d in shapes]
+    torch.cuda.synchronize()
+    assert all(bool((t == 7).all()) for t in mine)
+    with torch.cuda.stream(side):                              # ... and the default stream, given by its number
+        again = call()
+    torch.cuda.synchronize()
+    st = 0
+    if what != "step":
+        for a, b in zip(again, call()):
+            assert torch.equal(a.nan_to_num(), b.nan_to_num())
