@@ -13,7 +13,7 @@ import numpy as np
 
 from . import _lib
 from ._torch import memory_of
-from .moe import CudaError, InvalidConfig, InvalidInput, NetworkError, _stream
+from .moe import CudaError, InvalidConfig, InvalidInput, NetworkError
 
 _ERRORS = {_lib.INVALID_CONFIG: InvalidConfig, _lib.INVALID_INPUT: InvalidInput, _lib.UNSUPPORTED: InvalidConfig}
 _PRECISIONS = {"f32": _lib.PRECISION_F32, "bf16": _lib.PRECISION_BF16, "q4": _lib.PRECISION_Q4}
@@ -24,7 +24,10 @@ class KvCache:
     RoPE tables for ``max_seq_len`` positions (Rope::new, rope.rs:71-97).
 
     ``precision`` is the type of the activations and of the cache, "f32" or "bf16"; "q4" keeps the cache in 4 bits with a step and a base
-    per 32 channels of a head (bf16 activations, head_dim 32, 64, 128 or 256): a third of the bytes of a bf16 cache."""
+    per 32 channels of a head (bf16 activations, head_dim 32, 64, 128 or 256): a third of the bytes of a bf16 cache.
+
+    Every call takes a ``stream`` (its number; None: the current one of the cache's device).  Calls on one cache follow one another, on one stream or
+    ordered by the caller."""
 
     def __init__(self, sequences: int, num_heads: int, kv_heads: int, head_dim: int, capacity: int,
                  max_seq_len: Optional[int] = None, rope_base: float = 10000.0, rope: bool = True,
@@ -65,14 +68,14 @@ class KvCache:
     def lengths(self, stream=None) -> List[int]:
         """``KvCache::len`` of every sequence."""
         out = (C.c_int32 * self.sequences)()
-        self._check(_lib.lib().kv_cache_lengths(self._h, out, _stream(stream)))
+        self._check(_lib.lib().kv_cache_lengths(self._h, out, self._on(stream)))
         return list(out)
 
     def clear(self, sequence: int = -1, stream=None) -> None:
-        self._check(_lib.lib().kv_cache_clear(self._h, sequence, _stream(stream)))
+        self._check(_lib.lib().kv_cache_clear(self._h, sequence, self._on(stream)))
 
     def truncate(self, length: int, sequence: int = -1, stream=None) -> None:
-        self._check(_lib.lib().kv_cache_truncate(self._h, sequence, length, _stream(stream)))
+        self._check(_lib.lib().kv_cache_truncate(self._h, sequence, length, self._on(stream)))
 
     def keys_values(self, sequence: int, stream=None):
         """Cached (post-RoPE) keys and values of one sequence as f32 [len, kv_heads * head_dim]."""
@@ -81,7 +84,7 @@ class KvCache:
         k = np.empty((n, W), np.float32)
         v = np.empty((n, W), np.float32)
         fp = C.POINTER(C.c_float)
-        self._check(_lib.lib().kv_cache_read(self._h, sequence, k.ctypes.data_as(fp), v.ctypes.data_as(fp), _stream(stream)))
+        self._check(_lib.lib().kv_cache_read(self._h, sequence, k.ctypes.data_as(fp), v.ctypes.data_as(fp), self._on(stream)))
         return k, v
 
     # -- forward_cached -----------------------------------------------------------------------------
@@ -116,6 +119,7 @@ class KvCache:
         """The given stream, or the current one of the cache's device."""
         if self._raw_stream is None:
             import torch
+            torch.cuda.init()                                  # a cache can be the first thing on the device
             self._raw_stream = torch._C._cuda_getCurrentRawStream
         return self._raw_stream(self.device) if stream is None else int(stream)
 

@@ -357,3 +357,27 @@ def test_results_of_a_given_stream_are_its_own_memory(what):
     if what != "step":
         for a, b in zip(again, call()):
             assert torch.equal(a.nan_to_num(), b.nan_to_num())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("precision", ["q4", "bf16", "f32"])
+def test_a_cache_is_cut_read_and_cleared_in_the_order_of_its_stream(precision):
+    dt = torch.float32 if precision == "f32" else torch.bfloat16
+    cache = KvCache(2, 2, 1, 64, capacity=40, precision=precision)
+    k = torch.ones(20, 64, device="cuda", dtype=dt)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        _busy()
+        cache.append(k, k, rows_per_sequence=10)
+        cache.truncate(7, sequence=0)
+        assert cache.lengths() == [7, 10]
+        _busy()
+        cache.append(k, k, rows_per_sequence=10)
+        values = cache.keys_values(1)[1]
+        assert values.shape == (20, 64) and (values == 1).all()
+        _busy()
+        cache.append(k[:2], k[:2])
+        cache.clear(1)
+    side.synchronize()
+    assert cache.lengths() == [18, 0]
