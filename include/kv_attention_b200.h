@@ -74,7 +74,8 @@ int32_t kv_cache_lengths(kv_cache_t* cache, int32_t* lengths_host, void* stream)
  * rows of one sequence adjacent (row = j * rows_per_sequence + i for the j-th sequence of the range);
  * row i of a sequence sits at position len + i and sees positions 0 ..= len + i.  q, k and v are the
  * projections BEFORE rotation (`project`, attention.rs:920-944, rotates queries and keys; here the call
- * does).  q is scratch: one kernel path rotates it in place, the other rotates in registers and leaves it
+ * does).  q starts on a 16-byte boundary (InvalidInput where a kernel would load across one; a 4-bit cache takes any).
+ * q is scratch: one kernel path rotates it in place, the other rotates in registers and leaves it
  * alone, so its contents after the call are unspecified; k and v are read only.
  * merged [rows, num_heads * head_dim] is the input of the output projection; it may be q itself and overlaps nothing else.
  * SequenceTooLong -> MOE_INVALID_INPUT when a cache would pass its capacity (rope.rs:194-200); nothing

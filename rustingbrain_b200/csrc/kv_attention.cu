@@ -634,7 +634,7 @@ int kv_fail(kv_cache* c, int code, const char* fmt, ...) {
     if (e_ != cudaSuccess) return kv_fail(c, MOE_CUDA_ERROR, "%s failed: %s", #call, cudaGetErrorString(e_)); \
   } while (0)
 
-size_t elem_size(const kv_cache* c) { return c->cfg.precision == MOE_PRECISION_BF16 ? 2 : 4; }
+size_t elem_size(const kv_cache* c) { return c->cfg.precision == MOE_PRECISION_F32 ? 4 : 2; }   // of the activations, and of the older caches
 
 bool head_dim_ok(int hd) { return hd == 8 || hd == 16 || hd == 32 || hd == 64 || hd == 128 || hd == 256; }
 
@@ -963,8 +963,14 @@ int32_t kv_attention_forward_cached(kv_cache_t* c, int32_t first, int32_t n_seq,
   if (rc != MOE_OK) return rc;
   if (!q || !k || !v || !merged) return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: empty step or null buffer");
   if ((rc = check_room(c, first, n_seq, rows)) != MOE_OK) return rc;
+  // what the kernels load of a query at once: eight channels, on the tensor cores two; a 4-bit cache takes the channels one by one where it has to
+  const bool is_q4 = g.precision == MOE_PRECISION_Q4, pairs = g.precision == MOE_PRECISION_BF16 && takes_tc_path<bf16>(g.head_dim);
+  const size_t elem = elem_size(c), query = is_q4 ? elem : pairs ? 4 : 16;
+  auto off = [](const void* p, size_t boundary) { return reinterpret_cast<uintptr_t>(p) % boundary != 0; };
+  if (off(q, query) || off(k, elem) || off(v, elem) || off(merged, elem))
+    return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: q starts off a boundary of %zu bytes, or k, v or the result off one of %zu", query, elem);
   KCK(cudaSetDevice(g.device));
-  if (g.precision == MOE_PRECISION_Q4) return forward_q4(c, first, n_seq, q, k, v, rows, merged, (cudaStream_t)stream);
+  if (is_q4) return forward_q4(c, first, n_seq, q, k, v, rows, merged, (cudaStream_t)stream);
   return g.precision == MOE_PRECISION_BF16 ? forward_t<bf16>(c, first, n_seq, q, k, v, rows, merged, (cudaStream_t)stream)
                                            : forward_t<float>(c, first, n_seq, q, k, v, rows, merged, (cudaStream_t)stream);
 }

@@ -514,3 +514,25 @@ def test_out_has_any_shape(precision):
         with pytest.raises(InvalidInput):
             caches[0].forward_cached(q, k, v, rows_per_sequence=rows, out=bad)
     assert caches[0].lengths() == [rows] * S
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("precision,hd,off,ok", [("bf16", 64, 1, False), ("bf16", 64, 2, True), ("bf16", 32, 2, False), ("bf16", 32, 8, True), ("f32", 64, 1, False),
+                                                 ("f32", 64, 4, True), ("q4", 64, 1, True), ("q4", 64, 3, True)])
+def test_queries_off_their_boundary(precision, hd, off, ok):
+    """The kernels of the older caches load several channels of a query at once; where those would straddle a boundary the call is refused."""
+    H, Hkv = 4, 2
+    dt = torch.float32 if precision == "f32" else torch.bfloat16
+    cache, other = (KvCache(2, H, Hkv, hd, 8, precision=precision) for _ in range(2))
+    q, k, v = (torch.from_numpy(a).cuda().to(dt) for a in _rows(2, H, Hkv, hd, 91))
+    flat = torch.zeros(q.numel() + 16, device="cuda", dtype=dt)
+    moved = flat[off:off + q.numel()].view(q.shape)
+    moved.copy_(q)
+    if ok:
+        odd = torch.zeros(k.numel() + 1, device="cuda", dtype=dt)[1:].view(k.shape)     # keys and values are taken one by one
+        odd.copy_(k)
+        assert torch.equal(cache.forward_cached(moved, odd, v), other.forward_cached(q, k, v))
+    else:
+        with pytest.raises(InvalidInput, match="boundary"):
+            cache.forward_cached(moved, k, v)
+        assert cache.lengths() == [0, 0]
