@@ -89,7 +89,7 @@ inline bool rows_overlap(const void* a, long long a_ld, const void* b, long long
     const long long from = at + i * a_ld - bt, to = from + a_bytes;     // the row, counted from b
     if (to <= 0) continue;
     // the first row of b that ends behind `from`: it is the one that begins first of those
-    const long long j = from < b_bytes ? 0 : (from - b_bytes) / b_ld + 1;
+    const long long j = from < b_bytes ? 0 : rows > 1 ? (from - b_bytes) / b_ld + 1 : 1;
     if (j < rows && j * b_ld < to) return true;
     if (rows > 1 && a_ld == b_ld && i > 0) break;                       // the further rows lie alike
   }

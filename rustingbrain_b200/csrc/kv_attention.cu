@@ -969,6 +969,12 @@ int32_t kv_attention_forward_cached(kv_cache_t* c, int32_t first, int32_t n_seq,
   auto off = [](const void* p, size_t boundary) { return reinterpret_cast<uintptr_t>(p) % boundary != 0; };
   if (off(q, query) || off(k, elem) || off(v, elem) || off(merged, elem))
     return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: q starts off a boundary of %zu bytes, or k, v or the result off one of %zu", query, elem);
+  if (is_q4) {   // one launch may read new rows and write results
+    const long long all = (long long)n_seq * rows, heads = (long long)g.num_heads * g.head_dim * 2, kv = (long long)g.kv_heads * g.head_dim * 2;
+    if ((merged != q && rows_overlap(merged, 0, q, 0, all * heads, all * heads, 1)) || rows_overlap(merged, 0, k, 0, all * heads, all * kv, 1) ||
+        rows_overlap(merged, 0, v, 0, all * heads, all * kv, 1))
+      return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: the result overlaps q without being in its place, or k or v");
+  }
   KCK(cudaSetDevice(g.device));
   if (is_q4) return forward_q4(c, first, n_seq, q, k, v, rows, merged, (cudaStream_t)stream);
   return g.precision == MOE_PRECISION_BF16 ? forward_t<bf16>(c, first, n_seq, q, k, v, rows, merged, (cudaStream_t)stream)

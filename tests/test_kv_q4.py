@@ -536,3 +536,25 @@ def test_queries_off_their_boundary(precision, hd, off, ok):
         with pytest.raises(InvalidInput, match="boundary"):
             cache.forward_cached(moved, k, v)
         assert cache.lengths() == [0, 0]
+
+
+@pytest.mark.gpu
+def test_a_result_on_top_of_what_a_4_bit_step_reads_is_refused():
+    H, Hkv, hd, S = 4, 2, 64, 2
+    cache, other = (KvCache(S, H, Hkv, hd, 8, precision="q4") for _ in range(2))
+    q, k, v = (_dev(a) for a in _rows(S, H, Hkv, hd, 95))
+    n, w = q.numel(), k.numel()
+    flat = torch.zeros(2 * n + 2 * w, device="cuda").bfloat16()
+    at = {"q": 0, "k": n, "v": n + w, "free": n + 2 * w}
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        flat[at[name]:at[name] + t.numel()] = t.view(-1)
+    view = lambda start, t: flat[start:start + t.numel()].view(t.shape)
+    args = view(0, q), view(n, k), view(n + w, v)
+    for start in (8, n // 2, n, n + w - 8, n + w, n + 2 * w - 1):
+        with pytest.raises(InvalidInput, match="overlaps"):
+            cache.forward_cached(*args, out=view(start, q))
+    assert cache.lengths() == [0] * S
+    want = other.forward_cached(q, k, v)
+    assert torch.equal(cache.forward_cached(*args, out=view(n + 2 * w, q)), want)      # right behind them
+    cache.rollback(1)
+    assert torch.equal(cache.forward_cached(*args, out=args[0]), want)
