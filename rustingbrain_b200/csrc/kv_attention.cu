@@ -804,13 +804,13 @@ int forward_q4(kv_cache* c, int first, int n_seq, const void* q, const void* k, 
   return MOE_OK;
 }
 
-// The checks that every call with new rows makes.
-int check_step(kv_cache* c, int first, int n_seq, int rows) {
+// The checks of a range and its rows.  A call that launches `per_row` CTAs for each row (0: none) has so many rows at most.
+int check_step(kv_cache* c, int first, int n_seq, int rows, int per_row) {
   const kv_cache_config_t& g = c->cfg;
   if (first < 0 || n_seq <= 0 || n_seq > g.sequences - first)
     return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: sequences %d .. %lld of %d", first, (long long)first + n_seq - 1, g.sequences);
   if (rows <= 0) return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: empty step or null buffer");
-  if ((long long)n_seq * rows * g.num_heads > 0x7fffffffll) return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: too many rows");
+  if ((long long)n_seq * rows > (per_row > 0 ? 0x7fffffffll / per_row : 0x7fffffffffffffffll)) return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: too many rows");
   return MOE_OK;
 }
 int check_room(kv_cache* c, int first, int n_seq, int rows) {
@@ -959,7 +959,7 @@ int32_t kv_attention_forward_cached(kv_cache_t* c, int32_t first, int32_t n_seq,
                                     int32_t rows, void* merged, void* stream) {
   if (!c) return MOE_INVALID_INPUT;
   const kv_cache_config_t& g = c->cfg;
-  int rc = check_step(c, first, n_seq, rows);
+  int rc = check_step(c, first, n_seq, rows, g.num_heads);
   if (rc != MOE_OK) return rc;
   if (!q || !k || !v || !merged) return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: empty step or null buffer");
   if ((rc = check_room(c, first, n_seq, rows)) != MOE_OK) return rc;
@@ -984,7 +984,7 @@ int32_t kv_attention_forward_cached(kv_cache_t* c, int32_t first, int32_t n_seq,
 int32_t kv_cache_append(kv_cache_t* c, int32_t first, int32_t n_seq, const void* k, const void* v, int32_t rows, void* stream) {
   if (!c) return MOE_INVALID_INPUT;
   const kv_cache_config_t& g = c->cfg;
-  int rc = check_step(c, first, n_seq, rows);
+  int rc = check_step(c, first, n_seq, rows, g.kv_heads);
   if (rc != MOE_OK) return rc;
   if (!k || !v) return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: empty step or null buffer");
   if ((rc = check_room(c, first, n_seq, rows)) != MOE_OK) return rc;
@@ -1008,7 +1008,7 @@ int32_t kv_cache_append(kv_cache_t* c, int32_t first, int32_t n_seq, const void*
 
 int32_t kv_cache_rollback(kv_cache_t* c, int32_t first, int32_t n_seq, int32_t rows, void* stream) {
   if (!c) return MOE_INVALID_INPUT;
-  const int rc = check_step(c, first, n_seq, rows);
+  const int rc = check_step(c, first, n_seq, rows, 0);
   if (rc != MOE_OK) return rc;
   for (int i = 0; i < n_seq; ++i)
     if (c->host_len[first + i] < rows)
@@ -1022,7 +1022,7 @@ int32_t kv_cache_rollback(kv_cache_t* c, int32_t first, int32_t n_seq, int32_t r
 int32_t kv_cache_newest(kv_cache_t* c, int32_t first, int32_t n_seq, int32_t rows, float* keys, float* values, void* stream) {
   if (!c) return MOE_INVALID_INPUT;
   const kv_cache_config_t& g = c->cfg;
-  const int rc = check_step(c, first, n_seq, rows);
+  const int rc = check_step(c, first, n_seq, rows, 1);
   if (rc != MOE_OK) return rc;
   if (!keys || !values) return kv_fail(c, MOE_INVALID_INPUT, "InvalidInput: null buffer");
   for (int i = 0; i < n_seq; ++i)

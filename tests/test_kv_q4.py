@@ -558,3 +558,15 @@ def test_a_result_on_top_of_what_a_4_bit_step_reads_is_refused():
     assert torch.equal(cache.forward_cached(*args, out=view(n + 2 * w, q)), want)      # right behind them
     cache.rollback(1)
     assert torch.equal(cache.forward_cached(*args, out=args[0]), want)
+
+
+@pytest.mark.gpu
+def test_rollback_of_more_rows_than_queries_would_be_allowed():
+    """256 sequences of 140000 positions take back 135000 each: with 64 query heads that is past 31 bits, but no query is asked."""
+    S, n = 256, 140000
+    cache = KvCache(S, 64, 1, 32, capacity=n, precision="q4")
+    k = torch.ones(128 * 70000, 32, device="cuda").bfloat16()
+    for half in (0, 0, 1, 1):
+        cache.append(k, k, rows_per_sequence=70000, first_sequence=128 * half, n_sequences=128)
+    cache.rollback(135000)
+    assert cache.lengths() == [5000] * S
