@@ -38,6 +38,7 @@
 #include <cfloat>
 
 #include "kv_q4.cuh"
+#include "warp_ops.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -51,11 +52,6 @@ constexpr float HUGE_VALUE = 1.099511627776e12f; // 2^40: a larger number counts
 constexpr int RAW = 133;                        // bits 0 .. 7 of a bf16 are worth bits * 2^-RAW
 constexpr int STEP_UP = 90;                     // value steps are kept times 2^STEP_UP against raw codes
 constexpr int RAW_HALF = 24, Q_TOP = 13;        // bits 0 .. 7 of an f16: bits * 2^-24; a query's largest channel is in [2^13, 2^14) there
-__host__ __device__ constexpr float pow2(int e) {
-  float v = 1.f;
-  for (int i = 0; i < (e < 0 ? -e : e); ++i) v *= e < 0 ? 0.5f : 2.f;
-  return v;
-}
 // whether a value's code weighs 16 in its word
 __host__ __device__ inline int value_heavy(int p) { return (p >> 3) & 1; }
 
@@ -208,11 +204,6 @@ __global__ void __launch_bounds__(Append<HD>::WARPS * 32) append_kernel(Cache c,
 }
 
 // ---- attention ----
-__device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 // f16 operands; the second one from zero
 __device__ __forceinline__ void mma16816_half(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -221,12 +212,6 @@ __device__ __forceinline__ void mma16816_half(float* c, uint32_t a0, uint32_t a1
 }
 __device__ __forceinline__ void mma16816_half_new(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
-}
-// bf16 operands from zero
-__device__ __forceinline__ void mma16816_new(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
@@ -239,37 +224,8 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-__device__ __forceinline__ void copy16(uint32_t smem, const void* gmem) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
-}
-__device__ __forceinline__ float ex2(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-// two f32 lanes in one instruction
-__device__ __forceinline__ uint64_t pack2(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
 
-// codes i and i + 4 of a word as raw bf16 or f16 numbers, of weight 16 where i is odd
-template <int I>
-__device__ __forceinline__ uint32_t raw_pair(uint32_t w) { return (I < 2 ? w : w >> 8) & (I & 1 ? 0x00f000f0u : 0x000f000fu); }
-__device__ __forceinline__ __nv_bfloat162 as_pair(uint32_t v) { return *reinterpret_cast<const __nv_bfloat162*>(&v); }
-__device__ __forceinline__ uint32_t as_bits(__nv_bfloat162 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+// codes i and i + 4 of a word, raw bf16 or f16 numbers as raw_pair cuts them out,
 // ... and as values times 2^(STEP_UP - RAW); base has that factor already
 template <int I>
 __device__ __forceinline__ uint32_t value_pair(uint32_t w, uint32_t step, uint32_t base) {

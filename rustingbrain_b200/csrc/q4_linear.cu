@@ -32,6 +32,7 @@
 #include "../../include/moe_b200.h"
 #include "../../include/q4_linear_b200.h"
 #include "common.cuh"
+#include "warp_ops.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -41,11 +42,6 @@ namespace {
 constexpr int QL_MAX_WARPS = 16;
 constexpr int QL_MAX_IN = 1 << 16;       // a row of f32 activations, cut over a cluster, fits shared memory
 constexpr int QL_CODE = 6;               // operands are codes times 2^-QL_CODE
-__host__ __device__ constexpr float ql_pow2(int e) {
-  float v = 1.f;
-  for (int i = 0; i < (e < 0 ? -e : e); ++i) v *= e < 0 ? 0.5f : 2.f;
-  return v;
-}
 
 // A unit: 32 outputs and 128 channels, codes [2 output blocks][2 channel blocks][512 bytes], then scales [2][128 / group][8][2] bf16.
 constexpr int QL_CHANNELS = 128, QL_CODES = 2048;
@@ -131,27 +127,11 @@ __global__ void ql_dequantize_kernel(const unsigned char* __restrict__ packed, f
 }
 
 // ---- the product ----
-__device__ __forceinline__ void ql_mma_bf16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// the same from zero
-__device__ __forceinline__ void ql_mma_bf16_new(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
-}
-__device__ __forceinline__ void ql_copy16(uint32_t smem, const void* gmem) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
-}
-__device__ __forceinline__ __nv_bfloat162 ql_pair(uint32_t v) { return *reinterpret_cast<const __nv_bfloat162*>(&v); }
 // codes i and i + 4 of a word, times 2^-QL_CODE; exact
 template <int I>
 __device__ __forceinline__ uint32_t ql_codes(uint32_t w) {
-  const uint32_t bits = (I < 2 ? w : w >> 8) & (I & 1 ? 0x00f000f0u : 0x000f000fu);      // (code + 8) * 2^-133, times 16 where I is odd
-  const __nv_bfloat162 r = __hfma2(ql_pair(bits), __float2bfloat162_rn(ql_pow2(133 - QL_CODE - (I & 1 ? 4 : 0))), __float2bfloat162_rn(-8.f * ql_pow2(-QL_CODE)));
-  return *reinterpret_cast<const uint32_t*>(&r);
+  constexpr float by = pow2(133 - QL_CODE - (I & 1 ? 4 : 0)), eight = 8 * pow2(-QL_CODE);      // what was cut out is (code + 8) * 2^-133, or 16 times that
+  return as_bits(__hfma2(as_pair(raw_pair<I>(w)), __float2bfloat162_rn(by), __float2bfloat162_rn(-eight)));
 }
 
 // Eight activations as they are loaded, and as operands.
@@ -232,8 +212,8 @@ q4_linear_kernel(const T* __restrict__ x, long long ld_x, const unsigned char* _
   auto issue = [&] {
     if (next_pair < s.pairs) {
 #pragma unroll
-      for (int i = 0; i < QL_CODES; i += 512) ql_copy16(next_dst + i, next_src + i);
-      if (lane < (BYTES - QL_CODES) / 16) ql_copy16(next_dst + QL_CODES, next_src + QL_CODES);
+      for (int i = 0; i < QL_CODES; i += 512) copy16(next_dst + i, next_src + i);
+      if (lane < (BYTES - QL_CODES) / 16) copy16(next_dst + QL_CODES, next_src + QL_CODES);
       next_unit += wk_count;
       next_src += wk_count * BYTES;
       if (next_unit >= uend) {
@@ -337,9 +317,9 @@ q4_linear_kernel(const T* __restrict__ x, long long ld_x, const unsigned char* _
               const uint4 b = *reinterpret_cast<const uint4*>(mine[n] + q * plane + off);
 #pragma unroll
               for (int m = 0; m < 2; ++m) {
-                if (opens && q == 0) ql_mma_bf16_new(part[m][n], a[m][0], a[m][1], a[m][2], a[m][3], b.x, b.y);
-                else ql_mma_bf16(part[m][n], a[m][0], a[m][1], a[m][2], a[m][3], b.x, b.y);
-                ql_mma_bf16(part[m][n], a[m][4], a[m][5], a[m][6], a[m][7], b.z, b.w);
+                if (opens && q == 0) mma16816_new(part[m][n], a[m][0], a[m][1], a[m][2], a[m][3], b.x, b.y);
+                else mma16816(part[m][n], a[m][0], a[m][1], a[m][2], a[m][3], b.x, b.y);
+                mma16816(part[m][n], a[m][4], a[m][5], a[m][6], a[m][7], b.z, b.w);
               }
             }
           }
@@ -359,8 +339,8 @@ q4_linear_kernel(const T* __restrict__ x, long long ld_x, const unsigned char* _
         float* dst = red + (wk * rows + r) * width + wn * 32 + gid;
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-          dst[16 * m] = acc[m][n][e] * ql_pow2(QL_CODE);
-          dst[16 * m + 8] = acc[m][n][2 + e] * ql_pow2(QL_CODE);
+          dst[16 * m] = acc[m][n][e] * pow2(QL_CODE);
+          dst[16 * m + 8] = acc[m][n][2 + e] * pow2(QL_CODE);
         }
       }
     const int n0 = tile * width;
