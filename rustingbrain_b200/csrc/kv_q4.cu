@@ -18,9 +18,11 @@
 //   values: step and base belong to the position, which is what the product sums over, so they go on before it: one packed bf16
 //           instruction, one rounding of the value to bf16 (2^-8 of it at most).  The weights enter as two bf16 numbers each, so that the value's
 //           is the only rounding of that size before the output's: error against 64 bits 2.3e-3 of the output's rms, 3.3e-3 with one.
-// What bounds it is the issue of those instructions: 148 SMs would have to do a page of 64 x 64 channels every 215 cycles to keep up with HBM.
-// Measured with a rollback behind each step, in a graph: 64 sequences of 4096 positions, 16/4 heads of 64, 26.5 us (bf16 cache: 58 us), of
-// 16384 73 us (0.84 of the copy bandwidth for each further byte); 16 of 0 .. 32767, 32/8 heads of 128, one row 71 us, three rows 117 us,
+// What bounds it: to keep up with HBM, 148 SMs would have to do a page of 64 x 64 channels every 215 cycles, and its instructions take them about as
+// long.  They issue 1.8 to 2.0 of the 4 a cycle that they could, no pipe is busy for more than 41 % of the time: with 8 to 13 warps an SM (the ring
+// and the sums' registers allow no more) it is the warps' waits, for fixed latencies and at a CTA's start and end for one another, that nothing covers.
+// Measured with a rollback behind each step, in a graph: 64 sequences of 4096 positions, 16/4 heads of 64, 26.4 us (bf16 cache: 58 us), of
+// 16384 72.6 us (0.84 of the copy bandwidth for each further byte); 16 of 0 .. 32767, 32/8 heads of 128, one row 71 us, three rows 117 us,
 // where the bytes alone take 51 us; one of 700 8.4 us, one of 32000 12.7 us.
 //
 // Page layout, HD = head_dim, NG = HD / 32:

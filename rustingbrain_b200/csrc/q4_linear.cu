@@ -22,7 +22,9 @@
 // the same order: one launch, no workspace.
 //
 // Measured in a graph: 1 x 1024 -> 2816 3.5 us; 8 x 4096 -> 24576 15.9 us, one row 14.9 us, 16 rows 19.6 us, 64 rows 61.6 us (the bytes: 8.25 us); 64 x
-// 1024 -> 5632 7.8 us; f32 3 x 2048 -> 32003 17.1 us (5.7 us).  What bounds them: see the counters in the table of measurements.
+// 1024 -> 5632 7.8 us; f32 3 x 2048 -> 32003 17.1 us (5.7 us).  The large ones wait: 2.2 instructions a cycle of the 4 that an SM can issue (f32
+// 1.9), no pipe above 44 %, 12 to 16 warps an SM that wait for fixed latencies (1.3 of them for each issue; f32 2.1), loads (0.8) and their turn at
+// the pipes (0.6; f32 1.9, its three products for one keep the tensor cores at 41 %).
 
 #include <cooperative_groups.h>
 #include <algorithm>
