@@ -99,8 +99,8 @@ int32_t kv_cache_append(kv_cache_t* cache, int32_t first_sequence, int32_t n_seq
 
 /* Takes back the newest rows of each sequence of the range (draft tokens that were not accepted).  Unlike kv_cache_truncate it counts from
  * each sequence's own length, on the device, so that a captured step can contain it.  The rows of steps that were skipped for want of room
- * since the last step that was taken are the newest ones: they count first, and taking them back changes nothing else.  A mark that
- * kv_cache_lengths has yet to report does not matter here.  More rows than a sequence holds are InvalidInput. */
+ * since the last step that was taken are the newest ones: they count first, and taking them back changes nothing else, until kv_cache_lengths
+ * has reported the mark; from then on the host knows that they are not there.  More rows than a sequence holds are InvalidInput. */
 int32_t kv_cache_rollback(kv_cache_t* cache, int32_t first_sequence, int32_t n_sequences, int32_t rows_per_sequence, void* stream);
 
 /* The newest rows of each sequence of the range as the cache holds them, into device memory: f32
