@@ -385,9 +385,10 @@ bool ql_sizes_ok(int d_out, int d_in, int group) {
 // How to cut a product with `live` <= NT * 8 rows a pass: of the ways that fit, the one that should be done first.  False: none fits.
 // The estimate is in cycles of an SM and counts what was measured: a unit takes an SM the issue of its instructions (0.17 a cycle for each warp, up to 2.6), its
 // products (2.1 cycles each) or its share of HBM (24 bytes a cycle), whichever is longest, and a warp no less than its latency; a thread takes
-// 20 to 100 instructions for eight activations.  Joining a CTA's only tile takes 1200 cycles, over a cluster 2700 to 3700; each further tile,
-// for which the warps drain and fill again, 3500 and 5000 to 8000.  So a cluster of two pays where it makes rounds fewer: 8 x 4096 -> 24576 f32
-// 25.1 us against 40 without clusters and 29 with four SMs, but 1 x 1024 -> 2816 3.5 us without and 4.6 with two.
+// 20 to 100 instructions for eight activations.  Joining a CTA's only tile takes 1200 cycles, over a cluster 2700 to 3700 and 100 for each part beyond
+// 16 that comes from other SMs (1 x 8192 -> 1024: 32 parts 7.6 us, 64 parts 8.6 us); each further tile, for which the warps drain and fill
+// again, 3500 and 5000 to 8000.  So a cluster of two pays where it makes rounds fewer: 8 x 4096 -> 24576 f32 25.1 us against 40 without clusters
+// and 29 with four SMs, but 1 x 1024 -> 2816 3.5 us without and 4.6 with two.
 template <typename T, int NT, int GROUP>
 bool ql_plan(const QlShape& s, int rows, int live, QlPlan* out) {
   constexpr int P = QlPieces<T>::N, BYTES = ql_unit_bytes(GROUP), SM = 148;
@@ -427,7 +428,8 @@ bool ql_plan(const QlShape& s, int rows, int live, QlPlan* out) {
         const double unit = std::max(p.warps * on_sm * std::max(hbm, std::max(issue / rate, products)), std::max(350.0, 1100.0 / (p.stages - 1)));
         const double fill = 1500 + (double)live * p.slice * 16 / 32 * (P == 1 ? 20 : 100) * on_sm / rate;
         const double waves = (double)((ctas + on_sm * room - 1) / (on_sm * room));
-        const double time = waves * (fill + rounds * each * unit + first[log] + (rounds - 1) * more[log]);
+        const double join = p.cluster > 1 ? 100.0 * std::max(0, p.cluster * p.wk - 16) : 0.0;
+        const double time = waves * (fill + rounds * each * unit + first[log] + join + (rounds - 1) * more[log]);
         if (best < 0 || time < best) { best = time; *out = p; }
       }
     }
